@@ -18,6 +18,8 @@ MATH_FP32_MIRRORED, MATH_3XTF32, MATH_TF32, MATH_TF32_UNBOUNDED, MATH_TF32_U16 =
 MODE_LABELS = {0: "fp32", 1: "3xtf32", 2: "tf32", 4: "tf32-u16"}  # what fc_conv_math_mode / fc_resolve_plan report
 MODE_NAMES = {"fp32": MATH_FP32_MIRRORED, "ffma": MATH_FP32_MIRRORED, "3xtf32": MATH_3XTF32, "tf32": MATH_TF32,
               "tf32-unbounded": MATH_TF32_UNBOUNDED, "tf32-u16": MATH_TF32_U16}
+DTYPE_NAMES = {"fp32": 0, "bf16": 1, "fp16": 2}
+ACT_NAMES = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5}
 ALGO_NAMES = {"auto": ALGO_AUTO, "direct": ALGO_DIRECT, "im2col": ALGO_IM2COL, "winograd": ALGO_WINOGRAD}
 
 
@@ -27,6 +29,20 @@ class ConvDesc(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "batch", "ic", "ih", "iw", "oc", "kh", "kw", "sh", "sw",
         "pad_left", "pad_right", "pad_top", "pad_bottom", "group")]
+
+
+class GroupNormDesc(C.Structure):
+    """fc_group_norm_desc"""
+
+    _fields_ = ([(n, C.c_int32) for n in ("batch", "pixels", "channels", "groups", "type", "param_type", "act")]
+                + [("eps", C.c_float), ("x_stride", C.c_int64), ("y_stride", C.c_int64)])
+
+
+class GatedFfDesc(C.Structure):
+    """fc_gated_ff_desc"""
+
+    _fields_ = ([(n, C.c_int32) for n in ("rows", "in_channels", "hidden", "out_channels", "type", "act")]
+                + [("x_stride", C.c_int64), ("y_stride", C.c_int64)])
 
 
 class FastConvError(RuntimeError):
@@ -128,6 +144,14 @@ SIGNATURES = {
     "fc_sharded_conv_download": (C.c_int, [_vp, _vp]),
     "fc_sharded_conv_forward_host": (C.c_int, [_vp, _vp, _vp]),
     "fc_sharded_conv_time_device": (C.c_int, [_vp, C.c_int, C.c_int, _fp]),
+    "fc_map_to_channels_last": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int]),
+    "fc_map_from_channels_last": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int]),
+    "fc_group_norm_workspace": (C.c_int, [C.POINTER(GroupNormDesc), _szp, _szp]),
+    "fc_group_norm_forward": (C.c_int, [_vp, C.POINTER(GroupNormDesc)] + [_vp] * 7 + [C.c_size_t]),
+    "fc_group_norm_backward": (C.c_int, [_vp, C.POINTER(GroupNormDesc)] + [_vp] * 10 + [C.c_size_t]),
+    "fc_gated_ff_workspace": (C.c_int, [C.POINTER(GatedFfDesc), _szp, _szp]),
+    "fc_gated_ff_forward": (C.c_int, [_vp, C.POINTER(GatedFfDesc)] + [_vp] * 10 + [C.c_size_t]),
+    "fc_gated_ff_backward": (C.c_int, [_vp, C.POINTER(GatedFfDesc)] + [_vp] * 14 + [C.c_size_t]),
     "fc_diff": (C.c_float, [_vp, _vp, C.c_int]),
 }
 

@@ -29,13 +29,17 @@ SOURCES = [
     "fc_static_scratch.cu",
     "fc_peer.cu",
     "fc_comm.cu",
+    "fc_map_move.cu",
+    "fc_group_norm.cu",
+    "fc_gated_ff.cu",
+    "fc_ff_ffma.cu",
 ]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-O2,-Wall,-Wno-unused-function",
-    "-shared", "-cudart", "static", "-ldl",
+    "-shared", "-cudart", "static", "-ldl", "--threads", "0",
 ]
 
 

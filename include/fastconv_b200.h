@@ -389,6 +389,81 @@ int fc_sharded_conv_forward_host(fc_sharded_conv *sc, const float *h_in, float *
  * maximum over all ranks of the mean per forward */
 int fc_sharded_conv_time_device(fc_sharded_conv *sc, int warmup, int iters, float *ms_per_iter);
 
+/* ---- channels-last operators ---------------------------------------------------
+ * No counterpart in the reference, whose operators are convolutions; they are what stands between such layers in
+ * today's image networks.  A channels-last map is [batch][pixels][channels] with `pixels` = height * width: its element
+ * (n, p, c) is at (n * pixels + p) * stride + c, where `stride` (elements from one pixel to the next, 0 = channels)
+ * may be larger than `channels`: a slice of a wider map.  What lies between the channels and the stride is neither
+ * read nor written.
+ *
+ * Every function works on device pointers, asynchronously on the context's stream; the caller's current device is left
+ * as it was.  Addresses and strides need no alignment beyond their element's size (16-byte aligned rows are faster).
+ * Outputs must not overlap inputs or one another.  Sums and statistics are fp32 whatever the type, an output is rounded
+ * once, and no result depends on the order in which blocks run.  The workspace is the caller's (16-byte aligned, of the
+ * bytes that the _workspace function gives for the same descriptor); it holds nothing between calls, but calls
+ * that can overlap on the GPU need one each.  That includes replays of captured graphs: a captured call keeps the
+ * workspace that it was captured with.  Nothing is allocated or synchronised, so every call can be captured. */
+typedef enum fc_dtype { FC_DTYPE_F32 = 0, FC_DTYPE_BF16 = 1, FC_DTYPE_F16 = 2 } fc_dtype;
+typedef enum fc_activation {
+    FC_ACT_NONE = 0,
+    FC_ACT_RELU = 1,      /* max(z, 0), slope 0 at 0; a NaN stays a NaN */
+    FC_ACT_SILU = 2,      /* z / (1 + exp(-z)) */
+    FC_ACT_GELU = 3,      /* z (1 + erf(z / sqrt 2)) / 2 */
+    FC_ACT_GELU_TANH = 4, /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+    FC_ACT_SIGMOID = 5    /* 1 / (1 + exp(-z)) */
+} fc_activation;
+
+/* Between a convolution layer's maps, fp32 [batch][channels][pixels], and channels-last ones of element type `type`
+ * (rounded to nearest on the way in).  Each direction is the gradient of the other. */
+int fc_map_to_channels_last(fc_context *ctx, const float *d_planes, void *d_last, int batch, int channels, int pixels,
+                            int64_t last_stride, int type);
+int fc_map_from_channels_last(fc_context *ctx, const void *d_last, float *d_planes, int batch, int channels, int pixels,
+                              int64_t last_stride, int type);
+
+/* Group norm with an activation: y = act(gamma (x - mean) / sqrt(var + eps) + beta), mean and (biased) variance over the
+ * pixels and the channels/groups channels of a group, per image. */
+typedef struct fc_group_norm_desc {
+    int32_t batch, pixels, channels, groups; /* batch 0: nothing to do (the parameters' gradients are then zero) */
+    int32_t type;                            /* fc_dtype of x, y, dy, dx */
+    int32_t param_type;                      /* fc_dtype of gamma, beta and their gradients: FC_DTYPE_F32 or `type` */
+    int32_t act;                             /* fc_activation */
+    float eps;
+    int64_t x_stride, y_stride; /* of x and dx; of y and dy.  0 = channels */
+} fc_group_norm_desc;
+int fc_group_norm_workspace(const fc_group_norm_desc *desc, size_t *forward_bytes, size_t *backward_bytes);
+/* d_gamma, d_beta: [channels], NULL = 1, 0.  d_mean, d_rstd: fp32 [batch][groups], what the backward pass needs; NULL =
+ * not wanted. */
+int fc_group_norm_forward(fc_context *ctx, const fc_group_norm_desc *desc, const void *d_x, const void *d_gamma,
+                          const void *d_beta, void *d_y, float *d_mean, float *d_rstd, void *d_workspace,
+                          size_t workspace_bytes);
+/* d_dx, d_dgamma, d_dbeta: NULL = not wanted.  x, gamma, beta, mean and rstd are the forward pass's. */
+int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, const void *d_dy, const void *d_x,
+                           const void *d_gamma, const void *d_beta, const float *d_mean, const float *d_rstd, void *d_dx,
+                           void *d_dgamma, void *d_dbeta, void *d_workspace, size_t workspace_bytes);
+
+/* Gated feed-forward block over the rows (pixels of all images) of a channels-last map:
+ *   y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd
+ * with the weights of 1x1 convolutions, contiguous: w_gate, w_up [hidden][in_channels], w_down [out_channels][hidden];
+ * one row is a single token or pixel.  Weights, biases, gradients and maps are of one type; between the kernels the
+ * products of the activation, and in the backward pass the gradients of gate and up, are rounded to that type. */
+typedef struct fc_gated_ff_desc {
+    int32_t rows, in_channels, hidden, out_channels; /* rows 0: nothing to do (the weights' gradients are then zero) */
+    int32_t type;                                    /* fc_dtype */
+    int32_t act;                                     /* fc_activation of the gate */
+    int64_t x_stride, y_stride; /* of x and dx; of y and dy: elements from one row to the next.  0 = their channels */
+} fc_gated_ff_desc;
+int fc_gated_ff_workspace(const fc_gated_ff_desc *desc, size_t *forward_bytes, size_t *backward_bytes);
+/* d_b_gate, d_b_up [hidden], d_b_down [out_channels]: NULL = none.  d_saved: [2][rows][hidden], receives what stands before
+ * the activation (gate, then up) for the backward pass; NULL = not wanted. */
+int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const void *d_x, const void *d_w_gate,
+                        const void *d_w_up, const void *d_w_down, const void *d_b_gate, const void *d_b_up,
+                        const void *d_b_down, void *d_y, void *d_saved, void *d_workspace, size_t workspace_bytes);
+/* Gradients are laid out like what they belong to; each may be NULL = not wanted. */
+int fc_gated_ff_backward(fc_context *ctx, const fc_gated_ff_desc *desc, const void *d_dy, const void *d_x,
+                         const void *d_w_gate, const void *d_w_up, const void *d_w_down, const void *d_saved, void *d_dx,
+                         void *d_dw_gate, void *d_dw_up, void *d_dw_down, void *d_db_gate, void *d_db_up, void *d_db_down,
+                         void *d_workspace, size_t workspace_bytes);
+
 /* ---- error metrics on the host ---------------------------------------------- */
 /* diff(), utility/helper.cpp:74-89: mean |a-b| over the elements with |a-b| > 1e-5 */
 float fc_diff(const float *a, const float *b, int len);
