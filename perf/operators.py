@@ -175,7 +175,7 @@ def prepare(case, seed):
                                                 train=case["train"], ctx=ctx)
             state["y"] = new(x)
             if case["train"]:
-                state["saved"] = torch.empty(2, case["rows"], case["hidden"], device=DEVICE, dtype=x.dtype)
+                state["saved"] = torch.empty(2, case["rows"], case["hidden"], device=DEVICE)  # fp32, whatever the type
                 for name in ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down"):
                     state["d" + name] = None if state[name] is None else new(state[name])
     return state
