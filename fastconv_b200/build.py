@@ -33,6 +33,7 @@ SOURCES = [
     "fc_group_norm.cu",
     "fc_gated_ff.cu",
     "fc_ff_ffma.cu",
+    "fc_ff_tc.cu",
 ]
 
 NVCC_FLAGS = [

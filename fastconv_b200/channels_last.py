@@ -113,7 +113,7 @@ class GatedFeedForward(_Plan):
 
     def forward(self, x: int, y: int, *, w_gate: int, w_up: int, w_down: int, b_gate: int = 0, b_up: int = 0, b_down: int = 0,
                 saved: int = 0) -> None:
-        """`saved`: [2][rows][hidden] that the backward pass will need (0 = not wanted)."""
+        """`saved`: 2 * rows * hidden floats, whatever the type, that the backward pass will need (0 = not wanted)."""
         check(self._ready().fc_gated_ff_forward(self.ctx.handle, self._ref, x, w_gate, w_up, w_down, b_gate, b_up, b_down, y,
                                                 saved, self._workspace, self.workspace_bytes), "fc_gated_ff_forward")
 

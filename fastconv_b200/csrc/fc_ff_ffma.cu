@@ -170,8 +170,11 @@ __global__ void __launch_bounds__(FF_THREADS, 2) ff_ffma_kernel(const FfProduct 
                 if (bias1) u += Elem<T>::load(bias1[n]);
                 act_both_rt(p.act, g, act, slope);
                 ((T *)p.c0)[m * p.ldc + n] = Elem<T>::store(act * u);
-                if (p.gate_out) ((T *)p.gate_out)[m * p.n + n] = Elem<T>::store(g);
-                if (p.up_out) ((T *)p.up_out)[m * p.n + n] = Elem<T>::store(u);
+                if (p.gate) {
+                    const int64_t at = ff_saved_at(m, n, p.m, p.n);
+                    p.gate[at] = g;
+                    p.up[at] = u;
+                }
             }
         } else {
 #pragma unroll
@@ -179,8 +182,8 @@ __global__ void __launch_bounds__(FF_THREADS, 2) ff_ffma_kernel(const FfProduct 
                 const int64_t n = n0 + (j < 4 ? tx * 4 + j : 64 + tx * 4 + j - 4);
                 if (n >= p.n) continue;
                 if (KIND == FF_GATE_BACK) {
-                    const float g = Elem<T>::load(((const T *)p.gate_in)[m * p.n + n]);
-                    const float u = Elem<T>::load(((const T *)p.up_in)[m * p.n + n]);
+                    const int64_t at = ff_saved_at(m, n, p.m, p.n);
+                    const float g = p.gate[at], u = p.up[at];
                     float act, slope;
                     act_both_rt(p.act, g, act, slope);
                     ((T *)p.c0)[m * p.ldc + n] = Elem<T>::store(v[j] * u * slope);

@@ -120,40 +120,6 @@ int block_of(const fc_gated_ff_desc *d, Block *b) {
     return FC_OK;
 }
 
-struct Work {
-    uint8_t *h, *dgu;
-    float *part;
-    size_t part_floats, bytes;
-};
-
-size_t split_floats(int m, int n, int k) {
-    const int s = ff_ffma_splits(m, n, k);
-    return s > 1 ? (size_t)s * m * n : 0;
-}
-
-Work carve(const Block &b, void *base, bool backward) {
-    Carver c = {(uint8_t *)base, 0};
-    const size_t e = dtype_size(b.type), rh = (size_t)b.rows * b.hidden;
-    Work w = {};
-    size_t part = 0;
-    auto at_least = [&](size_t n) { if (n > part) part = n; };
-    w.h = c.take<uint8_t>(rh * e);
-    if (!backward) {
-        at_least(split_floats(b.rows, b.out, b.hidden));
-    } else {
-        w.dgu = c.take<uint8_t>(2 * rh * e);
-        at_least(split_floats(b.rows, b.in, 2 * b.hidden));
-        at_least(split_floats(2 * b.hidden, b.in, b.rows));
-        at_least(split_floats(b.out, b.hidden, b.rows));
-        at_least((size_t)colsum_chunks(b.rows, 2 * b.hidden) * 2 * b.hidden);
-        at_least((size_t)colsum_chunks(b.rows, b.out) * b.out);
-    }
-    w.part = c.take<float>(part);
-    w.part_floats = part;
-    w.bytes = c.used;
-    return w;
-}
-
 FfProduct product(const Block &b, int kind, int m, int n, int k, const void *a, int64_t lda, bool a_by_k, const void *b0,
                   int64_t ldb, bool b_by_k, void *c0, int64_t ldc) {
     FfProduct p = {};
@@ -166,11 +132,66 @@ FfProduct product(const Block &b, int kind, int m, int n, int k, const void *a, 
     return p;
 }
 
-int multiply(fc_context *ctx, FfProduct p, float *part) {
-    if (p.kind == FF_STORE) {
-        p.splits = ff_ffma_splits(p.m, p.n, p.k);
-        p.part = part;
+// the block's FF_STORE products
+FfProduct down_product(const Block &b, const void *h, const void *w_down, const void *bias, void *y) {
+    FfProduct p = product(b, FF_STORE, b.rows, b.out, b.hidden, h, b.hidden, true, w_down, b.hidden, true, y, b.ys);
+    p.bias0 = bias;
+    return p;
+}
+FfProduct dx_product(const Block &b, const void *dgu, const void *w_gate, const void *w_up, void *dx) {
+    FfProduct p = product(b, FF_STORE, b.rows, b.in, 2 * b.hidden, dgu, 2 * (int64_t)b.hidden, true, w_gate, b.in, false, dx, b.xs);
+    p.b1 = w_up;
+    p.b_split = b.hidden;
+    return p;
+}
+FfProduct dw_in_product(const Block &b, const void *dgu, const void *x, void *dw_gate, void *dw_up) {
+    FfProduct p =
+        product(b, FF_STORE, 2 * b.hidden, b.in, b.rows, dgu, 2 * (int64_t)b.hidden, false, x, b.xs, false, dw_gate, b.in);
+    p.c1 = dw_up;
+    p.row_split = b.hidden;
+    return p;
+}
+FfProduct dw_down_product(const Block &b, const void *dy, const void *h, void *dw_down) {
+    return product(b, FF_STORE, b.out, b.hidden, b.rows, dy, b.ys, false, h, b.hidden, false, dw_down, b.hidden);
+}
+
+struct Work {
+    uint8_t *h, *dgu;
+    float *part;
+    size_t bytes;
+};
+
+Work carve(const Block &b, void *base, bool backward) {
+    Carver c = {(uint8_t *)base, 0};
+    const size_t e = dtype_size(b.type), rh = (size_t)b.rows * b.hidden;
+    Work w = {};
+    size_t part = 0;
+    auto at_least = [&](size_t n) { if (n > part) part = n; };
+    auto shares = [&](const FfProduct &p) {  // of either kernel family: which one runs depends on the call's addresses too
+        const int s = ff_ffma_splits(p.m, p.n, p.k);
+        if (s > 1) at_least((size_t)s * p.m * p.n);
+        if (b.type != FC_DTYPE_F32 && p.k > 0) at_least(ff_tc_part_floats(p));
+    };
+    w.h = c.take<uint8_t>(rh * e);
+    if (!backward) {
+        shares(down_product(b, nullptr, nullptr, nullptr, nullptr));
+    } else {
+        w.dgu = c.take<uint8_t>(2 * rh * e);
+        shares(dx_product(b, nullptr, nullptr, nullptr, nullptr));
+        shares(dw_in_product(b, nullptr, nullptr, nullptr, nullptr));
+        shares(dw_down_product(b, nullptr, nullptr, nullptr));
+        at_least((size_t)colsum_chunks(b.rows, 2 * b.hidden) * 2 * b.hidden);
+        at_least((size_t)colsum_chunks(b.rows, b.out) * b.out);
     }
+    w.part = c.take<float>(part);
+    w.bytes = c.used;
+    return w;
+}
+
+int multiply(fc_context *ctx, FfProduct p, float *part) {
+    p.part = part;
+    if (ff_tc_fits(p)) return launch_ff_tc(ctx, p);
+    if (p.kind == FF_STORE) p.splits = ff_ffma_splits(p.m, p.n, p.k);
     FC_PROPAGATE(launch_ff_ffma(ctx, p));
     if (p.splits == 1) return FC_OK;
     return with_type(p.type, [&](auto t) -> int {
@@ -215,12 +236,13 @@ int fc_gated_ff_workspace(const fc_gated_ff_desc *desc, size_t *forward_bytes, s
 
 int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const void *d_x, const void *d_w_gate, const void *d_w_up,
                         const void *d_w_down, const void *d_b_gate, const void *d_b_up, const void *d_b_down, void *d_y,
-                        void *d_saved, void *d_workspace, size_t workspace_bytes) {
+                        float *d_saved, void *d_workspace, size_t workspace_bytes) {
     FC_REQUIRE(ctx != nullptr, FC_ERR_INVALID_ARG, "context is NULL");
     Block b;
     FC_PROPAGATE(block_of(desc, &b));
     if (b.rows == 0) return FC_OK;
-    FC_PROPAGATE(check_pointers(b, {d_x, d_w_gate, d_w_up, d_w_down, d_y}, {d_b_gate, d_b_up, d_b_down, d_saved}));
+    FC_PROPAGATE(check_pointers(b, {d_x, d_w_gate, d_w_up, d_w_down, d_y}, {d_b_gate, d_b_up, d_b_down}));
+    FC_REQUIRE((uintptr_t)d_saved % 4 == 0, FC_ERR_INVALID_ARG, "the saved values' address is no multiple of 4");
     const Work w = carve(b, d_workspace, false);
     FC_PROPAGATE(check_workspace(d_workspace, workspace_bytes, w.bytes));
     DeviceScope dev(ctx->device);
@@ -229,52 +251,37 @@ int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const voi
     p.b1 = d_w_up;
     p.bias0 = d_b_gate;
     p.bias1 = d_b_up;
-    p.gate_out = d_saved;
-    p.up_out = d_saved ? (uint8_t *)d_saved + (size_t)b.rows * b.hidden * dtype_size(b.type) : nullptr;
+    p.gate = d_saved;
+    p.up = d_saved ? d_saved + (size_t)b.rows * b.hidden : nullptr;
     FC_PROPAGATE(multiply(ctx, p, nullptr));
-    p = product(b, FF_STORE, b.rows, b.out, b.hidden, w.h, b.hidden, true, d_w_down, b.hidden, true, d_y, b.ys);
-    p.bias0 = d_b_down;
-    return multiply(ctx, p, w.part);
+    return multiply(ctx, down_product(b, w.h, d_w_down, d_b_down, d_y), w.part);
 }
 
 int fc_gated_ff_backward(fc_context *ctx, const fc_gated_ff_desc *desc, const void *d_dy, const void *d_x, const void *d_w_gate,
-                         const void *d_w_up, const void *d_w_down, const void *d_saved, void *d_dx, void *d_dw_gate,
+                         const void *d_w_up, const void *d_w_down, const float *d_saved, void *d_dx, void *d_dw_gate,
                          void *d_dw_up, void *d_dw_down, void *d_db_gate, void *d_db_up, void *d_db_down, void *d_workspace,
                          size_t workspace_bytes) {
     FC_REQUIRE(ctx != nullptr, FC_ERR_INVALID_ARG, "context is NULL");
     Block b;
     FC_PROPAGATE(block_of(desc, &b));
     if (b.rows > 0) FC_PROPAGATE(check_pointers(b, {d_dy, d_x, d_w_gate, d_w_up, d_w_down, d_saved}, {}));
+    FC_REQUIRE((uintptr_t)d_saved % 4 == 0, FC_ERR_INVALID_ARG, "the saved values' address is no multiple of 4");
     FC_PROPAGATE(check_pointers(b, {}, {d_dx, d_dw_gate, d_dw_up, d_dw_down, d_db_gate, d_db_up, d_db_down}));
     const Work w = carve(b, d_workspace, true);
     FC_PROPAGATE(check_workspace(d_workspace, workspace_bytes, w.bytes));
     DeviceScope dev(ctx->device);
     FC_CHECK_CUDA(dev.status());
     const int64_t two = 2 * (int64_t)b.hidden;
-    FfProduct p;
     if (b.rows > 0) {
-        p = product(b, FF_GATE_BACK, b.rows, b.hidden, b.out, d_dy, b.ys, true, d_w_down, b.hidden, false, w.dgu, two);
-        p.gate_in = d_saved;
-        p.up_in = (const uint8_t *)d_saved + (size_t)b.rows * b.hidden * dtype_size(b.type);
+        FfProduct p = product(b, FF_GATE_BACK, b.rows, b.hidden, b.out, d_dy, b.ys, true, d_w_down, b.hidden, false, w.dgu, two);
+        p.gate = const_cast<float *>(d_saved);
+        p.up = p.gate + (size_t)b.rows * b.hidden;
         p.c1 = w.h;
         FC_PROPAGATE(multiply(ctx, p, nullptr));
-        if (d_dx) {
-            p = product(b, FF_STORE, b.rows, b.in, (int)two, w.dgu, two, true, d_w_gate, b.in, false, d_dx, b.xs);
-            p.b1 = d_w_up;
-            p.b_split = b.hidden;
-            FC_PROPAGATE(multiply(ctx, p, w.part));
-        }
+        if (d_dx) FC_PROPAGATE(multiply(ctx, dx_product(b, w.dgu, d_w_gate, d_w_up, d_dx), w.part));
     }
-    if (d_dw_gate || d_dw_up) {
-        p = product(b, FF_STORE, (int)two, b.in, b.rows, w.dgu, two, false, d_x, b.xs, false, d_dw_gate, b.in);
-        p.c1 = d_dw_up;
-        p.row_split = b.hidden;
-        FC_PROPAGATE(multiply(ctx, p, w.part));
-    }
-    if (d_dw_down) {
-        p = product(b, FF_STORE, b.out, b.hidden, b.rows, d_dy, b.ys, false, w.h, b.hidden, false, d_dw_down, b.hidden);
-        FC_PROPAGATE(multiply(ctx, p, w.part));
-    }
+    if (d_dw_gate || d_dw_up) FC_PROPAGATE(multiply(ctx, dw_in_product(b, w.dgu, d_x, d_dw_gate, d_dw_up), w.part));
+    if (d_dw_down) FC_PROPAGATE(multiply(ctx, dw_down_product(b, d_dy, w.h, d_dw_down), w.part));
     if (d_db_gate || d_db_up)
         FC_PROPAGATE(colsum(ctx, b.type, w.dgu, two, b.rows, (int)two, b.hidden, d_db_gate, d_db_up, w.part));
     if (d_db_down) FC_PROPAGATE(colsum(ctx, b.type, d_dy, b.ys, b.rows, b.out, b.out, d_db_down, nullptr, w.part));

@@ -25,16 +25,34 @@ struct FfProduct {
     int b_split;  // !b_by_k: rows k >= b_split come from b1, at k - b_split.  k where there is one matrix
     void *c0, *c1;
     int64_t ldc;
-    int row_split;             // FF_STORE: m where there is one destination.  A null destination is not stored to
+    int row_split;             // FF_STORE: m where there is one destination.  A null destination is not computed
     const void *bias0, *bias1; // one value a column, or null
-    const void *gate_in, *up_in;  // FF_GATE_BACK: [m][n]
-    void *gate_out, *up_out;      // FF_GATE: [m][n], or null
+    float *gate, *up;          // what stands before the activation: written by FF_GATE (null: not wanted), read by FF_GATE_BACK
     float *part;               // FF_STORE with splits > 1: [splits][m][n]
     int splits;
 };
 
+// Where the saved value of row m, column n lies in the gate's or the up projection's share of `saved`: [rows][n] in fp32, in
+// blocks of 32 rows that are ordered [4 columns][row][column], so that a warp whose lanes are rows moves 16 bytes a lane to
+// neighbouring addresses.  The last block has fewer rows; plain rows where n is no multiple of 4.
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline int64_t ff_saved_at(int64_t m, int64_t n, int64_t rows, int64_t cols) {
+    if (cols % 4) return m * cols + n;
+    const int64_t block = m / 32 * 32, in_block = rows - block < 32 ? rows - block : 32;
+    return block * cols + ((n >> 2) * in_block + (m - block)) * 4 + (n & 3);
+}
+
 int launch_ff_ffma(fc_context *ctx, const FfProduct &p);
 // shares of the reduction for an FF_STORE product, so that few output tiles still occupy the GPU
 int ff_ffma_splits(int m, int n, int k);
+
+struct FfTcPlan {
+    int bn, splits;
+};
+bool ff_tc_fits(const FfProduct &p);
+size_t ff_tc_part_floats(const FfProduct &p);  // what p.part has to hold
+int launch_ff_tc(fc_context *ctx, const FfProduct &p);
 
 }  // namespace fc

@@ -445,7 +445,7 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
  *   y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd
  * with the weights of 1x1 convolutions, contiguous: w_gate, w_up [hidden][in_channels], w_down [out_channels][hidden];
  * one row is a single token or pixel.  Weights, biases, gradients and maps are of one type; between the kernels the
- * products of the activation, and in the backward pass the gradients of gate and up, are rounded to that type. */
+ * products act(.) * (.), and in the backward pass the gradients of gate and up, are rounded to that type. */
 typedef struct fc_gated_ff_desc {
     int32_t rows, in_channels, hidden, out_channels; /* rows 0: nothing to do (the weights' gradients are then zero) */
     int32_t type;                                    /* fc_dtype */
@@ -453,14 +453,14 @@ typedef struct fc_gated_ff_desc {
     int64_t x_stride, y_stride; /* of x and dx; of y and dy: elements from one row to the next.  0 = their channels */
 } fc_gated_ff_desc;
 int fc_gated_ff_workspace(const fc_gated_ff_desc *desc, size_t *forward_bytes, size_t *backward_bytes);
-/* d_b_gate, d_b_up [hidden], d_b_down [out_channels]: NULL = none.  d_saved: [2][rows][hidden], receives what stands before
- * the activation (gate, then up) for the backward pass; NULL = not wanted. */
+/* d_b_gate, d_b_up [hidden], d_b_down [out_channels]: NULL = none.  d_saved: 2 * rows * hidden floats whatever the type, what the
+ * backward pass needs of the values before the activation (in an order of the library's own); NULL = not wanted. */
 int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const void *d_x, const void *d_w_gate,
                         const void *d_w_up, const void *d_w_down, const void *d_b_gate, const void *d_b_up,
-                        const void *d_b_down, void *d_y, void *d_saved, void *d_workspace, size_t workspace_bytes);
+                        const void *d_b_down, void *d_y, float *d_saved, void *d_workspace, size_t workspace_bytes);
 /* Gradients are laid out like what they belong to; each may be NULL = not wanted. */
 int fc_gated_ff_backward(fc_context *ctx, const fc_gated_ff_desc *desc, const void *d_dy, const void *d_x,
-                         const void *d_w_gate, const void *d_w_up, const void *d_w_down, const void *d_saved, void *d_dx,
+                         const void *d_w_gate, const void *d_w_up, const void *d_w_down, const float *d_saved, void *d_dx,
                          void *d_dw_gate, void *d_dw_up, void *d_dw_down, void *d_db_gate, void *d_db_up, void *d_db_down,
                          void *d_workspace, size_t workspace_bytes);
 

@@ -127,7 +127,6 @@ def ff(t, kind, dtype, dy=None):
     out = {"y": (y, ey), "gate": (g, eg), "up": (u, eu)}
     if dy is None:
         return out
-    eg, eu = eg + half * (g.abs() + eg) + tiny, eu + half * (u.abs() + eu) + tiny  # as saved
     a, d = act(g, kind)
     ea, ed = act_error(g, eg, kind)
     dh, edh = dy @ wd, (dy.shape[1] + 4) * U * mag(dy, wd)

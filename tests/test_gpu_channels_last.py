@@ -244,7 +244,7 @@ def run_ff(ctx, rows, k, f, o, kind, dtype, *, bias=True, xs=0, ys=0, train=True
     t = {"x": x, "w_gate": rnd(f, k, by=scale * k ** -0.5), "w_up": rnd(f, k, by=scale * k ** -0.5), "w_down": rnd(o, f, by=f ** -0.5)}
     for name, size in (("b_gate", f), ("b_up", f), ("b_down", o)):
         t[name] = rnd(size, by=0.2) if bias else None
-    saved = torch.full((2, rows, f), GUARD, dtype=dt, device="cuda") if train else None
+    saved = torch.full((2, rows, f), GUARD, device="cuda") if train else None
     plan = fc.GatedFeedForward(rows, k, f, o, act=kind, dtype=dtype, x_stride=xs, y_stride=ys, train=train, ctx=ctx)
     weights = {n: at(t[n]) for n in ("w_gate", "w_up", "w_down")}
     grads = {"dx": dx}
@@ -261,8 +261,9 @@ def run_ff(ctx, rows, k, f, o, kind, dtype, *, bias=True, xs=0, ys=0, train=True
     check(y, *want["y"], dtype, "y")
     assert guards_hold(fy, rows, o, ys)
     if train:
-        check(saved[0], *want["gate"], dtype, "gate")
-        check(saved[1], *want["up"], dtype, "up")
+        for v, n in zip(saved, ("gate", "up")):  # in an order of the library's own: compared as sets
+            w, e = (q.flatten() for q in want[n])
+            check(v.flatten().sort().values, w.sort().values, e.max().expand_as(w), "fp32", n)
         for n, v in grads.items():
             check(v, *want[n], dtype, n)
         assert guards_hold(fdx, rows, k, xs)
@@ -329,7 +330,7 @@ def test_ff_gradients_one_by_one(lctx, dtype, rows):
     dt = DTYPES[dtype]
     g = gen(21)
     rnd = lambda *s: (0.3 * torch.randn(*s, generator=g)).to(dt).cuda()  # noqa: E731
-    x, dy, saved = rnd(rows, k), rnd(rows, k), rnd(2, rows, f)
+    x, dy, saved = rnd(rows, k), rnd(rows, k), rnd(2, rows, f).float()
     w = {"w_gate": rnd(f, k), "w_up": rnd(f, k), "w_down": rnd(k, f)}
     sizes = {"dx": (rows, k), "dw_gate": (f, k), "dw_up": (f, k), "dw_down": (k, f), "db_gate": (f,), "db_up": (f,), "db_down": (k,)}
     full = {n: torch.full(s, GUARD, dtype=dt, device="cuda") for n, s in sizes.items()}
