@@ -19,20 +19,6 @@ using namespace last;
 
 constexpr int BM = 128, BN = 128, BK = 16, FF_THREADS = 256, PAD = 4;
 
-__device__ __forceinline__ uint64_t twice(float v) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(v));
-    return r;
-}
-__device__ __forceinline__ void fma2(uint64_t &c, uint64_t a, uint64_t b) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
-}
-
 __device__ __forceinline__ void act_both_rt(int act, float z, float &a, float &d) {
     switch (act) {
         case FC_ACT_RELU: return act_both<FC_ACT_RELU, true>(z, a, d);
@@ -52,7 +38,7 @@ __device__ __forceinline__ void load8(const T *row, int64_t at, int64_t end, boo
 #pragma unroll
         for (int i = 0; i < 8; i += VEC) {
             float g[VEC];
-            ((const Vec<T, VEC> *)(row + at + i))->unpack(g);
+            Vec<T, VEC>::load(row + at + i).unpack(g);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) f[i + j] = g[j];
         }
@@ -71,10 +57,10 @@ __global__ void __launch_bounds__(FF_THREADS, 2) ff_ffma_kernel(const FfProduct 
     const long long id = blockIdx.x;
     const int nt = (int)(id % n_tiles);
     const long long rest = id / n_tiles;
-    const int mt = (int)(rest % m_tiles), split = (int)(rest / m_tiles);
+    const int mt = (int)(rest % m_tiles), part = (int)(rest / m_tiles);
     constexpr int N_STEP = KIND == FF_GATE ? BN / 2 : BN;  // output columns of a tile
     const int64_t m0 = (int64_t)mt * BM, n0 = (int64_t)nt * N_STEP;
-    const int64_t k_begin = (int64_t)split * k_share, k_end = min((int64_t)p.k, k_begin + k_share);
+    const int64_t k_begin = (int64_t)part * k_share, k_end = min((int64_t)p.k, k_begin + k_share);
     const T *a = (const T *)p.a, *b0 = (const T *)p.b0, *b1 = (const T *)p.b1;
 
     float ra[8], rb[8];
@@ -117,7 +103,7 @@ __global__ void __launch_bounds__(FF_THREADS, 2) ff_ffma_kernel(const FfProduct 
     };
 
     const int tx = tid & 15, ty = tid >> 4;
-    uint64_t acc[8][4];
+    Pair acc[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -137,11 +123,11 @@ __global__ void __launch_bounds__(FF_THREADS, 2) ff_ffma_kernel(const FfProduct 
             ulonglong2 bl = *(const ulonglong2 *)&Bs[s][k][tx * 4], bh = *(const ulonglong2 *)&Bs[s][k][64 + tx * 4];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint64_t v = twice(av[i]);
-                fma2(acc[i][0], v, bl.x);
-                fma2(acc[i][1], v, bl.y);
-                fma2(acc[i][2], v, bh.x);
-                fma2(acc[i][3], v, bh.y);
+                const Pair v = pair(av[i], av[i]);
+                acc[i][0] = fma2(v, bl.x, acc[i][0]);
+                acc[i][1] = fma2(v, bl.y, acc[i][1]);
+                acc[i][2] = fma2(v, bh.x, acc[i][2]);
+                acc[i][3] = fma2(v, bh.y, acc[i][3]);
             }
         }
         if (more) put(s ^ 1);
@@ -156,7 +142,7 @@ __global__ void __launch_bounds__(FF_THREADS, 2) ff_ffma_kernel(const FfProduct 
         float v[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float2 f = halves(acc[i][j]);
+            const float2 f = split(acc[i][j]);
             v[2 * j] = f.x;
             v[2 * j + 1] = f.y;
         }
@@ -190,7 +176,7 @@ __global__ void __launch_bounds__(FF_THREADS, 2) ff_ffma_kernel(const FfProduct 
                     ((T *)p.c0)[m * p.ldc + p.n + n] = Elem<T>::store(v[j] * act);
                     ((T *)p.c1)[m * p.n + n] = Elem<T>::store(act * u);
                 } else if (p.splits > 1) {
-                    p.part[((int64_t)split * p.m + m) * p.n + n] = v[j];
+                    p.part[((int64_t)part * p.m + m) * p.n + n] = v[j];
                 } else {
                     const bool second = m >= p.row_split;
                     T *c = (T *)(second ? p.c1 : p.c0);

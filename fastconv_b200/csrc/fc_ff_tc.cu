@@ -165,7 +165,7 @@ __device__ __forceinline__ void add_bias(const void *bias, int n, int n_end, flo
     for (int i = 0; i < 4; ++i) {
         if (n + 8 * i >= n_end) break;
         float f[8];
-        ((const Vec<T, 8> *)((const T *)bias + n + 8 * i))->unpack(f);
+        Vec<T, 8>::load((const T *)bias + n + 8 * i).unpack(f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[8 * i + j] += f[j];
     }
@@ -454,11 +454,13 @@ __global__ void __launch_bounds__(256) ff_tc_join_kernel(const FfTc P, T *c0, T 
         }
         if (P.bias0) {
             float b[4];
-            ((const Vec<T, 4> *)((const T *)P.bias0 + 4 * q))->unpack(b);
+            Vec<T, 4>::load((const T *)P.bias0 + 4 * q).unpack(b);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += b[i];
         }
-        ((Vec<T, 4> *)(c + (size_t)row * ldc + 4 * q))->pack(v);
+        Vec<T, 4> out;
+        out.pack(v);
+        out.store(c + (size_t)row * ldc + 4 * q);
     }
 }
 

@@ -9,7 +9,11 @@
 //   M2 = M2a + M2b + (mean_a - mean_b)^2 na nb / (na + nb),
 // so that a level far from zero costs no digits.  No atomics: results are the same from run to run.
 //
-// Three kernels each way: sums of a chunk of pixels per channel; their join per group; the map itself.
+// One kernel where a cluster's shared memory holds an image's block of channels (then a map is read once); otherwise
+// three each way: sums of a chunk of pixels per channel, their join per group, the map itself.
+#include <cooperative_groups.h>
+
+#include <numeric>
 #include <type_traits>
 
 #include "fc_last.cuh"
@@ -51,7 +55,7 @@ __device__ __forceinline__ Place place_of(const NormShape &s) {
     b.chunk = (int)(rest % s.chunks);
     b.img = (int)(rest / s.chunks);
     b.p0 = b.chunk * s.chunk_pixels;
-    b.p1 = min(s.pixels, b.p0 + s.chunk_pixels);
+    b.p1 = b.p0 + min(s.chunk_pixels, s.pixels - b.p0);
     b.rows = NORM_THREADS / s.cols;
     b.row = threadIdx.x / s.cols;
     b.col = threadIdx.x % s.cols;
@@ -96,11 +100,11 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_part_kernel(const T *__rest
     if (b.live) {
         const T *src = x + (size_t)b.img * s.pixels * s.xs + b.c0;
         int p = b.p0 + b.row;
-        if (p < b.p1) ((const Vec<T, VEC> *)(src + (size_t)p * s.xs))->unpack(k);
+        if (p < b.p1) Vec<T, VEC>::load(src + (size_t)p * s.xs).unpack(k);
 #pragma unroll 4
         for (; p < b.p1; p += b.rows, ++n) {
             float f[VEC];
-            ((const Vec<T, VEC> *)(src + (size_t)p * s.xs))->unpack(f);
+            Vec<T, VEC>::load(src + (size_t)p * s.xs).unpack(f);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float d = f[i] - k[i];
@@ -136,15 +140,16 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_join_kernel(const float2 *_
     const float2 *src = part + (size_t)img * s.chunks * s.channels + g * s.cpg;
     const int items = s.chunks * s.cpg;
     const float inv = 1.0f / ((float)s.pixels * (float)s.cpg);
+    const float level = src[0].x;  // means are added as distances from one of them, which costs no digits
     float a = 0.0f;
     for (int i = threadIdx.x; i < items; i += NORM_THREADS) {
-        const int chunk = i / s.cpg, n = min(s.pixels, (chunk + 1) * s.chunk_pixels) - chunk * s.chunk_pixels;
-        a = fmaf(src[(size_t)chunk * s.channels + i % s.cpg].x, (float)n, a);
+        const int chunk = i / s.cpg, n = min(s.chunk_pixels, s.pixels - chunk * s.chunk_pixels);
+        a = fmaf(src[(size_t)chunk * s.channels + i % s.cpg].x - level, (float)n, a);
     }
-    const float m = block_sum(a, scratch) * inv;
+    const float m = fmaf(block_sum(a, scratch), inv, level);
     float q = 0.0f;
     for (int i = threadIdx.x; i < items; i += NORM_THREADS) {
-        const int chunk = i / s.cpg, n = min(s.pixels, (chunk + 1) * s.chunk_pixels) - chunk * s.chunk_pixels;
+        const int chunk = i / s.cpg, n = min(s.chunk_pixels, s.pixels - chunk * s.chunk_pixels);
         const float2 v = src[(size_t)chunk * s.channels + i % s.cpg];
         const float d = v.x - m;
         q += fmaf(d * d, (float)n, v.y);
@@ -178,10 +183,14 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_apply_kernel(const T *__res
 #pragma unroll 4
     for (int p = b.p0 + b.row; p < b.p1; p += b.rows) {
         float f[VEC];
-        ((const Vec<T, VEC> *)(src + (size_t)p * s.xs))->unpack(f);
+        Vec<T, VEC>::load(src + (size_t)p * s.xs).unpack(f);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) f[i] = act_value<ACT, kExact>(fmaf(f[i] - m[i], a[i], o[i]));
-        ((Vec<T, VEC> *)(dst + (size_t)p * s.ys))->pack(f);
+        {
+            Vec<T, VEC> out;
+            out.pack(f);
+            out.store(dst + (size_t)p * s.ys);
+        }
     }
 }
 
@@ -233,8 +242,8 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_part_kernel(const T *_
 #pragma unroll 2
         for (int p = b.p0 + b.row; p < b.p1; p += b.rows) {
             float f[VEC], d[VEC];
-            ((const Vec<T, VEC> *)(sx + (size_t)p * s.xs))->unpack(f);
-            ((const Vec<T, VEC> *)(sdy + (size_t)p * s.ys))->unpack(d);
+            Vec<T, VEC>::load(sx + (size_t)p * s.xs).unpack(f);
+            Vec<T, VEC>::load(sdy + (size_t)p * s.ys).unpack(d);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 float dz, xhat;
@@ -307,30 +316,511 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_apply_kernel(const T *
 #pragma unroll 2
     for (int p = b.p0 + b.row; p < b.p1; p += b.rows) {
         float f[VEC], d[VEC];
-        ((const Vec<T, VEC> *)(sx + (size_t)p * s.xs))->unpack(f);
-        ((const Vec<T, VEC> *)(sdy + (size_t)p * s.ys))->unpack(d);
+        Vec<T, VEC>::load(sx + (size_t)p * s.xs).unpack(f);
+        Vec<T, VEC>::load(sdy + (size_t)p * s.ys).unpack(d);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             float dz, xhat;
             ch.template at<ACT>(i, f[i], d[i], dz, xhat);
             f[i] = ch.r[i] * (fmaf(dz, ch.g[i], -t[i].x) - xhat * t[i].y);
         }
-        ((Vec<T, VEC> *)(dst + (size_t)p * s.xs))->pack(f);
+        {
+            Vec<T, VEC> out;
+            out.pack(f);
+            out.store(dst + (size_t)p * s.xs);
+        }
     }
 }
 
-// dgamma[c], dbeta[c]: the images' sums, added in order
+// ---- one kernel: the map stays in shared memory between its statistics and its result ---------------------------------
+//
+// A cluster of 1 to 8 blocks has one image's block of channels (whole groups, whole vectors), each block a share of the
+// pixels, which it copies to shared memory once; sums go through the blocks' shared memory.  A thread reads back only
+// what it copied itself.
+struct Fused {
+    int cb, vectors, rows;  // channels and vectors of a block of channels; threads of one vector column
+    int blocks;             // blocks of channels of an image
+    int cluster, pc;        // blocks of a cluster; pixels of one block
+    int groups, tg;         // groups of a block of channels; threads that add one up
+    int width, per_row;     // channels of a slot of GroupSums, slots of a group in a row
+    size_t smem;
+};
+constexpr int FUSED_THREADS = 256, COPY_GROUPS = 4;
+
+struct FusedPlace {
+    int rank, cblk, img, np, row, col, c0;
+    int g0, j0;  // group of the thread's first channel, counted in the block; that channel's place in it
+    bool live;
+    int64_t p0;
+};
+__device__ __forceinline__ FusedPlace fused_place(const NormShape &s, const Fused &f, int vec) {
+    FusedPlace b;
+    b.rank = blockIdx.x & (f.cluster - 1);  // clusters of 1, 2, 4 or 8
+    b.cblk = blockIdx.x / f.cluster;
+    b.img = blockIdx.y;
+    b.p0 = (int64_t)b.rank * f.pc;
+    b.np = (int)max((int64_t)0, min((int64_t)f.pc, s.pixels - b.p0));
+    b.row = threadIdx.x / f.vectors;
+    b.col = threadIdx.x - b.row * f.vectors;
+    b.live = b.row < f.rows;
+    b.c0 = b.cblk * f.cb + b.col * vec;
+    b.g0 = b.col * vec / s.cpg;
+    b.j0 = b.col * vec - b.g0 * s.cpg;
+    return b;
+}
+// use(i, group of the block that the thread's channel i belongs to)
+template <int VEC, typename F>
+__device__ __forceinline__ void over_groups(const NormShape &s, const FusedPlace &b, F &&use) {
+    int g = b.g0, j = b.j0;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        use(i, g);
+        if (++j == s.cpg) j = 0, ++g;
+    }
+}
+__device__ __forceinline__ void copy16(void *to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// f(begin, end) for each of the thread's COPY_GROUPS parts of its pixels, once the part's copies have landed
+template <typename F>
+__device__ __forceinline__ void as_they_land(int np, int rows, F &&f) {
+    const int part = ((np + rows - 1) / rows + COPY_GROUPS - 1) / COPY_GROUPS * rows;
+    copies_wait<3>();
+    f(0, min(np, part));
+    copies_wait<2>();
+    f(part, min(np, 2 * part));
+    copies_wait<1>();
+    f(2 * part, min(np, 3 * part));
+    copies_wait<0>();
+    f(3 * part, np);
+}
+__device__ __forceinline__ int first_part(int np, int rows) {
+    return min(np, ((np + rows - 1) / rows + COPY_GROUPS - 1) / COPY_GROUPS * rows);
+}
+template <typename F>
+__device__ __forceinline__ void copy_parts(int np, int rows, F &&f) {
+    const int part = ((np + rows - 1) / rows + COPY_GROUPS - 1) / COPY_GROUPS * rows;
+#pragma unroll
+    for (int i = 0; i < COPY_GROUPS; ++i) {
+        f(i * part, i + 1 < COPY_GROUPS ? min(np, (i + 1) * part) : np);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+}
+
+// Block-wide sums per group of what the threads hold per channel.  A thread hands in one value a slot, a slot being its whole
+// vector where a group's channels are whole vectors, else a channel; a group's slots of all rows lie together, so that
+// `tg` neighbouring threads (a power of two) add them without index arithmetic.
+struct GroupSums {
+    int groups, slots, tg;  // groups of the block; slots of a group in all rows; threads to a group
+    int width;              // channels of a slot
+    float *stat, *scratch, *red;  // [planes][rows * cb], [planes][8], [planes][groups]
+    int plane, per_row;
+    template <int VEC>
+    __device__ __forceinline__ void put(const NormShape &s, const FusedPlace &b, int which, const float (&v)[VEC]) const {
+        float *to = stat + which * plane + b.row * per_row;
+        if (width == VEC) {
+            float t = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) t += v[i];
+            to[b.g0 * slots + b.j0 / VEC] = t;
+        } else {
+            int at = b.g0 * slots + b.j0, j = b.j0;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i, ++at) {
+                to[at] = v[i];
+                if (++j == s.cpg) j = 0, at += slots - s.cpg;
+            }
+        }
+    }
+    // red[which * groups + g] for `planes` planes, complete and visible to the block on return
+    template <int PLANES>
+    __device__ __forceinline__ void add() const {
+        __syncthreads();
+        const int l = threadIdx.x & (tg - 1), lane = threadIdx.x & 31;
+        for (int g = threadIdx.x / tg; g < groups || tg > 1; g += FUSED_THREADS / tg) {
+            float t[PLANES];
+#pragma unroll
+            for (int k = 0; k < PLANES; ++k) {
+                t[k] = 0.0f;
+                if (g < groups)
+                    for (int e = l; e < slots; e += tg) t[k] += stat[k * plane + g * slots + e];
+                for (int o = min(tg, 32) / 2; o > 0; o >>= 1) t[k] += __shfl_xor_sync(0xffffffffu, t[k], o);
+                if (tg > 32) {
+                    if (lane == 0) scratch[k * 8 + (threadIdx.x >> 5)] = t[k];
+                } else if (l == 0 && g < groups) {
+                    red[k * groups + g] = t[k];
+                }
+            }
+            if (tg > 1) break;  // then every group has its threads
+        }
+        __syncthreads();
+        if (tg > 32) {
+            if (threadIdx.x < PLANES * groups) {
+                const int k = threadIdx.x / groups, g = threadIdx.x - k * groups;
+                float t = 0.0f;
+                for (int w = 0; w < tg / 32; ++w) t += scratch[k * 8 + g * (tg / 32) + w];
+                red[k * groups + g] = t;
+            }
+            __syncthreads();
+        }
+    }
+};
+
+// The level that deviations are taken from is the mean of the first part of the block's pixels to land, known while the others
+// are on their way: a quarter's mean is within sqrt(3) standard deviations of the whole's, so the squares lose no digits
+// however far the map is from zero.  The blocks of a cluster are joined by `join`.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__restrict__ x, const void *__restrict__ gamma,
+                                                                  const void *__restrict__ beta, T *__restrict__ y,
+                                                                  float *__restrict__ mean, float *__restrict__ rstd,
+                                                                  const NormShape s, const Fused f) {
+    constexpr int VEC = 16 / sizeof(T);
+    constexpr bool kExact = std::is_same<T, float>::value;
+    using V = Vec<T, VEC>;
+    namespace cg = cooperative_groups;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float scratch[2 * 8];
+    V *data = (V *)smem;  // [pc][vectors]
+    GroupSums gs;
+    gs.groups = f.groups;
+    gs.width = f.width;
+    gs.per_row = f.per_row;
+    gs.slots = f.rows * f.per_row;
+    gs.tg = f.tg;
+    gs.plane = f.rows * f.cb;
+    gs.stat = (float *)(data + (size_t)f.pc * f.vectors);
+    gs.scratch = scratch;
+    gs.red = gs.stat + 2 * gs.plane;
+    float2 *share = (float2 *)(gs.red + 2 * gs.groups);  // [groups]: this block's (mean, M2)
+    float2 *total = share + gs.groups;                   // [groups]: (mean, rstd)
+    const FusedPlace b = fused_place(s, f, VEC);
+    V *mine = data + b.row * f.vectors + b.col;
+    const int hop = f.rows * f.vectors;
+    const int first = first_part(b.np, f.rows);  // pixels that the level is taken from
+    pdl_wait();
+    if (b.live) {
+        const T *src = x + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.xs + b.c0;
+        const int64_t src_hop = f.rows * s.xs;
+        V *to = mine;
+        copy_parts(b.np, f.rows, [&](int from, int upto) {
+            for (int p = from + b.row; p < upto; p += f.rows, to += hop, src += src_hop) copy16(to, src);
+        });
+    }
+    float v[VEC], u[VEC];
+    {
+        Pair sum[VEC / 2];
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) sum[i] = 0;
+        copies_wait<COPY_GROUPS - 1>();
+        if (b.live) {
+            const V *at = mine;
+#pragma unroll 2
+            for (int p = b.row; p < first; p += f.rows, at += hop) {
+                Pair q[VEC / 2];
+                unpack_pairs(V::load(at), q);
+#pragma unroll
+                for (int i = 0; i < VEC / 2; ++i) sum[i] = add2(sum[i], q[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) v[2 * i] = split(sum[i]).x, v[2 * i + 1] = split(sum[i]).y;
+            gs.put<VEC>(s, b, 0, v);
+        }
+    }
+    gs.template add<1>();
+    const float first_inv = 1.0f / ((float)first * (float)s.cpg);
+    {
+        Pair level[VEC / 2], sum[VEC / 2], sq[VEC / 2];
+        over_groups<VEC>(s, b, [&](int i, int g) { v[i] = b.live ? -gs.red[g] * first_inv : 0.0f; });
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            level[i] = pair(v[2 * i], v[2 * i + 1]);
+            sum[i] = sq[i] = 0;
+        }
+        const V *at = mine;
+        as_they_land(b.np, f.rows, [&](int from, int upto) {
+            if (!b.live) return;
+#pragma unroll 2
+            for (int p = from + b.row; p < upto; p += f.rows, at += hop) {
+                Pair q[VEC / 2];
+                unpack_pairs(V::load(at), q);
+#pragma unroll
+                for (int i = 0; i < VEC / 2; ++i) {
+                    const Pair d = add2(q[i], level[i]);
+                    sum[i] = add2(sum[i], d);
+                    sq[i] = fma2(d, d, sq[i]);
+                }
+            }
+        });
+        if (b.live) {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                v[2 * i] = split(sum[i]).x, v[2 * i + 1] = split(sum[i]).y;
+                u[2 * i] = split(sq[i]).x, u[2 * i + 1] = split(sq[i]).y;
+            }
+            gs.put<VEC>(s, b, 0, v);
+            gs.put<VEC>(s, b, 1, u);
+        }
+    }
+    const float level = threadIdx.x < gs.groups ? gs.red[threadIdx.x] * first_inv : 0.0f;  // before it is written again
+    gs.template add<2>();
+    if (threadIdx.x < gs.groups) {
+        const float d = gs.red[threadIdx.x], q = gs.red[gs.groups + threadIdx.x], n_inv = 1.0f / ((float)b.np * (float)s.cpg);
+        share[threadIdx.x] = make_float2(fmaf(d, n_inv, level), fmaxf(fmaf(-d * n_inv, d, q), 0.0f));
+    }
+    if (f.cluster > 1)
+        cg::this_cluster().sync();
+    else
+        __syncthreads();
+    if (threadIdx.x < gs.groups) {
+        const int g = threadIdx.x;
+        float n = 0.0f, m = 0.0f, q = 0.0f;
+        for (int r = 0; r < f.cluster; ++r) {
+            const float2 w = f.cluster > 1 ? *cg::this_cluster().map_shared_rank(share + g, r) : share[g];
+            const int np = (int)min((int64_t)f.pc, s.pixels - (int64_t)r * f.pc);
+            join(n, m, q, (float)np, w.x, w.y / s.cpg);
+        }
+        const float rs = 1.0f / sqrtf(q / n + s.eps);
+        total[g] = make_float2(m, rs);
+        const int at = b.img * s.groups + b.cblk * gs.groups + g;
+        if (b.rank == 0 && mean != nullptr) mean[at] = m;
+        if (b.rank == 0 && rstd != nullptr) rstd[at] = rs;
+    }
+    __syncthreads();
+    if (f.cluster > 1) cg::this_cluster().barrier_arrive();
+    if (b.live) {
+        Pair m[VEC / 2], a[VEC / 2], o[VEC / 2];
+        float w[VEC];
+        over_groups<VEC>(s, b, [&](int i, int g) {
+            const float2 t = total[g];
+            u[i] = t.y * param<T>(gamma, b.c0 + i, s.params_f32, 1.0f);
+            v[i] = param<T>(beta, b.c0 + i, s.params_f32, 0.0f);
+            w[i] = -t.x;
+        });
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            m[i] = pair(w[2 * i], w[2 * i + 1]);
+            a[i] = pair(u[2 * i], u[2 * i + 1]);
+            o[i] = pair(v[2 * i], v[2 * i + 1]);
+        }
+        T *dst = y + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.ys + b.c0;
+        const int64_t dst_hop = f.rows * s.ys;
+        const V *at = mine;
+#pragma unroll 2
+        for (int p = b.row; p < b.np; p += f.rows, at += hop, dst += dst_hop) {
+            Pair q[VEC / 2];
+            unpack_pairs(V::load(at), q);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i)
+                q[i] = act_value2<ACT, kExact>(fma2(add2(q[i], m[i]), a[i], o[i]));
+            V out;
+            pack_pairs(out, q);
+            out.store(dst);
+        }
+    }
+    if (f.cluster > 1) cg::this_cluster().barrier_wait();  // the others have read this block's sums
+}
+
+// sums[img * channels + c]: the image's (sum dz, sum dz xhat)
+template <typename T, int ACT>
+__global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T *__restrict__ dy, const T *__restrict__ x,
+                                                                       const void *__restrict__ gamma,
+                                                                       const void *__restrict__ beta,
+                                                                       const float *__restrict__ mean,
+                                                                       const float *__restrict__ rstd, T *__restrict__ dx,
+                                                                       float2 *__restrict__ sums, const NormShape s, const Fused f) {
+    constexpr int VEC = 16 / sizeof(T);
+    using V = Vec<T, VEC>;
+    namespace cg = cooperative_groups;
+    extern __shared__ __align__(16) uint8_t smem[];
+    V *xs = (V *)smem, *ds = xs + (size_t)f.pc * f.vectors;    // [pc][vectors] each
+    float2 *stat = (float2 *)(ds + (size_t)f.pc * f.vectors);  // [rows][cb]: a thread's sums
+    float2 *share = stat + f.rows * f.cb;                      // [cb]: this block's
+    float2 *total = share + f.cb;                              // [cb]: the image's
+    float2 *ab = total + f.cb;                                 // [groups of the block]
+    const FusedPlace b = fused_place(s, f, VEC);
+    const int hop = f.rows * f.vectors, start = b.row * f.vectors + b.col;
+    pdl_wait();
+    if (b.live) {
+        const T *sx = x + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.xs + b.c0;
+        const T *sd = dy + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.ys + b.c0;
+        const int64_t x_hop = f.rows * s.xs, d_hop = f.rows * s.ys;
+        int at = start;
+        copy_parts(b.np, f.rows, [&](int from, int upto) {
+            for (int p = from + b.row; p < upto; p += f.rows, at += hop, sx += x_hop, sd += d_hop) {
+                copy16(xs + at, sx);
+                copy16(ds + at, sd);
+            }
+        });
+    }
+    constexpr bool kExact = std::is_same<T, float>::value;
+    Pair m[VEC / 2], r[VEC / 2], gm[VEC / 2], bt[VEC / 2];  // -mean, rstd, gamma, beta
+    if (b.live) {
+        float fm[VEC], fr[VEC], fg[VEC], fb[VEC];
+        over_groups<VEC>(s, b, [&](int i, int g) {
+            const int at = b.img * s.groups + b.cblk * f.groups + g;
+            fr[i] = rstd[at];
+            fm[i] = -mean[at];
+            fg[i] = param<T>(gamma, b.c0 + i, s.params_f32, 1.0f);
+            fb[i] = param<T>(beta, b.c0 + i, s.params_f32, 0.0f);
+        });
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            m[i] = pair(fm[2 * i], fm[2 * i + 1]);
+            r[i] = pair(fr[2 * i], fr[2 * i + 1]);
+            gm[i] = pair(fg[2 * i], fg[2 * i + 1]);
+            bt[i] = pair(fb[2 * i], fb[2 * i + 1]);
+        }
+    }
+    // dz and xhat of a pair of channels
+    auto one = [&](int i, Pair v, Pair d, Pair &dz, Pair &xhat) {
+        xhat = mul2(add2(v, m[i]), r[i]);
+        Pair a, slope;
+        act_both2<ACT, kExact>(fma2(xhat, gm[i], bt[i]), a, slope);
+        dz = mul2(d, slope);
+    };
+    {
+        Pair s1[VEC / 2], s2[VEC / 2];
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) s1[i] = s2[i] = 0;
+        int at = start;
+        as_they_land(b.np, f.rows, [&](int from, int upto) {
+            if (!b.live) return;
+            for (int p = from + b.row; p < upto; p += f.rows, at += hop) {
+                Pair v[VEC / 2], d[VEC / 2];
+                unpack_pairs(V::load(xs + at), v);
+                unpack_pairs(V::load(ds + at), d);
+#pragma unroll
+                for (int i = 0; i < VEC / 2; ++i) {
+                    Pair dz, xhat;
+                    one(i, v[i], d[i], dz, xhat);
+                    s1[i] = add2(s1[i], dz);
+                    s2[i] = fma2(dz, xhat, s2[i]);
+                }
+            }
+        });
+        if (b.live) {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                const float2 p = split(s1[i]), q = split(s2[i]);
+                stat[b.row * f.cb + b.col * VEC + 2 * i] = make_float2(p.x, q.x);
+                stat[b.row * f.cb + b.col * VEC + 2 * i + 1] = make_float2(p.y, q.y);
+            }
+        }
+    }
+    __syncthreads();
+    // a channel's rows are added by FUSED_THREADS / cb threads, and those by the first
+    const int parts = f.cb >= FUSED_THREADS ? 1 : min(f.rows, FUSED_THREADS / f.cb);
+    if (parts > 1) {
+        const int c = threadIdx.x % f.cb, part = threadIdx.x / f.cb;
+        if (part < parts) {
+            float2 t = make_float2(0.0f, 0.0f);
+            for (int r = part; r < f.rows; r += parts) {
+                const float2 v = stat[r * f.cb + c];
+                t.x += v.x;
+                t.y += v.y;
+            }
+            stat[part * f.cb + c] = t;  // nobody else reads row `part` of this channel
+        }
+        __syncthreads();
+    }
+    for (int c = threadIdx.x; c < f.cb; c += FUSED_THREADS) {
+        float2 t = make_float2(0.0f, 0.0f);
+        for (int r = 0; r < (parts > 1 ? parts : f.rows); ++r) {
+            const float2 v = stat[r * f.cb + c];
+            t.x += v.x;
+            t.y += v.y;
+        }
+        share[c] = t;
+    }
+    if (f.cluster > 1)
+        cg::this_cluster().sync();
+    else
+        __syncthreads();
+    for (int c = threadIdx.x; c < f.cb; c += FUSED_THREADS) {
+        float2 t = make_float2(0.0f, 0.0f);
+        for (int r = 0; r < f.cluster; ++r) {
+            const float2 v = f.cluster > 1 ? *cg::this_cluster().map_shared_rank(share + c, r) : share[c];
+            t.x += v.x;
+            t.y += v.y;
+        }
+        total[c] = t;
+        if (b.rank == 0) sums[(size_t)b.img * s.channels + b.cblk * f.cb + c] = t;
+    }
+    __syncthreads();
+    if (f.cluster > 1) cg::this_cluster().barrier_arrive();
+    if (dx != nullptr) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = f.cb / s.cpg;
+        const float inv = 1.0f / ((float)s.pixels * (float)s.cpg);
+        for (int g = warp; g < groups; g += FUSED_THREADS / 32) {
+            float a = 0.0f, q = 0.0f;
+            for (int i = lane; i < s.cpg; i += 32) {
+                const int c = g * s.cpg + i;
+                const float w = param<T>(gamma, b.cblk * f.cb + c, s.params_f32, 1.0f);
+                a = fmaf(w, total[c].x, a);
+                q = fmaf(w, total[c].y, q);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                a += __shfl_xor_sync(0xffffffffu, a, o);
+                q += __shfl_xor_sync(0xffffffffu, q, o);
+            }
+            if (lane == 0) ab[g] = make_float2(a * inv, q * inv);
+        }
+        __syncthreads();
+        if (b.live) {
+            float fa[VEC], fb[VEC];
+            over_groups<VEC>(s, b, [&](int i, int g) { fa[i] = -ab[g].x, fb[i] = -ab[g].y; });
+            Pair ta[VEC / 2], tb[VEC / 2];
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) ta[i] = pair(fa[2 * i], fa[2 * i + 1]), tb[i] = pair(fb[2 * i], fb[2 * i + 1]);
+            T *dst = dx + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.xs + b.c0;
+            const int64_t dst_hop = f.rows * s.xs;
+            int at = start;
+            for (int p = b.row; p < b.np; p += f.rows, at += hop, dst += dst_hop) {
+                Pair v[VEC / 2], d[VEC / 2];
+                unpack_pairs(V::load(xs + at), v);
+                unpack_pairs(V::load(ds + at), d);
+#pragma unroll
+                for (int i = 0; i < VEC / 2; ++i) {
+                    Pair dz, xhat;
+                    one(i, v[i], d[i], dz, xhat);
+                    v[i] = mul2(r[i], fma2(xhat, tb[i], fma2(dz, gm[i], ta[i])));
+                }
+                V out;
+                pack_pairs(out, v);
+                out.store(dst);
+            }
+        }
+    }
+    if (f.cluster > 1) cg::this_cluster().barrier_wait();
+}
+
+// dgamma[c], dbeta[c]: the images' sums.  32 channels x 8 shares of the images to a block; the shares are added in order.
 template <typename T>
 __global__ void __launch_bounds__(NORM_THREADS) norm_back_params_kernel(const float2 *__restrict__ sums, void *dgamma, void *dbeta,
                                                                        const NormShape s) {
+    __shared__ float2 shares[8][32];
     pdl_wait();
-    const int c = blockIdx.x * NORM_THREADS + threadIdx.x;
-    if (c >= s.channels) return;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
     float2 t = make_float2(0.0f, 0.0f);
-    for (int n = 0; n < s.batch; ++n) {
-        const float2 v = sums[(size_t)n * s.channels + c];
-        t.x += v.x;
-        t.y += v.y;
+    if (c < s.channels)
+#pragma unroll 4
+        for (int n = ty; n < s.batch; n += 8) {
+            const float2 v = sums[(size_t)n * s.channels + c];
+            t.x += v.x;
+            t.y += v.y;
+        }
+    shares[ty][tx] = t;
+    __syncthreads();
+    if (ty > 0 || c >= s.channels) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        t.x += shares[i][tx].x;
+        t.y += shares[i][tx].y;
     }
     if (s.params_f32) {
         if (dgamma) ((float *)dgamma)[c] = t.y;
@@ -375,6 +865,45 @@ void norm_split(NormShape *s, int vec) {
     if (chunks < 1) chunks = 1;
     s->chunk_pixels = (int)(((long long)s->pixels + chunks - 1) / chunks);
     s->chunks = (s->pixels + s->chunk_pixels - 1) / s->chunk_pixels;
+}
+
+// The one-kernel form for vectors of 16 bytes, or false where an image's smallest block of channels is more than eight
+// blocks' shared memory holds.  Chosen by an estimate in nanoseconds: `waves` rounds of blocks of about 2.5 us (3.5 in a
+// cluster), which two or more blocks of an SM overlap; 0.7 us of instructions that a block takes whatever it holds; and the bytes at 6500 a nanosecond, less where the runs of a pixel are
+// short (memory moves 32 bytes, and is quick from 128 on) or where there are fewer blocks than SMs.
+bool fused_plan(const NormShape &s, int esize, bool backward, Fused *best) {
+    const int vec = 16 / esize, arrays = backward ? 2 : 1;
+    if (s.channels % vec || s.batch > 65535) return false;
+    const int unit = std::lcm(s.cpg, vec);  // divides channels, as both do
+    double best_cost = 1e300;
+    const double bytes = (double)s.batch * s.pixels * s.channels * esize * (arrays + 1);
+    for (int k = 1; k * unit <= s.channels; ++k) {
+        const int cb = k * unit, vectors = cb / vec, run = cb * esize;
+        if (vectors > FUSED_THREADS || cb / s.cpg > FUSED_THREADS) break;
+        if (s.channels % cb) continue;
+        for (int cluster = 1; cluster <= 8; cluster *= 2) {
+            Fused f = {cb, vectors, FUSED_THREADS / vectors, s.channels / cb, cluster, (s.pixels + cluster - 1) / cluster, cb / s.cpg, 1, 1, 1, 0};
+            f.width = s.cpg % vec ? 1 : vec;
+            f.per_row = s.cpg / f.width;
+            if (cluster > 1 && (long long)f.pc * (cluster - 1) >= s.pixels) break;  // a block would have no pixels
+            f.smem = (size_t)f.pc * run * arrays + ((size_t)f.rows * cb + 3 * cb) * sizeof(float2);
+            while (2 * f.tg * f.groups <= FUSED_THREADS) f.tg *= 2;
+            if (f.smem > 200 * 1024) continue;
+            const double blocks = (double)s.batch * f.blocks * cluster;
+            double per_sm = 220.0 * 1024 / (f.smem + 1024.0);
+            per_sm = per_sm > 6 ? 6 : (double)(int)per_sm;
+            const double waves = (double)(long long)((blocks + 148 * per_sm - 1) / (148 * per_sm));
+            const double eff = (run >= 128 ? 1.0 : run >= 64 ? 0.85 : run >= 32 ? 0.6 : 0.3) * (blocks < 148 ? blocks / 148 : 1.0) *
+                               (per_sm < 2 ? 0.75 : 1.0);
+            const double cost = waves * (cluster > 1 ? 3500.0 : 2500.0) / (waves > 1 ? per_sm : 1.0) + blocks / 148 * 700.0 +
+                                bytes / (6500.0 * eff);
+            if (cost < best_cost) {
+                best_cost = cost;
+                *best = f;
+            }
+        }
+    }
+    return best_cost < 1e300;
 }
 
 struct NormWork {
@@ -470,6 +999,17 @@ int fc_group_norm_forward(fc_context *ctx, const fc_group_norm_desc *desc, const
     return with_vectors(s, desc->type, {d_x, d_y}, [&](auto t, auto v) -> int {
         using T = decltype(t);
         constexpr int VEC = decltype(v)::value;
+        Fused f;
+        if constexpr (VEC > 1) {
+            if (fused_plan(s, sizeof(T), false, &f))
+                return with_act(desc->act, [&](auto a) -> int {
+                    auto kernel = norm_fused_kernel<T, decltype(a)::value>;
+                    FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+                    FC_CHECK_CUDA(launch_clusters(kernel, dim3(f.blocks * f.cluster, s.batch), FUSED_THREADS, f.cluster, f.smem,
+                                                  ctx->stream, (const T *)d_x, d_gamma, d_beta, (T *)d_y, d_mean, d_rstd, s, f));
+                    return FC_OK;
+                });
+        }
         norm_split(&s, VEC);
         const long long blocks = (long long)s.batch * s.chunks * s.col_tiles;
         FC_REQUIRE(blocks < (1ll << 31), FC_ERR_UNSUPPORTED, "%lld blocks", blocks);
@@ -510,7 +1050,20 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
         const long long blocks = (long long)s.batch * s.chunks * s.col_tiles;
         FC_REQUIRE(blocks < (1ll << 31), FC_ERR_UNSUPPORTED, "%lld blocks", blocks);
         const NormWork w = norm_carve(s, d_workspace, true);
-        if (s.batch > 0) {
+        Fused f;
+        bool fused = false;
+        if constexpr (VEC > 1) fused = s.batch > 0 && fused_plan(s, sizeof(T), true, &f);
+        if (fused) {
+            if constexpr (VEC > 1)
+                FC_PROPAGATE(with_act(desc->act, [&](auto a) -> int {
+                    auto kernel = norm_back_fused_kernel<T, decltype(a)::value>;
+                    FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+                    FC_CHECK_CUDA(launch_clusters(kernel, dim3(f.blocks * f.cluster, s.batch), FUSED_THREADS, f.cluster, f.smem,
+                                                  ctx->stream, (const T *)d_dy, (const T *)d_x, d_gamma, d_beta, d_mean, d_rstd,
+                                                  (T *)d_dx, w.sums, s, f));
+                    return FC_OK;
+                }));
+        } else if (s.batch > 0) {
             FC_PROPAGATE(with_act(desc->act, [&](auto a) -> int {
                 FC_CHECK_CUDA(launch_pdl(norm_back_part_kernel<T, VEC, decltype(a)::value>, dim3((unsigned)blocks),
                                          dim3(NORM_THREADS), 0, ctx->stream, (const T *)d_dy, (const T *)d_x, d_gamma, d_beta,
@@ -528,7 +1081,7 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
                 }));
         }
         if (d_dgamma != nullptr || d_dbeta != nullptr)
-            FC_CHECK_CUDA(launch_pdl(norm_back_params_kernel<T>, dim3((s.channels + NORM_THREADS - 1) / NORM_THREADS),
+            FC_CHECK_CUDA(launch_pdl(norm_back_params_kernel<T>, dim3((s.channels + 31) / 32),
                                      dim3(NORM_THREADS), 0, ctx->stream, (const float2 *)w.sums, d_dgamma, d_dbeta, s));
         return FC_OK;
     });

@@ -25,25 +25,69 @@ struct Elem<__nv_bfloat16> {
     static constexpr int kType = FC_DTYPE_BF16;
     static __device__ __forceinline__ float load(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 store(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ void load2(const __nv_bfloat16 *from, float &a, float &b) {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(from);  // a bf16 is the upper half of its fp32
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void store2(__nv_bfloat16 *to, float a, float b) {
+        *reinterpret_cast<__nv_bfloat162 *>(to) = __floats2bfloat162_rn(a, b);
+    }
 };
 template <>
 struct Elem<__half> {
     static constexpr int kType = FC_DTYPE_F16;
     static __device__ __forceinline__ float load(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half store(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ void load2(const __half *from, float &a, float &b) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(from));
+        a = f.x;
+        b = f.y;
+    }
+    static __device__ __forceinline__ void store2(__half *to, float a, float b) {
+        *reinterpret_cast<__half2 *>(to) = __floats2half2_rn(a, b);
+    }
 };
 
 // N neighbouring elements, moved with one access (N * sizeof(T) is 2, 4, 8 or 16 bytes and the address a multiple of it)
+template <int BYTES>
+struct Word;
+template <>
+struct Word<16> { typedef uint4 type; };
+template <>
+struct Word<8> { typedef uint2 type; };
+template <>
+struct Word<4> { typedef uint32_t type; };
+template <>
+struct Word<2> { typedef uint16_t type; };
+
 template <typename T, int N>
 struct alignas(N * sizeof(T)) Vec {
     T v[N];
+    typedef typename Word<N * sizeof(T)>::type W;
+    static __device__ __forceinline__ Vec load(const void *p) {
+        Vec r;
+        *reinterpret_cast<W *>(&r) = *reinterpret_cast<const W *>(p);
+        return r;
+    }
+    __device__ __forceinline__ void store(void *p) const { *reinterpret_cast<W *>(p) = *reinterpret_cast<const W *>(this); }
     __device__ __forceinline__ void unpack(float (&f)[N]) const {
+        if constexpr (sizeof(T) == 2 && N % 2 == 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = Elem<T>::load(v[i]);
+            for (int i = 0; i < N; i += 2) Elem<T>::load2(v + i, f[i], f[i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = Elem<T>::load(v[i]);
+        }
     }
     __device__ __forceinline__ void pack(const float (&f)[N]) {
+        if constexpr (sizeof(T) == 2 && N % 2 == 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = Elem<T>::store(f[i]);
+            for (int i = 0; i < N; i += 2) Elem<T>::store2(v + i, f[i], f[i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = Elem<T>::store(f[i]);
+        }
     }
 };
 
@@ -53,12 +97,46 @@ inline bool act_ok(int act) { return act >= FC_ACT_NONE && act <= FC_ACT_SIGMOID
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // ---- activations ------------------------------------------------------------------------------------------------
-// kExact: the correctly scaled library functions, for results that are kept in fp32.  Otherwise the hardware's
-// exponential and division (a few units in the 23rd bit), for results that are rounded to 8 or 11 bits anyway.
+// kExact: the library's functions, for results that are kept in fp32.  Otherwise the hardware's power of two and
+// reciprocal (a few units in the 23rd bit, subnormals as zero), for results that are rounded to 8 or 11 bits anyway: two
+// instructions of the special-function unit instead of some twenty.
+__device__ __forceinline__ float fast_exp(float z) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(z * 1.44269504088896341f));
+    return r;
+}
 template <bool kExact>
 __device__ __forceinline__ float sigmoid(float z) {
     // exp(-z) = inf for very negative z: the quotient is then 0, as it should be
-    return kExact ? 1.0f / (1.0f + expf(-z)) : __fdividef(1.0f, 1.0f + __expf(-z));
+    if (kExact) return 1.0f / (1.0f + expf(-z));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + fast_exp(-z)));
+    return r;
+}
+
+// erfc(x) exp(x^2) for x >= 0: Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26; times exp(-x^2) it is within
+// 1.5e-7 of erfc
+__device__ __forceinline__ float erfc_scaled(float x) {
+    float t;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, x, 1.0f)));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    return p * t;
+}
+// the normal distribution's function at z, and its density
+template <bool kExact>
+__device__ __forceinline__ void normal(float z, float &cdf, float &density) {
+    if (kExact) {
+        cdf = 0.5f * erfcf(-0.70710678118654752f * z);  // erfc keeps the digits of the tail
+        density = 0.39894228040143268f * expf(-0.5f * z * z);
+    } else {
+        const float e = fast_exp(-0.5f * z * z);
+        const float tail = 0.5f * e * erfc_scaled(0.70710678118654752f * fabsf(z));
+        cdf = z < 0.0f ? tail : 1.0f - tail;
+        density = 0.39894228040143268f * e;
+    }
 }
 
 // act(z); kAct is an fc_activation.  A NaN stays one in every activation.
@@ -66,7 +144,11 @@ template <int kAct, bool kExact>
 __device__ __forceinline__ float act_value(float z) {
     if (kAct == FC_ACT_RELU) return z < 0.0f ? 0.0f : z;
     if (kAct == FC_ACT_SILU) return z * sigmoid<kExact>(z);
-    if (kAct == FC_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);  // erfc keeps the digits of the tail
+    if (kAct == FC_ACT_GELU) {
+        float cdf, density;
+        normal<kExact>(z, cdf, density);
+        return z * cdf;
+    }
     if (kAct == FC_ACT_GELU_TANH) {
         // 0.5 (1 + tanh v) = sigmoid(2 v); the square is bounded so that huge z give 0 or z and no inf * 0
         const float t = fminf(z * z, 1e6f);
@@ -87,9 +169,10 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d) {
         a = z * s;
         d = s + a * (1.0f - s);
     } else if (kAct == FC_ACT_GELU) {
-        const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+        float cdf, density;
+        normal<kExact>(z, cdf, density);
         a = z * cdf;
-        d = cdf + 0.39894228040143268f * z * (kExact ? expf(-0.5f * z * z) : __expf(-0.5f * z * z));
+        d = fmaf(z, density, cdf);
     } else if (kAct == FC_ACT_GELU_TANH) {
         const float t = fminf(z * z, 1e6f);
         const float s = sigmoid<kExact>(1.59576912160573071f * z * (1.0f + 0.044715f * t));
@@ -102,6 +185,86 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d) {
         a = z;
         d = 1.0f;
     }
+}
+
+// ---- pairs ------------------------------------------------------------------------------------------------------
+// Two fp32 values in one 64-bit register: one instruction adds, multiplies or multiplies and adds both, each half rounded
+// like the scalar instruction.
+typedef uint64_t Pair;
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 split(Pair p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void unpack_pairs(const Vec<T, N> &v, Pair (&p)[N / 2]) {
+    float f[N];
+    v.unpack(f);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) p[i] = pair(f[2 * i], f[2 * i + 1]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void pack_pairs(Vec<T, N> &v, const Pair (&p)[N / 2]) {
+    float f[N];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const float2 h = split(p[i]);
+        f[2 * i] = h.x;
+        f[2 * i + 1] = h.y;
+    }
+    v.pack(f);
+}
+__device__ __forceinline__ Pair sigmoid_fast2(Pair z) {
+    const float2 t = split(mul2(z, pair(-1.44269504088896341f, -1.44269504088896341f)));
+    float a, b;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(t.y));
+    const float2 u = split(add2(pair(a, b), pair(1.0f, 1.0f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(u.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(u.y));
+    return pair(a, b);
+}
+template <int kAct, bool kExact>
+__device__ __forceinline__ Pair act_value2(Pair z) {
+    if (kAct == FC_ACT_NONE) return z;
+    if (kAct == FC_ACT_SILU && !kExact) return mul2(z, sigmoid_fast2(z));
+    const float2 f = split(z);
+    return pair(act_value<kAct, kExact>(f.x), act_value<kAct, kExact>(f.y));
+}
+template <int kAct, bool kExact>
+__device__ __forceinline__ void act_both2(Pair z, Pair &a, Pair &d) {
+    if (kAct == FC_ACT_SILU && !kExact) {
+        const Pair s = sigmoid_fast2(z), one = pair(1.0f, 1.0f), minus = pair(-1.0f, -1.0f);
+        a = mul2(z, s);
+        d = fma2(a, fma2(s, minus, one), s);
+        return;
+    }
+    const float2 f = split(z);
+    float a0, a1, d0, d1;
+    act_both<kAct, kExact>(f.x, a0, d0);
+    act_both<kAct, kExact>(f.y, a1, d1);
+    a = pair(a0, a1);
+    d = pair(d0, d1);
 }
 
 // Calls f(std::integral_constant<int, act>) for a run-time activation.
@@ -144,6 +307,26 @@ class DeviceScope {
     int before_;
     cudaError_t status_;
 };
+
+// A launch of clusters of `cluster` blocks, in stream order like every other (programmatic dependent launch).
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, unsigned threads, unsigned cluster, size_t smem,
+                                   cudaStream_t stream, Args &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
 
 // A bump allocator over the workspace that the caller passed; with a null base it only counts.
 struct Carver {
