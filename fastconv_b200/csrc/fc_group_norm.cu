@@ -41,6 +41,36 @@ __device__ __forceinline__ float param(const void *p, int c, int f32, float abse
     return f32 ? __ldg((const float *)p + c) : Elem<T>::load(((const T *)p)[c]);
 }
 
+// the values of VEC channels from c on; c is a multiple of VEC
+template <typename T, int VEC>
+__device__ __forceinline__ void params(const void *p, int c, int f32, float absent, float (&v)[VEC]) {
+    if (p == nullptr) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = absent;
+    } else if (((uintptr_t)p & 15) != 0 || VEC == 1) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = param<T>(p, c + i, f32, absent);
+    } else if (f32) {
+        constexpr int N = VEC < 4 ? VEC : 4;
+#pragma unroll
+        for (int i = 0; i < VEC; i += N) {
+            float w[N];
+            Vec<float, N>::load((const float *)p + c + i).unpack(w);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[i + j] = w[j];
+        }
+    } else {
+        Vec<T, VEC>::load((const T *)p + c).unpack(v);
+    }
+}
+__device__ __forceinline__ float quick_inverse(float v) {  // to a unit in the last place
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// a / b for 0 <= a < 2^22, where by = 1 / b to a unit in the last place
+__device__ __forceinline__ int quotient(int a, float by) { return (int)(((float)a + 0.5f) * by); }
+
 // which image, share of pixels and columns a block has
 struct Place {
     int img, chunk, p0, p1, col, row, rows, c0;
@@ -171,12 +201,14 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_apply_kernel(const T *__res
     const Place b = place_of<VEC>(s);
     if (!b.live) return;
     float m[VEC], a[VEC], o[VEC];
+    params<T, VEC>(gamma, b.c0, s.params_f32, 1.0f, a);
+    params<T, VEC>(beta, b.c0, s.params_f32, 0.0f, o);
+    int g = b.c0 / s.cpg, j = b.c0 - g * s.cpg;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-        const int c = b.c0 + i, at = b.img * s.groups + c / s.cpg;
-        m[i] = mean[at];
-        a[i] = rstd[at] * param<T>(gamma, c, s.params_f32, 1.0f);
-        o[i] = param<T>(beta, c, s.params_f32, 0.0f);
+        m[i] = mean[b.img * s.groups + g];
+        a[i] *= rstd[b.img * s.groups + g];
+        if (++j == s.cpg) j = 0, ++g;
     }
     const T *src = x + (size_t)b.img * s.pixels * s.xs + b.c0;
     T *dst = y + (size_t)b.img * s.pixels * s.ys + b.c0;
@@ -202,13 +234,14 @@ struct BackChannels {
     float m[VEC], r[VEC], g[VEC], o[VEC];
     __device__ __forceinline__ BackChannels(const void *gamma, const void *beta, const float *mean, const float *rstd, int img,
                                             int c0, const NormShape &s) {
+        params<T, VEC>(gamma, c0, s.params_f32, 1.0f, g);
+        params<T, VEC>(beta, c0, s.params_f32, 0.0f, o);
+        int k = c0 / s.cpg, j = c0 - k * s.cpg;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const int c = c0 + i, at = img * s.groups + c / s.cpg;
-            m[i] = mean[at];
-            r[i] = rstd[at];
-            g[i] = param<T>(gamma, c, s.params_f32, 1.0f);
-            o[i] = param<T>(beta, c, s.params_f32, 0.0f);
+            m[i] = mean[img * s.groups + k];
+            r[i] = rstd[img * s.groups + k];
+            if (++j == s.cpg) j = 0, ++k;
         }
     }
     // dz and xhat of channel i
@@ -341,8 +374,10 @@ struct Fused {
     int cb, vectors, rows;  // channels and vectors of a block of channels; threads of one vector column
     int blocks;             // blocks of channels of an image
     int cluster, pc;        // blocks of a cluster; pixels of one block
-    int groups, tg;         // groups of a block of channels; threads that add one up
+    int groups, log_tg;     // groups of a block of channels; 2^log_tg threads add one up
     int width, per_row;     // channels of a slot of GroupSums, slots of a group in a row
+    int part;               // pixels of one of the COPY_GROUPS parts that copies are waited for in
+    float by_vectors, by_cpg;  // 1 / vectors, 1 / channels of a group
     size_t smem;
 };
 constexpr int FUSED_THREADS = 256, COPY_GROUPS = 4;
@@ -356,27 +391,42 @@ struct FusedPlace {
 __device__ __forceinline__ FusedPlace fused_place(const NormShape &s, const Fused &f, int vec) {
     FusedPlace b;
     b.rank = blockIdx.x & (f.cluster - 1);  // clusters of 1, 2, 4 or 8
-    b.cblk = blockIdx.x / f.cluster;
+    b.cblk = blockIdx.x >> (f.cluster == 8 ? 3 : f.cluster >> 1);
     b.img = blockIdx.y;
     b.p0 = (int64_t)b.rank * f.pc;
     b.np = (int)max((int64_t)0, min((int64_t)f.pc, s.pixels - b.p0));
-    b.row = threadIdx.x / f.vectors;
+    b.row = quotient(threadIdx.x, f.by_vectors);
     b.col = threadIdx.x - b.row * f.vectors;
     b.live = b.row < f.rows;
     b.c0 = b.cblk * f.cb + b.col * vec;
-    b.g0 = b.col * vec / s.cpg;
+    b.g0 = quotient(b.col * vec, f.by_cpg);
     b.j0 = b.col * vec - b.g0 * s.cpg;
     return b;
 }
 // use(i, group of the block that the thread's channel i belongs to)
 template <int VEC, typename F>
-__device__ __forceinline__ void over_groups(const NormShape &s, const FusedPlace &b, F &&use) {
+__device__ __forceinline__ void over_groups(const NormShape &s, const Fused &f, const FusedPlace &b, F &&use) {
+    if (f.width == VEC) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) use(i, b.g0);
+        return;
+    }
     int g = b.g0, j = b.j0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         use(i, g);
         if (++j == s.cpg) j = 0, ++g;
     }
+}
+// The cluster's barrier.  Only threads that wrote what other blocks will read make their writes visible: the fence waits for
+// everything that a thread has under way.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync(bool wrote) {
+    if (wrote) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
 }
 __device__ __forceinline__ void copy16(void *to, const void *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
@@ -385,10 +435,9 @@ template <int N>
 __device__ __forceinline__ void copies_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// f(begin, end) for each of the thread's COPY_GROUPS parts of its pixels, once the part's copies have landed
+// f(begin, end) for each of the COPY_GROUPS parts of the block's pixels, once this thread's copies of the part have landed
 template <typename F>
-__device__ __forceinline__ void as_they_land(int np, int rows, F &&f) {
-    const int part = ((np + rows - 1) / rows + COPY_GROUPS - 1) / COPY_GROUPS * rows;
+__device__ __forceinline__ void as_they_land(int np, int part, F &&f) {
     copies_wait<3>();
     f(0, min(np, part));
     copies_wait<2>();
@@ -398,12 +447,8 @@ __device__ __forceinline__ void as_they_land(int np, int rows, F &&f) {
     copies_wait<0>();
     f(3 * part, np);
 }
-__device__ __forceinline__ int first_part(int np, int rows) {
-    return min(np, ((np + rows - 1) / rows + COPY_GROUPS - 1) / COPY_GROUPS * rows);
-}
 template <typename F>
-__device__ __forceinline__ void copy_parts(int np, int rows, F &&f) {
-    const int part = ((np + rows - 1) / rows + COPY_GROUPS - 1) / COPY_GROUPS * rows;
+__device__ __forceinline__ void copy_parts(int np, int part, F &&f) {
 #pragma unroll
     for (int i = 0; i < COPY_GROUPS; ++i) {
         f(i * part, i + 1 < COPY_GROUPS ? min(np, (i + 1) * part) : np);
@@ -415,7 +460,7 @@ __device__ __forceinline__ void copy_parts(int np, int rows, F &&f) {
 // vector where a group's channels are whole vectors, else a channel; a group's slots of all rows lie together, so that
 // `tg` neighbouring threads (a power of two) add them without index arithmetic.
 struct GroupSums {
-    int groups, slots, tg;  // groups of the block; slots of a group in all rows; threads to a group
+    int groups, slots, log_tg;  // groups of the block; slots of a group in all rows; 2^log_tg threads to a group
     int width;              // channels of a slot
     float *stat, *scratch, *red;  // [planes][rows * cb], [planes][8], [planes][groups]
     int plane, per_row;
@@ -440,8 +485,8 @@ struct GroupSums {
     template <int PLANES>
     __device__ __forceinline__ void add() const {
         __syncthreads();
-        const int l = threadIdx.x & (tg - 1), lane = threadIdx.x & 31;
-        for (int g = threadIdx.x / tg; g < groups || tg > 1; g += FUSED_THREADS / tg) {
+        const int tg = 1 << log_tg, l = threadIdx.x & (tg - 1), lane = threadIdx.x & 31;
+        for (int g = threadIdx.x >> log_tg; g < groups || tg > 1; g += FUSED_THREADS >> log_tg) {
             float t[PLANES];
 #pragma unroll
             for (int k = 0; k < PLANES; ++k) {
@@ -459,20 +504,22 @@ struct GroupSums {
         }
         __syncthreads();
         if (tg > 32) {
-            if (threadIdx.x < PLANES * groups) {
-                const int k = threadIdx.x / groups, g = threadIdx.x - k * groups;
-                float t = 0.0f;
-                for (int w = 0; w < tg / 32; ++w) t += scratch[k * 8 + g * (tg / 32) + w];
-                red[k * groups + g] = t;
+            if (threadIdx.x < groups) {
+#pragma unroll
+                for (int k = 0; k < PLANES; ++k) {
+                    float t = 0.0f;
+                    for (int w = 0; w < tg / 32; ++w) t += scratch[k * 8 + threadIdx.x * (tg / 32) + w];
+                    red[k * groups + threadIdx.x] = t;
+                }
             }
             __syncthreads();
         }
     }
 };
 
-// The level that deviations are taken from is the mean of the first part of the block's pixels to land, known while the others
-// are on their way: a quarter's mean is within sqrt(3) standard deviations of the whole's, so the squares lose no digits
-// however far the map is from zero.  The blocks of a cluster are joined by `join`.
+// Squares are taken around one value of the group, its first in the block.  Where that turns out to be more than four standard
+// deviations from the mean, they are taken once more around the mean, so the variance never loses more than some four of
+// its 24 bits, however far the map is from zero.  The blocks of a cluster are joined by the means' distances.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__restrict__ x, const void *__restrict__ gamma,
                                                                   const void *__restrict__ beta, T *__restrict__ y,
@@ -490,7 +537,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
     gs.width = f.width;
     gs.per_row = f.per_row;
     gs.slots = f.rows * f.per_row;
-    gs.tg = f.tg;
+    gs.log_tg = f.log_tg;
     gs.plane = f.rows * f.cb;
     gs.stat = (float *)(data + (size_t)f.pc * f.vectors);
     gs.scratch = scratch;
@@ -500,104 +547,111 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
     const FusedPlace b = fused_place(s, f, VEC);
     V *mine = data + b.row * f.vectors + b.col;
     const int hop = f.rows * f.vectors;
-    const int first = first_part(b.np, f.rows);  // pixels that the level is taken from
     pdl_wait();
     if (b.live) {
         const T *src = x + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.xs + b.c0;
         const int64_t src_hop = f.rows * s.xs;
         V *to = mine;
-        copy_parts(b.np, f.rows, [&](int from, int upto) {
+        copy_parts(b.np, f.part, [&](int from, int upto) {
             for (int p = from + b.row; p < upto; p += f.rows, to += hop, src += src_hop) copy16(to, src);
         });
     }
+    // this thread's group, where a thread sums one up in the end, and its level
+    const T *corner = x + ((size_t)b.img * s.pixels + b.p0) * s.xs + b.cblk * f.cb;
+    const bool sums = threadIdx.x < gs.groups;
+    float level = sums ? Elem<T>::load(corner[threadIdx.x * s.cpg]) : 0.0f;
     float v[VEC], u[VEC];
-    {
-        Pair sum[VEC / 2];
-#pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) sum[i] = 0;
-        copies_wait<COPY_GROUPS - 1>();
-        if (b.live) {
-            const V *at = mine;
-#pragma unroll 2
-            for (int p = b.row; p < first; p += f.rows, at += hop) {
-                Pair q[VEC / 2];
-                unpack_pairs(V::load(at), q);
-#pragma unroll
-                for (int i = 0; i < VEC / 2; ++i) sum[i] = add2(sum[i], q[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) v[2 * i] = split(sum[i]).x, v[2 * i + 1] = split(sum[i]).y;
-            gs.put<VEC>(s, b, 0, v);
-        }
-    }
-    gs.template add<1>();
-    const float first_inv = 1.0f / ((float)first * (float)s.cpg);
-    {
-        Pair level[VEC / 2], sum[VEC / 2], sq[VEC / 2];
-        over_groups<VEC>(s, b, [&](int i, int g) { v[i] = b.live ? -gs.red[g] * first_inv : 0.0f; });
+    over_groups<VEC>(s, f, b, [&](int i, int g) { v[i] = b.live ? -Elem<T>::load(corner[g * s.cpg]) : 0.0f; });
+    const float n_inv = quick_inverse((float)b.np * (float)s.cpg);
+    auto deviations = [&](auto &&passes) {  // from -v; their sums and squares' sums to gs.red
+        Pair from[VEC / 2], sum[VEC / 2], sq[VEC / 2];
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) {
-            level[i] = pair(v[2 * i], v[2 * i + 1]);
+            from[i] = pair(v[2 * i], v[2 * i + 1]);
             sum[i] = sq[i] = 0;
         }
         const V *at = mine;
-        as_they_land(b.np, f.rows, [&](int from, int upto) {
+        passes([&](int begin, int end) {
             if (!b.live) return;
 #pragma unroll 2
-            for (int p = from + b.row; p < upto; p += f.rows, at += hop) {
+            for (int p = begin + b.row; p < end; p += f.rows, at += hop) {
                 Pair q[VEC / 2];
                 unpack_pairs(V::load(at), q);
 #pragma unroll
                 for (int i = 0; i < VEC / 2; ++i) {
-                    const Pair d = add2(q[i], level[i]);
+                    const Pair d = add2(q[i], from[i]);
                     sum[i] = add2(sum[i], d);
                     sq[i] = fma2(d, d, sq[i]);
                 }
             }
         });
         if (b.live) {
+            float a[VEC], c[VEC];
 #pragma unroll
             for (int i = 0; i < VEC / 2; ++i) {
-                v[2 * i] = split(sum[i]).x, v[2 * i + 1] = split(sum[i]).y;
-                u[2 * i] = split(sq[i]).x, u[2 * i + 1] = split(sq[i]).y;
+                a[2 * i] = split(sum[i]).x, a[2 * i + 1] = split(sum[i]).y;
+                c[2 * i] = split(sq[i]).x, c[2 * i + 1] = split(sq[i]).y;
             }
-            gs.put<VEC>(s, b, 0, v);
-            gs.put<VEC>(s, b, 1, u);
+            gs.put<VEC>(s, b, 0, a);
+            gs.put<VEC>(s, b, 1, c);
         }
+        gs.template add<2>();
+    };
+    deviations([&](auto &&part) { as_they_land(b.np, f.part, part); });
+    float d = 0.0f, q = 0.0f;
+    if (sums) {
+        d = gs.red[threadIdx.x] * n_inv;
+        q = fmaf(-d, gs.red[threadIdx.x], gs.red[gs.groups + threadIdx.x]);
+        level += d;
+        share[threadIdx.x] = make_float2(level, fmaxf(q, 0.0f));
     }
-    const float level = threadIdx.x < gs.groups ? gs.red[threadIdx.x] * first_inv : 0.0f;  // before it is written again
-    gs.template add<2>();
-    if (threadIdx.x < gs.groups) {
-        const float d = gs.red[threadIdx.x], q = gs.red[gs.groups + threadIdx.x], n_inv = 1.0f / ((float)b.np * (float)s.cpg);
-        share[threadIdx.x] = make_float2(fmaf(d, n_inv, level), fmaxf(fmaf(-d * n_inv, d, q), 0.0f));
+    if (__syncthreads_or(sums && !(gs.red[threadIdx.x] * d <= 16.0f * q) && d != 0.0f)) {
+        over_groups<VEC>(s, f, b, [&](int i, int g) { v[i] = b.live ? -share[g].x : 0.0f; });
+        deviations([&](auto &&part) { part(0, b.np); });
+        if (sums) {
+            d = gs.red[threadIdx.x] * n_inv;
+            q = fmaf(-d, gs.red[threadIdx.x], gs.red[gs.groups + threadIdx.x]);
+            share[threadIdx.x] = make_float2(level + d, fmaxf(q, 0.0f));
+        }
     }
     if (f.cluster > 1)
-        cg::this_cluster().sync();
+        cluster_sync(sums);
     else
         __syncthreads();
-    if (threadIdx.x < gs.groups) {
+    if (sums) {
         const int g = threadIdx.x;
-        float n = 0.0f, m = 0.0f, q = 0.0f;
-        for (int r = 0; r < f.cluster; ++r) {
-            const float2 w = f.cluster > 1 ? *cg::this_cluster().map_shared_rank(share + g, r) : share[g];
-            const int np = (int)min((int64_t)f.pc, s.pixels - (int64_t)r * f.pc);
-            join(n, m, q, (float)np, w.x, w.y / s.cpg);
-        }
-        const float rs = 1.0f / sqrtf(q / n + s.eps);
+        float2 w[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r < f.cluster) w[r] = f.cluster > 1 ? *cg::this_cluster().map_shared_rank(share + g, r) : share[g];
+        const float all_inv = quick_inverse((float)s.pixels), m0 = w[0].x;
+        float m = 0.0f, sq = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r < f.cluster) m = fmaf((float)min(f.pc, s.pixels - r * f.pc), w[r].x - m0, m);
+        m = fmaf(m, all_inv, m0);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r < f.cluster) {
+                const float e = w[r].x - m;
+                sq = fmaf((float)min(f.pc, s.pixels - r * f.pc) * (float)s.cpg, e * e, sq + w[r].y);
+            }
+        const float rs = 1.0f / sqrtf(fmaf(sq, all_inv * quick_inverse((float)s.cpg), s.eps));
         total[g] = make_float2(m, rs);
         const int at = b.img * s.groups + b.cblk * gs.groups + g;
         if (b.rank == 0 && mean != nullptr) mean[at] = m;
         if (b.rank == 0 && rstd != nullptr) rstd[at] = rs;
     }
     __syncthreads();
-    if (f.cluster > 1) cg::this_cluster().barrier_arrive();
+    if (f.cluster > 1) cluster_arrive();
     if (b.live) {
         Pair m[VEC / 2], a[VEC / 2], o[VEC / 2];
         float w[VEC];
-        over_groups<VEC>(s, b, [&](int i, int g) {
+        params<T, VEC>(gamma, b.c0, s.params_f32, 1.0f, u);
+        params<T, VEC>(beta, b.c0, s.params_f32, 0.0f, v);
+        over_groups<VEC>(s, f, b, [&](int i, int g) {
             const float2 t = total[g];
-            u[i] = t.y * param<T>(gamma, b.c0 + i, s.params_f32, 1.0f);
-            v[i] = param<T>(beta, b.c0 + i, s.params_f32, 0.0f);
+            u[i] *= t.y;
             w[i] = -t.x;
         });
 #pragma unroll
@@ -621,7 +675,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
             out.store(dst);
         }
     }
-    if (f.cluster > 1) cg::this_cluster().barrier_wait();  // the others have read this block's sums
+    if (f.cluster > 1) cluster_wait();  // the others have read this block's sums
 }
 
 // sums[img * channels + c]: the image's (sum dz, sum dz xhat)
@@ -649,7 +703,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
         const T *sd = dy + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.ys + b.c0;
         const int64_t x_hop = f.rows * s.xs, d_hop = f.rows * s.ys;
         int at = start;
-        copy_parts(b.np, f.rows, [&](int from, int upto) {
+        copy_parts(b.np, f.part, [&](int from, int upto) {
             for (int p = from + b.row; p < upto; p += f.rows, at += hop, sx += x_hop, sd += d_hop) {
                 copy16(xs + at, sx);
                 copy16(ds + at, sd);
@@ -660,13 +714,13 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
     Pair m[VEC / 2], r[VEC / 2], gm[VEC / 2], bt[VEC / 2];  // -mean, rstd, gamma, beta
     if (b.live) {
         float fm[VEC], fr[VEC], fg[VEC], fb[VEC];
-        over_groups<VEC>(s, b, [&](int i, int g) {
+        over_groups<VEC>(s, f, b, [&](int i, int g) {
             const int at = b.img * s.groups + b.cblk * f.groups + g;
             fr[i] = rstd[at];
             fm[i] = -mean[at];
-            fg[i] = param<T>(gamma, b.c0 + i, s.params_f32, 1.0f);
-            fb[i] = param<T>(beta, b.c0 + i, s.params_f32, 0.0f);
         });
+        params<T, VEC>(gamma, b.c0, s.params_f32, 1.0f, fg);
+        params<T, VEC>(beta, b.c0, s.params_f32, 0.0f, fb);
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) {
             m[i] = pair(fm[2 * i], fm[2 * i + 1]);
@@ -687,7 +741,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) s1[i] = s2[i] = 0;
         int at = start;
-        as_they_land(b.np, f.rows, [&](int from, int upto) {
+        as_they_land(b.np, f.part, [&](int from, int upto) {
             if (!b.live) return;
             for (int p = from + b.row; p < upto; p += f.rows, at += hop) {
                 Pair v[VEC / 2], d[VEC / 2];
@@ -737,24 +791,26 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
         share[c] = t;
     }
     if (f.cluster > 1)
-        cg::this_cluster().sync();
+        cluster_sync(threadIdx.x < f.cb);
     else
         __syncthreads();
     for (int c = threadIdx.x; c < f.cb; c += FUSED_THREADS) {
         float2 t = make_float2(0.0f, 0.0f);
-        for (int r = 0; r < f.cluster; ++r) {
-            const float2 v = f.cluster > 1 ? *cg::this_cluster().map_shared_rank(share + c, r) : share[c];
-            t.x += v.x;
-            t.y += v.y;
-        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r < f.cluster) {
+                const float2 v = f.cluster > 1 ? *cg::this_cluster().map_shared_rank(share + c, r) : share[c];
+                t.x += v.x;
+                t.y += v.y;
+            }
         total[c] = t;
         if (b.rank == 0) sums[(size_t)b.img * s.channels + b.cblk * f.cb + c] = t;
     }
     __syncthreads();
-    if (f.cluster > 1) cg::this_cluster().barrier_arrive();
+    if (f.cluster > 1) cluster_arrive();
     if (dx != nullptr) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = f.cb / s.cpg;
-        const float inv = 1.0f / ((float)s.pixels * (float)s.cpg);
+        const float inv = quick_inverse((float)s.pixels * (float)s.cpg);
         for (int g = warp; g < groups; g += FUSED_THREADS / 32) {
             float a = 0.0f, q = 0.0f;
             for (int i = lane; i < s.cpg; i += 32) {
@@ -773,7 +829,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
         __syncthreads();
         if (b.live) {
             float fa[VEC], fb[VEC];
-            over_groups<VEC>(s, b, [&](int i, int g) { fa[i] = -ab[g].x, fb[i] = -ab[g].y; });
+            over_groups<VEC>(s, f, b, [&](int i, int g) { fa[i] = -ab[g].x, fb[i] = -ab[g].y; });
             Pair ta[VEC / 2], tb[VEC / 2];
 #pragma unroll
             for (int i = 0; i < VEC / 2; ++i) ta[i] = pair(fa[2 * i], fa[2 * i + 1]), tb[i] = pair(fb[2 * i], fb[2 * i + 1]);
@@ -796,7 +852,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
             }
         }
     }
-    if (f.cluster > 1) cg::this_cluster().barrier_wait();
+    if (f.cluster > 1) cluster_wait();
 }
 
 // dgamma[c], dbeta[c]: the images' sums.  32 channels x 8 shares of the images to a block; the shares are added in order.
@@ -882,12 +938,15 @@ bool fused_plan(const NormShape &s, int esize, bool backward, Fused *best) {
         if (vectors > FUSED_THREADS || cb / s.cpg > FUSED_THREADS) break;
         if (s.channels % cb) continue;
         for (int cluster = 1; cluster <= 8; cluster *= 2) {
-            Fused f = {cb, vectors, FUSED_THREADS / vectors, s.channels / cb, cluster, (s.pixels + cluster - 1) / cluster, cb / s.cpg, 1, 1, 1, 0};
+            Fused f = {cb, vectors, FUSED_THREADS / vectors, s.channels / cb, cluster, (s.pixels + cluster - 1) / cluster, cb / s.cpg};
             f.width = s.cpg % vec ? 1 : vec;
             f.per_row = s.cpg / f.width;
+            f.part = (int)ceil_div(ceil_div(f.pc, f.rows), COPY_GROUPS) * f.rows;
+            f.by_vectors = 1.0f / vectors;
+            f.by_cpg = 1.0f / s.cpg;
             if (cluster > 1 && (long long)f.pc * (cluster - 1) >= s.pixels) break;  // a block would have no pixels
             f.smem = (size_t)f.pc * run * arrays + ((size_t)f.rows * cb + 3 * cb) * sizeof(float2);
-            while (2 * f.tg * f.groups <= FUSED_THREADS) f.tg *= 2;
+            while ((2 << f.log_tg) * f.groups <= FUSED_THREADS) ++f.log_tg;
             if (f.smem > 200 * 1024) continue;
             const double blocks = (double)s.batch * f.blocks * cluster;
             double per_sm = 220.0 * 1024 / (f.smem + 1024.0);

@@ -234,20 +234,29 @@ __device__ __forceinline__ void pack_pairs(Vec<T, N> &v, const Pair (&p)[N / 2])
     }
     v.pack(f);
 }
+// Two sigmoids with one reciprocal: 1/a = b/(ab), 1/b = a/(ab).  The exponentials are bounded by 2^60 so that the product is
+// finite (and a NaN stays in its half: z itself is multiplied in later); a sigmoid below 2^-60 comes out as 2^-60.  The
+// special-function unit, which gives four results a clock to a quarter of an SM, is what the activations wait for.
 __device__ __forceinline__ Pair sigmoid_fast2(Pair z) {
     const float2 t = split(mul2(z, pair(-1.44269504088896341f, -1.44269504088896341f)));
-    float a, b;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(t.x));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(t.y));
+    float a, b, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(fminf(t.x, 60.0f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(fminf(t.y, 60.0f)));
     const float2 u = split(add2(pair(a, b), pair(1.0f, 1.0f)));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(u.x));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(u.y));
-    return pair(a, b);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u.x * u.y));
+    return mul2(pair(r, r), pair(u.y, u.x));
+}
+__device__ __forceinline__ Pair gelu_tanh_argument(Pair z) {  // sqrt(8 / pi) (z + 0.044715 z^3), |z| bounded in the cube
+    const float2 q = split(mul2(z, z));
+    const Pair t = pair(fminf(q.x, 1e6f), fminf(q.y, 1e6f));
+    const Pair k = pair(0.044715f * 1.59576912160573071f, 0.044715f * 1.59576912160573071f);
+    return mul2(z, fma2(t, k, pair(1.59576912160573071f, 1.59576912160573071f)));
 }
 template <int kAct, bool kExact>
 __device__ __forceinline__ Pair act_value2(Pair z) {
     if (kAct == FC_ACT_NONE) return z;
     if (kAct == FC_ACT_SILU && !kExact) return mul2(z, sigmoid_fast2(z));
+    if (kAct == FC_ACT_GELU_TANH && !kExact) return mul2(z, sigmoid_fast2(gelu_tanh_argument(z)));
     const float2 f = split(z);
     return pair(act_value<kAct, kExact>(f.x), act_value<kAct, kExact>(f.y));
 }
