@@ -34,6 +34,7 @@ SOURCES = [
     "fc_gated_ff.cu",
     "fc_ff_ffma.cu",
     "fc_ff_tc.cu",
+    "fc_ff_few.cu",
 ]
 
 NVCC_FLAGS = [

@@ -19,17 +19,6 @@ using namespace last;
 
 constexpr int BM = 128, BN = 128, BK = 16, FF_THREADS = 256, PAD = 4;
 
-__device__ __forceinline__ void act_both_rt(int act, float z, float &a, float &d) {
-    switch (act) {
-        case FC_ACT_RELU: return act_both<FC_ACT_RELU, true>(z, a, d);
-        case FC_ACT_SILU: return act_both<FC_ACT_SILU, true>(z, a, d);
-        case FC_ACT_GELU: return act_both<FC_ACT_GELU, true>(z, a, d);
-        case FC_ACT_GELU_TANH: return act_both<FC_ACT_GELU_TANH, true>(z, a, d);
-        case FC_ACT_SIGMOID: return act_both<FC_ACT_SIGMOID, true>(z, a, d);
-        default: return act_both<FC_ACT_NONE, true>(z, a, d);
-    }
-}
-
 // eight neighbouring elements of a row from `at` on, zero from `end` on
 template <typename T>
 __device__ __forceinline__ void load8(const T *row, int64_t at, int64_t end, bool wide, float (&f)[8]) {

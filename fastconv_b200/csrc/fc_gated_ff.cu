@@ -190,6 +190,7 @@ Work carve(const Block &b, void *base, bool backward) {
 
 int multiply(fc_context *ctx, FfProduct p, float *part) {
     p.part = part;
+    if (p.kind != FF_GATE_BACK && ff_few_fits(p)) return launch_ff_few(ctx, p);
     if (ff_tc_fits(p)) return launch_ff_tc(ctx, p);
     if (p.kind == FF_STORE) p.splits = ff_ffma_splits(p.m, p.n, p.k);
     FC_PROPAGATE(launch_ff_ffma(ctx, p));

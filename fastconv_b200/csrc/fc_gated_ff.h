@@ -1,5 +1,5 @@
-// The matrix products of the gated feed-forward block, as its two kernel families take them (fc_ff_ffma.cu for fp32 and
-// for what the tensor cores' copies cannot address, fc_ff_tc.cu for bf16 and fp16).
+// The matrix products of the gated feed-forward block, as its kernel families take them (fc_ff_few.cu for a few rows,
+// fc_ff_tc.cu for bf16 and fp16, fc_ff_ffma.cu for fp32 and for what the tensor cores' copies cannot address).
 #pragma once
 
 #include "fc_internal.h"
@@ -47,6 +47,9 @@ inline int64_t ff_saved_at(int64_t m, int64_t n, int64_t rows, int64_t cols) {
 int launch_ff_ffma(fc_context *ctx, const FfProduct &p);
 // shares of the reduction for an FF_STORE product, so that few output tiles still occupy the GPU
 int ff_ffma_splits(int m, int n, int k);
+
+bool ff_few_fits(const FfProduct &p);  // at most 8 rows
+int launch_ff_few(fc_context *ctx, const FfProduct &p);
 
 struct FfTcPlan {
     int bn, splits;

@@ -187,6 +187,18 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d) {
     }
 }
 
+// the same for an activation that is known at run time only
+__device__ __forceinline__ void act_both_rt(int act, float z, float &a, float &d) {
+    switch (act) {
+        case FC_ACT_RELU: return act_both<FC_ACT_RELU, true>(z, a, d);
+        case FC_ACT_SILU: return act_both<FC_ACT_SILU, true>(z, a, d);
+        case FC_ACT_GELU: return act_both<FC_ACT_GELU, true>(z, a, d);
+        case FC_ACT_GELU_TANH: return act_both<FC_ACT_GELU_TANH, true>(z, a, d);
+        case FC_ACT_SIGMOID: return act_both<FC_ACT_SIGMOID, true>(z, a, d);
+        default: return act_both<FC_ACT_NONE, true>(z, a, d);
+    }
+}
+
 // ---- pairs ------------------------------------------------------------------------------------------------------
 // Two fp32 values in one 64-bit register: one instruction adds, multiplies or multiplies and adds both, each half rounded
 // like the scalar instruction.
