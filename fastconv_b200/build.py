@@ -32,7 +32,6 @@ SOURCES = [
     "fc_map_move.cu",
     "fc_group_norm.cu",
     "fc_gated_ff.cu",
-    "fc_ff_ffma.cu",
     "fc_ff_tc.cu",
     "fc_ff_few.cu",
 ]

@@ -1,9 +1,9 @@
-// The feed-forward block's matrix products on the 5th-generation tensor cores, bf16 and fp16.
+// The feed-forward block's matrix products on the 5th-generation tensor cores.
 //
 // A pair of CTAs computes 256 x bn outputs (bn = 64, 128 or 256) with tcgen05.mma.cta_group::2: each CTA stages its own 128
 // rows of A and half of B's columns, so an operand byte is fetched into shared memory once for 256 rows or bn columns.
 // Persistent; per CTA
-//   warp 0      producer: TMA boxes of 64 reduction steps into a ring of 5 stages (16 KB of A, up to 16 KB of B)
+//   warp 0      producer: TMA boxes of 64 reduction steps into a ring of stages
 //   warp 1      of the pair's first CTA: the matrix instructions, into one of two accumulators in tensor memory
 //   warps 2..9  epilogue of the other accumulator: 32 rows x 32 columns at a time, from tensor memory through registers and
 //               a swizzled 2 KB piece of shared memory to a TMA store, which also cuts off what lies outside the matrix
@@ -12,6 +12,12 @@
 //
 // FF_GATE: the first CTA's half of B are rows of the gate's weights, the second's the same rows of the up projection's, so
 // columns j and bn/2 + j of the accumulator are the two values that one output needs.
+//
+// fp32 (three planes): a value is the sum of three bf16 values exactly, x = h + m + l (8 bits each).  Of the nine products of two
+// values the six largest are taken, hh, hm, mh, hl, lh, mm; the others are below 2^-25 of the result.  The tensor cores' fp32
+// additions round toward zero, which over a long reduction adds up to a bias of some 2e-8 an instruction: the five small
+// products, where that does not matter, have an accumulator of their own, and the sum of hh is taken over into registers,
+// rounded to nearest, every 256 steps.  Six times the work of a bf16 product, and still four times the FP32 pipe's rate.
 #include <cstring>
 #include <type_traits>
 
@@ -26,16 +32,22 @@ namespace {
 using namespace last;
 using namespace tc;
 
-constexpr int KB = 64;                        // reduction steps of a stage: 128 bytes, one swizzle span
-constexpr int FF_STAGES = 5;
-constexpr int HALF_BYTES = 128 * KB * 2;      // one CTA's A, and the most of its B, in a stage
+constexpr int KB = 64;                    // reduction steps of a stage: 128 bytes, one swizzle span
+constexpr int HALF_BYTES = 128 * KB * 2;  // one CTA's A in a stage and plane
 constexpr int EPI_WARPS = 8;
-constexpr int PIECE = 32 * 32 * 2;            // 32 rows x 32 columns of 16 bits
-constexpr int PIECES = 4;                     // a warp's ring of pieces on their way out
+constexpr int PIECE = 32 * 32 * 2;        // 32 rows x 32 columns of 16 bits
+constexpr int PIECES = 4;                 // a warp's ring of pieces on their way out
 constexpr int FF_TC_THREADS = 64 + 32 * EPI_WARPS;
-constexpr int RING_BYTES = FF_STAGES * 2 * HALF_BYTES;
 constexpr int OUT_BYTES = EPI_WARPS * PIECES * PIECE;
-constexpr int FF_SMEM = 1024 + RING_BYTES + OUT_BYTES + 256;
+constexpr int CHUNK = 4;                  // k-blocks whose sum stays in tensor memory, three planes
+
+template <int PLANES>
+struct Ring {
+    static constexpr int kStages = PLANES == 1 ? 5 : 2;
+    static constexpr int kB = PLANES == 1 ? HALF_BYTES : HALF_BYTES / 2;  // the most of one CTA's B in a stage and plane
+    static constexpr int kStage = PLANES * (HALF_BYTES + kB);
+    static constexpr int kSmem = 1024 + kStages * kStage + OUT_BYTES + 256;
+};
 
 struct FfMaps {
     CUtensorMap a[2], b[2], c[3];
@@ -50,7 +62,12 @@ struct FfTc {
     int bn, act;
     long long items;
     const void *bias0, *bias1;
-    float *gate, *up;  // saved: written (FF_GATE) or read (FF_GATE_BACK)
+    int bias_wide;            // the biases can be read in 16-byte vectors
+    float *gate, *up;         // saved: written (FF_GATE) or read (FF_GATE_BACK)
+    int saved_wide;           // in float4
+    void *c0, *c1;            // FF_STORE: destinations that are stored to without TMA (else null)
+    int64_t ldc;
+    int c_wide;               // in 16-byte vectors
     float *part;
     int *status;
 };
@@ -72,14 +89,16 @@ __device__ __forceinline__ void arrive_remote(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // into this CTA's shared memory, reported to the first CTA's barrier
-__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
+__device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(x), "r"(y)
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
-__device__ __forceinline__ void store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y)
+__device__ __forceinline__ void store_3d(const CUtensorMap *map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y),
+                 "r"(z)
                  : "memory");
 }
 __device__ __forceinline__ void pair_commit(uint32_t bar) {  // arrives at the barrier of both CTAs
@@ -133,7 +152,7 @@ struct Outlet {
         return p;
     }
     template <typename T>
-    __device__ __forceinline__ void put(const CUtensorMap *map, const float (&v)[32], int x, int y, int lane) {
+    __device__ __forceinline__ void put(const CUtensorMap *map, const float (&v)[32], int x, int y, int z, int lane) {
         const uint32_t p = open();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -150,57 +169,139 @@ struct Outlet {
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) {
-            store_2d(map, p, x, y);
-        }
+        if (lane == 0) store_3d(map, p, x, y, z);
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // one group a piece in every lane, so that all count alike
     }
 };
 
-// 32 columns from n on of a 16-byte aligned vector of n_end (a multiple of 8) values, added to v
+// the values of the vector's columns from n on, added to v
 template <typename T>
-__device__ __forceinline__ void add_bias(const void *bias, int n, int n_end, float (&v)[32]) {
+__device__ __forceinline__ void add_bias(const void *bias, int wide, int n, int n_end, float (&v)[32]) {
+    constexpr int VEC = 16 / sizeof(T);
     if (bias == nullptr) return;
+    if (wide && n + 32 <= n_end) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (n + 8 * i >= n_end) break;
-        float f[8];
-        Vec<T, 8>::load((const T *)bias + n + 8 * i).unpack(f);
+        for (int i = 0; i < 32; i += VEC) {
+            float f[VEC];
+            Vec<T, VEC>::load((const T *)bias + n + i).unpack(f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[8 * i + j] += f[j];
+            for (int j = 0; j < VEC; ++j) v[i + j] += f[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (n + i < n_end) v[i] += Elem<T>::load(((const T *)bias)[n + i]);
     }
 }
 
-template <int ACT>
-__device__ __forceinline__ void gate_values(const float (&g)[32], const float (&u)[32], float (&h)[32]) {
+// 32 columns of one row, from n on
+template <typename T>
+__device__ __forceinline__ void store_row(T *row, int wide, int n, int n_end, const float (&v)[32]) {
+    constexpr int VEC = 16 / sizeof(T);
+    if (wide && n + 32 <= n_end) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) h[j] = act_value<ACT, false>(g[j]) * u[j];
+        for (int i = 0; i < 32; i += VEC) {
+            float f[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = v[i + j];
+            Vec<T, VEC> w;
+            w.pack(f);
+            w.store(row + n + i);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (n + i < n_end) row[n + i] = Elem<T>::store(v[i]);
+    }
 }
-template <int ACT>
+
+// 32 saved values of the row y + lane, from column x on (ff_saved_at)
+template <bool STORE>
+__device__ __forceinline__ void saved_row(const FfTc &P, float *base, int y, int lane, int x, float (&v)[32]) {
+    const int block_rows = min(32, P.m - y);
+    if (P.saved_wide) {
+        float4 *p = (float4 *)(base + (size_t)y * P.n) + (size_t)(x / 4) * block_rows + lane;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (x + 4 * j >= P.n) break;
+            if (STORE) {
+                p[(size_t)j * block_rows] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            } else {
+                const float4 f = __ldg(p + (size_t)j * block_rows);
+                v[4 * j] = f.x, v[4 * j + 1] = f.y, v[4 * j + 2] = f.z, v[4 * j + 3] = f.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if (x + j >= P.n) break;
+            float *p = base + ff_saved_at(y + lane, x + j, P.m, P.n);
+            if (STORE)
+                *p = v[j];
+            else
+                v[j] = __ldg(p);
+        }
+    }
+}
+
+// to a matrix that a product will read again: one plane of 16 bits, or the three bf16 parts
+template <typename OT, int PLANES>
+__device__ __forceinline__ void put_planes(Outlet &out, const CUtensorMap *map, float (&v)[32], int x, int y, int lane) {
+    if constexpr (PLANES == 1) {
+        out.put<OT>(map, v, x, y, 0, lane);
+    } else {
+        float part[32];
+#pragma unroll
+        for (int z = 0; z < 3; ++z) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                part[j] = z < 2 ? bf16_part(v[j]) : v[j];
+                v[j] = fabsf(part[j]) <= 3.4028234e38f ? v[j] - part[j] : 0.0f;
+            }
+            out.put<OT>(map, part, x, y, z, lane);
+        }
+    }
+}
+
+template <int ACT, bool kExact>
+__device__ __forceinline__ void gate_values(float (&g)[32], const float (&u)[32]) {  // in: g, u; out: h in g
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        const float2 h = split(mul2(act_value2<ACT, kExact>(pair(g[j], g[j + 1])), pair(u[j], u[j + 1])));
+        g[j] = h.x, g[j + 1] = h.y;
+    }
+}
+template <int ACT, bool kExact>
 __device__ __forceinline__ void gate_back_values(float (&g)[32], float (&u)[32], float (&dh)[32]) {
     // in: g, u, dh; out: dg, du, h
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        float a, d;
-        act_both<ACT, false>(g[j], a, d);
-        g[j] = dh[j] * u[j] * d;
-        const float h = a * u[j];
-        u[j] = dh[j] * a;
-        dh[j] = h;
+    for (int j = 0; j < 32; j += 2) {
+        Pair a, d;
+        act_both2<ACT, kExact>(pair(g[j], g[j + 1]), a, d);
+        const Pair up = pair(u[j], u[j + 1]), e = pair(dh[j], dh[j + 1]);
+        const float2 dg = split(mul2(mul2(e, up), d)), du = split(mul2(e, a)), h = split(mul2(a, up));
+        g[j] = dg.x, g[j + 1] = dg.y;
+        u[j] = du.x, u[j + 1] = du.y;
+        dh[j] = h.x, dh[j + 1] = h.y;
     }
 }
 
-template <typename T, bool A_BY_K, bool B_BY_K, int KIND>
+// OT: type of the operands.  T: of biases and of what FF_STORE stores.
+template <typename OT, typename T, int PLANES, bool A_BY_K, bool B_BY_K, int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     ff_tc_kernel(const __grid_constant__ FfMaps maps, const FfTc P) {
+    using R = Ring<PLANES>;
+    constexpr bool kExact = PLANES == 3;
+    constexpr int kStages = R::kStages;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-    const uint32_t out_base = smem + RING_BYTES;
+    const uint32_t out_base = smem + kStages * R::kStage;
     const uint32_t bars = out_base + OUT_BYTES;
     auto bar_full = [&](int s) { return bars + 8 * s; };
-    auto bar_empty = [&](int s) { return bars + 8 * (FF_STAGES + s); };
-    auto bar_acc_full = [&](int a) { return bars + 8 * (2 * FF_STAGES + a); };
-    auto bar_acc_empty = [&](int a) { return bars + 8 * (2 * FF_STAGES + 2 + a); };
+    auto bar_empty = [&](int s) { return bars + 8 * (kStages + s); };
+    auto bar_acc_full = [&](int a) { return bars + 8 * (2 * kStages + a); };
+    auto bar_acc_empty = [&](int a) { return bars + 8 * (2 * kStages + 2 + a); };
+    auto bar_small_empty = [&](int a) { return bars + 8 * (2 * kStages + 4 + a); };  // three planes: the small products' accumulators
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
@@ -208,22 +309,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
-    const uint32_t b_bytes = (uint32_t)P.bn / 2 * 128;  // this CTA's share of B in a stage
+    const uint32_t b_bytes = (uint32_t)P.bn / 2 * 128;  // this CTA's share of B in a stage and plane
+    const uint32_t tmem_cols = PLANES == 1 ? 2 * P.bn : 4 * P.bn;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < FF_STAGES; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             mbar_init(bar_full(s), 1);
             mbar_init(bar_empty(s), 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(bar_acc_full(a), 1);
             mbar_init(bar_acc_empty(a), 2 * EPI_WARPS);
+            mbar_init(bar_small_empty(a), 2 * EPI_WARPS);
         }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(2 * P.bn)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(tmem_cols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
@@ -234,11 +337,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     const uint32_t tmem = tmem_slot;
     pdl_wait();
 
-    auto decode = [&](long long item, int &mt, int &nt, int &split) {
+    auto decode = [&](long long item, int &mt, int &nt, int &share) {
         nt = (int)(item % P.n_tiles);
         const long long rest = item / P.n_tiles;
         mt = P.skip + (int)(rest % P.live_tiles);
-        split = (int)(rest / P.live_tiles);
+        share = (int)(rest / P.live_tiles);
     };
 
     if (warp == 0) {
@@ -246,174 +349,221 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
             int g = 0;
             bool ok = true;
             for (long long item = first; item < P.items && ok; item += step) {
-                int mt, nt, split;
-                decode(item, mt, nt, split);
+                int mt, nt, share;
+                decode(item, mt, nt, share);
                 const int dest = mt / P.dest_tiles;
                 const int m0 = (mt - dest * P.dest_tiles) * 256 + (int)rank * 128;
                 const int n0 = KIND == FF_GATE ? nt * (P.bn / 2) : nt * P.bn + (int)rank * (P.bn / 2);
-                const int lo = split * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
+                const int lo = share * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
                 for (int kb = lo; kb < hi; ++kb, ++g) {
-                    const int s = g % FF_STAGES;
-                    if (!mbar_wait(bar_empty(s), ((g / FF_STAGES) & 1) ^ 1, abort_flag, P.status)) {
+                    const int s = g % kStages;
+                    if (!mbar_wait(bar_empty(s), ((g / kStages) & 1) ^ 1, abort_flag, P.status)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t a_at = smem + s * 2 * HALF_BYTES, b_at = a_at + HALF_BYTES;
+                    const uint32_t a_at = smem + s * R::kStage, b_at = a_at + PLANES * HALF_BYTES;
                     const uint32_t full = first_cta(bar_full(s));
-                    if (rank == 0) mbar_expect_tx(bar_full(s), 2 * (HALF_BYTES + b_bytes));
+                    if (rank == 0) mbar_expect_tx(bar_full(s), 2 * PLANES * (HALF_BYTES + b_bytes));
                     const int second = kb >= P.kb_first;
                     const int k0 = (second ? kb - P.kb_first : kb) * KB;
                     const CUtensorMap *am = &maps.a[A_BY_K ? second : dest];
                     const CUtensorMap *bm = &maps.b[KIND == FF_GATE ? (int)rank : second];
-                    if (A_BY_K) {
-                        pair_load_2d(a_at, am, full, k0, m0);
-                    } else {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) pair_load_2d(a_at + i * KB * 128, am, full, m0 + 64 * i, k0);
-                    }
-                    if (B_BY_K) {
-                        pair_load_2d(b_at, bm, full, k0, n0);
-                    } else {
-                        for (int i = 0; i < P.bn / 128; ++i) pair_load_2d(b_at + i * KB * 128, bm, full, n0 + 64 * i, k0);
+                    for (int z = 0; z < PLANES; ++z) {
+                        const uint32_t az = a_at + z * HALF_BYTES, bz = b_at + z * R::kB;
+                        if (A_BY_K) {
+                            pair_load(az, am, full, k0, m0, z);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) pair_load(az + i * KB * 128, am, full, m0 + 64 * i, k0, z);
+                        }
+                        if (B_BY_K) {
+                            pair_load(bz, bm, full, k0, n0, z);
+                        } else {
+                            for (int i = 0; i < P.bn / 128; ++i) pair_load(bz + i * KB * 128, bm, full, n0 + 64 * i, k0, z);
+                        }
                     }
                 }
             }
             // the other CTA's last releases have arrived here before this one may end
-            for (int i = 0; i < FF_STAGES && ok; ++i, ++g)
-                ok = mbar_wait(bar_empty(g % FF_STAGES), ((g / FF_STAGES) & 1) ^ 1, abort_flag, P.status);
+            for (int i = 0; i < kStages && ok; ++i, ++g)
+                ok = mbar_wait(bar_empty(g % kStages), ((g / kStages) & 1) ^ 1, abort_flag, P.status);
         }
     } else if (warp == 1) {
         if (rank == 0 && lane == 0) {
-            constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+            constexpr uint32_t type = std::is_same<OT, __nv_bfloat16>::value ? 1 : 0;
             const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((A_BY_K ? 0u : 1u) << 15) | ((B_BY_K ? 0u : 1u) << 16) |
                                    ((uint32_t)(P.bn >> 3) << 17) | ((256u >> 4) << 24);
-            int g = 0, t = 0;
+            int g = 0, t = 0, c = 0;  // k-blocks, tiles and accumulators so far
             bool ok = true;
             for (long long item = first; item < P.items && ok; item += step, ++t) {
-                int mt, nt, split;
-                decode(item, mt, nt, split);
-                const int lo = split * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
-                const int acc = t & 1;
-                if (!mbar_wait(bar_acc_empty(acc), ((t >> 1) & 1) ^ 1, abort_flag, P.status)) break;
-                tc_fence_after();
-                const uint32_t d = tmem + acc * P.bn;
-                for (int kb = lo; kb < hi; ++kb, ++g) {
-                    const int s = g % FF_STAGES;
-                    if (!mbar_wait(bar_full(s), (g / FF_STAGES) & 1, abort_flag, P.status)) {
+                int mt, nt, share;
+                decode(item, mt, nt, share);
+                const int lo = share * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
+                const uint32_t small = tmem + (2 + (t & 1)) * P.bn;
+                if (PLANES == 3 && !mbar_wait(bar_small_empty(t & 1), ((t >> 1) & 1) ^ 1, abort_flag, P.status)) break;
+                for (int k_lo = lo; k_lo < hi && ok; k_lo += PLANES == 3 ? CHUNK : hi - lo, ++c) {
+                    const int k_hi = PLANES == 3 ? min(hi, k_lo + CHUNK) : hi, acc = c & 1;
+                    if (!mbar_wait(bar_acc_empty(acc), ((c >> 1) & 1) ^ 1, abort_flag, P.status)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a_at = smem + s * 2 * HALF_BYTES, b_at = a_at + HALF_BYTES;
+                    const uint32_t d = tmem + acc * P.bn;
+                    for (int kb = k_lo; kb < k_hi; ++kb, ++g) {
+                        const int s = g % kStages;
+                        if (!mbar_wait(bar_full(s), (g / kStages) & 1, abort_flag, P.status)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t a_at = smem + s * R::kStage, b_at = a_at + PLANES * HALF_BYTES;
 #pragma unroll
-                    for (int k = 0; k < KB / 16; ++k)  // 16 steps: 32 bytes along a row, or 16 rows
-                        pair_mma(d, operand<A_BY_K>(a_at + k * (A_BY_K ? 32 : 2048)), operand<B_BY_K>(b_at + k * (B_BY_K ? 32 : 2048)),
-                                 idesc, kb > lo || k > 0);
-                    pair_commit(bar_empty(s));
+                        for (int k = 0; k < KB / 16; ++k) {  // 16 steps: 32 bytes along a row, or 16 rows
+                            auto a = [&](int z) { return operand<A_BY_K>(a_at + z * HALF_BYTES + k * (A_BY_K ? 32 : 2048)); };
+                            auto b = [&](int z) { return operand<B_BY_K>(b_at + z * R::kB + k * (B_BY_K ? 32 : 2048)); };
+                            pair_mma(d, a(0), b(0), idesc, kb > k_lo || k > 0);
+                            if (PLANES == 3) {
+                                pair_mma(small, a(0), b(1), idesc, kb > lo || k > 0);
+                                pair_mma(small, a(1), b(0), idesc, 1);
+                                pair_mma(small, a(0), b(2), idesc, 1);
+                                pair_mma(small, a(2), b(0), idesc, 1);
+                                pair_mma(small, a(1), b(1), idesc, 1);
+                            }
+                        }
+                        pair_commit(bar_empty(s));
+                    }
+                    if (ok) pair_commit(bar_acc_full(acc));
                 }
-                if (ok) pair_commit(bar_acc_full(acc));
             }
         }
     } else {
         const int quad = warp & 3, half = (warp - 2) >> 2;  // tensor memory lanes of this warp; every second column piece
         Outlet out = {out_base + (uint32_t)(warp - 2) * PIECES * PIECE, 0};
         const int cols = KIND == FF_GATE ? P.bn / 2 : P.bn;  // output columns of a tile
-        int t = 0;
-        for (long long item = first; item < P.items; item += step, ++t) {
-            int mt, nt, split;
-            decode(item, mt, nt, split);
+        int t = 0, c = 0;
+        bool ok = true;
+        for (long long item = first; item < P.items && ok; item += step, ++t) {
+            int mt, nt, share;
+            decode(item, mt, nt, share);
             const int dest = mt / P.dest_tiles;
             const int y = (mt - dest * P.dest_tiles) * 256 + (int)rank * 128 + quad * 32;  // the warp's first row
-            const int acc = t & 1;
-            if (!mbar_wait(bar_acc_full(acc), (t >> 1) & 1, abort_flag, P.status)) break;
-            tc_fence_after();
-            const uint32_t d = tmem + acc * P.bn + ((uint32_t)(quad * 32) << 16);
-            const int row = y + lane, block_rows = min(32, P.m - y);  // of the block of 32 rows in the saved layout
-            for (int c = half * 32; c < cols; c += 64) {
-                const int x = nt * cols + c;
-                if (x >= P.n || y >= P.m) break;
+            const int row = y + lane;
+            const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+            auto fetch = [&](uint32_t at, float (&v)[32], bool add) {
                 uint32_t r[32];
-                float v[32];
-                tmem_ld32(d + c, r);
+                tmem_ld32(at + lanes, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = add ? v[j] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
+            };
+            // 32 columns from x on: v the product; FF_GATE: v the gate's, u the up projection's
+            auto emit = [&](int x, float (&v)[32], float (&u)[32]) {
+                if (x >= P.n || y >= P.m) return;
                 if (KIND == FF_GATE) {
-                    uint32_t r2[32];
-                    float u[32];
-                    tmem_ld32(d + cols + c, r2);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]), u[j] = __uint_as_float(r2[j]);
-                    add_bias<T>(P.bias0, x, P.n, v);
-                    add_bias<T>(P.bias1, x, P.n, u);
+                    add_bias<T>(P.bias0, P.bias_wide, x, P.n, v);
+                    add_bias<T>(P.bias1, P.bias_wide, x, P.n, u);
                     if (P.gate != nullptr && row < P.m) {
-                        float4 *gs = (float4 *)(P.gate + (size_t)y * P.n) + (size_t)(x / 4) * block_rows + lane;
-                        float4 *us = (float4 *)(P.up + (size_t)y * P.n) + (size_t)(x / 4) * block_rows + lane;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (x + 4 * j >= P.n) break;
-                            gs[(size_t)j * block_rows] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                            us[(size_t)j * block_rows] = make_float4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
-                        }
+                        saved_row<true>(P, P.gate, y, lane, x, v);
+                        saved_row<true>(P, P.up, y, lane, x, u);
                     }
-                    float h[32];
                     switch (P.act) {
-                        case FC_ACT_RELU: gate_values<FC_ACT_RELU>(v, u, h); break;
-                        case FC_ACT_SILU: gate_values<FC_ACT_SILU>(v, u, h); break;
-                        case FC_ACT_GELU: gate_values<FC_ACT_GELU>(v, u, h); break;
-                        case FC_ACT_GELU_TANH: gate_values<FC_ACT_GELU_TANH>(v, u, h); break;
-                        case FC_ACT_SIGMOID: gate_values<FC_ACT_SIGMOID>(v, u, h); break;
-                        default: gate_values<FC_ACT_NONE>(v, u, h);
+                        case FC_ACT_RELU: gate_values<FC_ACT_RELU, kExact>(v, u); break;
+                        case FC_ACT_SILU: gate_values<FC_ACT_SILU, kExact>(v, u); break;
+                        case FC_ACT_GELU: gate_values<FC_ACT_GELU, kExact>(v, u); break;
+                        case FC_ACT_GELU_TANH: gate_values<FC_ACT_GELU_TANH, kExact>(v, u); break;
+                        case FC_ACT_SIGMOID: gate_values<FC_ACT_SIGMOID, kExact>(v, u); break;
+                        default: gate_values<FC_ACT_NONE, kExact>(v, u);
                     }
-                    out.put<T>(&maps.c[0], h, x, y, lane);
+                    put_planes<OT, PLANES>(out, &maps.c[0], v, x, y, lane);
                 } else if (KIND == FF_GATE_BACK) {
-                    float g[32], u[32];
+                    float g[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) g[j] = u[j] = 0.0f;
                     if (row < P.m) {
-                        const float4 *gs = (const float4 *)(P.gate + (size_t)y * P.n) + (size_t)(x / 4) * block_rows + lane;
-                        const float4 *us = (const float4 *)(P.up + (size_t)y * P.n) + (size_t)(x / 4) * block_rows + lane;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (x + 4 * j >= P.n) break;
-                            const float4 a = __ldg(gs + (size_t)j * block_rows), b = __ldg(us + (size_t)j * block_rows);
-                            g[4 * j] = a.x, g[4 * j + 1] = a.y, g[4 * j + 2] = a.z, g[4 * j + 3] = a.w;
-                            u[4 * j] = b.x, u[4 * j + 1] = b.y, u[4 * j + 2] = b.z, u[4 * j + 3] = b.w;
-                        }
+                        saved_row<false>(P, P.gate, y, lane, x, g);
+                        saved_row<false>(P, P.up, y, lane, x, u);
                     }
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
                     switch (P.act) {
-                        case FC_ACT_RELU: gate_back_values<FC_ACT_RELU>(g, u, v); break;
-                        case FC_ACT_SILU: gate_back_values<FC_ACT_SILU>(g, u, v); break;
-                        case FC_ACT_GELU: gate_back_values<FC_ACT_GELU>(g, u, v); break;
-                        case FC_ACT_GELU_TANH: gate_back_values<FC_ACT_GELU_TANH>(g, u, v); break;
-                        case FC_ACT_SIGMOID: gate_back_values<FC_ACT_SIGMOID>(g, u, v); break;
-                        default: gate_back_values<FC_ACT_NONE>(g, u, v);
+                        case FC_ACT_RELU: gate_back_values<FC_ACT_RELU, kExact>(g, u, v); break;
+                        case FC_ACT_SILU: gate_back_values<FC_ACT_SILU, kExact>(g, u, v); break;
+                        case FC_ACT_GELU: gate_back_values<FC_ACT_GELU, kExact>(g, u, v); break;
+                        case FC_ACT_GELU_TANH: gate_back_values<FC_ACT_GELU_TANH, kExact>(g, u, v); break;
+                        case FC_ACT_SIGMOID: gate_back_values<FC_ACT_SIGMOID, kExact>(g, u, v); break;
+                        default: gate_back_values<FC_ACT_NONE, kExact>(g, u, v);
                     }
-                    out.put<T>(&maps.c[0], g, x, y, lane);
-                    out.put<T>(&maps.c[1], u, x, y, lane);
-                    out.put<T>(&maps.c[2], v, x, y, lane);
+                    put_planes<OT, PLANES>(out, &maps.c[0], g, x, y, lane);
+                    put_planes<OT, PLANES>(out, &maps.c[1], u, x, y, lane);
+                    put_planes<OT, PLANES>(out, &maps.c[2], v, x, y, lane);
+                } else if (P.splits > 1) {  // [share][block of 32 rows][4 columns][row]
+                    const int quads = (P.n + 3) / 4;
+                    const size_t block = ((size_t)share * P.m_tiles + mt) * 8 + rank * 4 + quad;
+                    float4 *ps = (float4 *)P.part + (block * quads + x / 4) * 32 + lane;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (x + 4 * j >= P.n) break;
+                        ps[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    }
                 } else {
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-                    if (P.splits > 1) {  // [share][block of 32 rows][4 columns][row]
-                        const size_t block = ((size_t)split * P.m_tiles + mt) * 8 + rank * 4 + quad;
-                        float4 *ps = (float4 *)P.part + (block * (P.n / 4) + x / 4) * 32 + lane;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (x + 4 * j >= P.n) break;
-                            ps[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                        }
-                    } else {
-                        add_bias<T>(P.bias0, x, P.n, v);
-                        out.put<T>(&maps.c[dest], v, x, y, lane);
+                    add_bias<T>(P.bias0, P.bias_wide, x, P.n, v);
+                    T *c = (T *)(dest ? P.c1 : P.c0);
+                    if (c != nullptr) {
+                        if (row < P.m) store_row(c + (size_t)row * P.ldc, P.c_wide, x, P.n, v);
+                    } else if constexpr (PLANES == 1) {
+                        out.put<OT>(&maps.c[dest], v, x, y, 0, lane);
                     }
                 }
+            };
+            if constexpr (PLANES == 1) {
+                const int acc = c & 1;
+                if (!mbar_wait(bar_acc_full(acc), (c >> 1) & 1, abort_flag, P.status)) break;
+                ++c;
+                tc_fence_after();
+                const uint32_t d = tmem + acc * P.bn;
+                for (int j = half * 32; j < cols; j += 64) {
+                    if (nt * cols + j >= P.n || y >= P.m) break;
+                    float v[32], u[32];
+                    fetch(d + j, v, false);
+                    if (KIND == FF_GATE) fetch(d + cols + j, u, false);
+                    emit(nt * cols + j, v, u);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_remote(first_cta(bar_acc_empty(acc)));
+            } else {
+                // bn = 128: this warp's two pieces, the gate's and the up projection's, or two neighbours
+                const int p0 = KIND == FF_GATE ? half * 32 : half * 64, p1 = KIND == FF_GATE ? 64 + half * 32 : half * 64 + 32;
+                const int lo = share * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
+                float v[32], u[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = u[j] = 0.0f;
+                for (int k = lo; k < hi; k += CHUNK, ++c) {
+                    const int acc = c & 1;
+                    ok = mbar_wait(bar_acc_full(acc), (c >> 1) & 1, abort_flag, P.status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    fetch(tmem + acc * P.bn + p0, v, true);
+                    fetch(tmem + acc * P.bn + p1, u, true);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_remote(first_cta(bar_acc_empty(acc)));
+                }
+                if (!ok) break;
+                // the last accumulator's barrier stood for the small products too
+                tc_fence_after();
+                fetch(tmem + (2 + (t & 1)) * P.bn + p0, v, true);
+                fetch(tmem + (2 + (t & 1)) * P.bn + p1, u, true);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_remote(first_cta(bar_small_empty(t & 1)));
+                if (KIND == FF_GATE) {
+                    emit(nt * cols + p0, v, u);
+                } else {
+                    float w[32];
+                    emit(nt * cols + p0, v, w);
+                    emit(nt * cols + p1, u, w);
+                }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_remote(first_cta(bar_acc_empty(acc)));
         }
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
@@ -426,15 +576,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     cluster_sync();
     if (warp == 1) {
         __syncwarp();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * P.bn) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
     }
 }
 
 // the shares of a split reduction, added in order; a thread has four columns of one row
 template <typename T>
-__global__ void __launch_bounds__(256) ff_tc_join_kernel(const FfTc P, T *c0, T *c1, int64_t ldc) {
+__global__ void __launch_bounds__(256) ff_tc_join_kernel(const FfTc P, T *c0, T *c1, int wide) {
     pdl_wait();
-    const int quads = P.n / 4, col_blocks = (quads + 3) / 4;
+    const int quads = (P.n + 3) / 4, col_blocks = (quads + 3) / 4;
     const long long blocks = (long long)P.m_tiles * 8 * col_blocks * 4;  // of 8 rows x 4 quads: a warp each
     for (long long w = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5; w < blocks; w += (long long)gridDim.x * 8) {
         const int lane = threadIdx.x & 31;
@@ -452,30 +602,36 @@ __global__ void __launch_bounds__(256) ff_tc_join_kernel(const FfTc P, T *c0, T 
             const float4 f = __ldg((const float4 *)P.part + (((size_t)s * P.m_tiles * 8 + block) * quads + q) * 32 + r);
             v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
         }
-        if (P.bias0) {
-            float b[4];
-            Vec<T, 4>::load((const T *)P.bias0 + 4 * q).unpack(b);
+        if (P.bias0)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += b[i];
+            for (int i = 0; i < 4; ++i)
+                if (4 * q + i < P.n) v[i] += Elem<T>::load(((const T *)P.bias0)[4 * q + i]);
+        T *to = c + (size_t)row * P.ldc + 4 * q;
+        if (wide && 4 * q + 4 <= P.n) {
+            Vec<T, 4> out;
+            out.pack(v);
+            out.store(to);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * q + i < P.n) to[i] = Elem<T>::store(v[i]);
         }
-        Vec<T, 4> out;
-        out.pack(v);
-        out.store(c + (size_t)row * ldc + 4 * q);
     }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
-// a matrix of 16-bit values, rows `ld` apart; box = box_cols x box_rows
-int matrix_map(CUtensorMap *map, int type, const void *base, long long cols, long long rows, int64_t ld, int box_cols, int box_rows) {
+// matrices of 16-bit values, rows `ld` apart, planes `plane` apart; box = box_cols x box_rows of one plane
+int matrix_map(CUtensorMap *map, bool bf16, const void *base, long long cols, long long rows, int64_t ld, int planes, int64_t plane,
+               int box_cols, int box_rows) {
     EncodeTiledFn enc;
     FC_PROPAGATE(get_encoder(&enc));
-    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(map, type == FC_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                           const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(planes > 1 ? plane : ld) * 2};
+    cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base),
+                           dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     FC_REQUIRE(r == CUDA_SUCCESS, FC_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d (%lld x %lld, rows %lld apart)", (int)r, rows, cols,
@@ -489,18 +645,21 @@ int matrix_map(CUtensorMap *map, int type, const void *base, long long cols, lon
 // pipe and (16 KB + 64 bn bytes) at about 56 bytes a clock of operand copies; the first tile's latency and a tile's epilogue
 // that nothing hides, about 2500; a split result is written and read once more by every share (about 3000 bytes a clock, all SMs),
 // and joined by a kernel of its own (about 4000).
-FfTcPlan ff_tc_plan(int kind, int dests, int m, int n, int kb_total, bool b_by_k) {
+struct FfTcPlan {
+    int bn, splits;
+};
+static FfTcPlan ff_tc_plan(int planes, int kind, int dests, int m, int n, int kb_total, bool b_by_k) {
     const int pairs = 74;
-    FfTcPlan best = {256, 1};
+    FfTcPlan best = {128, 1};
     double best_cost = 1e300;
-    for (int bn = 256; bn >= (b_by_k ? 64 : 128); bn /= 2) {
+    for (int bn = planes == 1 ? 256 : 128; bn >= (b_by_k && planes == 1 ? 64 : 128); bn /= 2) {
         const int cols = kind == FF_GATE ? bn / 2 : bn;
         const double tiles = (double)dests * ceil_div(m, 256) * ceil_div(n, cols);
         for (int s = 1; s <= (kind == FF_STORE ? 16 : 1); ++s) {
             if (s > 1 && kb_total / s < 4) break;
             const int share = (int)ceil_div(kb_total, s);
             if (s > 1 && (s - 1) * share >= kb_total) continue;  // the last share would be empty
-            const double copies = (16384.0 + 64.0 * bn) / 56.0, mma = 2.0 * bn;
+            const double copies = planes * (16384.0 + 64.0 * bn) / 56.0, mma = (planes == 1 ? 2.0 : 12.0) * bn;
             const double waves = (double)ceil_div((size_t)(tiles * s), pairs);
             double cost = waves * share * (copies > mma ? copies : mma) + 2500.0;
             if (s > 1) cost += 4000.0 + (double)s * dests * m * n * 8.0 / 3000.0;
@@ -521,29 +680,18 @@ static void tc_shape(const FfProduct &p, int *dests, int *m, int *kb_first, int 
 }
 
 size_t ff_tc_part_floats(const FfProduct &p) {
-    if (p.kind != FF_STORE) return 0;
+    if (p.kind != FF_STORE || p.m == 0 || p.k == 0) return 0;
     int dests, m, kb_first, kb_total;
     tc_shape(p, &dests, &m, &kb_first, &kb_total);
-    const FfTcPlan plan = ff_tc_plan(p.kind, dests, m, p.n, kb_total, p.b_by_k);
-    return plan.splits > 1 ? (size_t)plan.splits * dests * ceil_div(m, 256) * 256 * p.n : 0;
-}
-
-// what the copies need: rows that are multiples of 16 bytes, on 16-byte boundaries
-bool ff_tc_fits(const FfProduct &p) {
-    if (p.type == FC_DTYPE_F32 || p.m == 0 || p.k == 0) return false;
-    if (p.lda % 8 || p.ldb % 8 || p.ldc % 8 || p.n % 8) return false;
-    if (p.b_split < p.k && p.b_split % 8) return false;
-    if (p.row_split < p.m && p.row_split % 8) return false;
-    const void *all[] = {p.a, p.b0, p.b1, p.c0, p.c1, p.bias0, p.bias1, p.gate, p.up};
-    for (const void *q : all)
-        if (!aligned16(q)) return false;
-    return true;
+    const FfTcPlan plan = ff_tc_plan(p.planes, p.kind, dests, m, p.n, kb_total, p.b_by_k);
+    return plan.splits > 1 ? (size_t)plan.splits * dests * ceil_div(m, 256) * 256 * round_up(p.n, 4) : 0;
 }
 
 int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
     int dests, m, kb_first, kb_total;
     tc_shape(p, &dests, &m, &kb_first, &kb_total);
-    const FfTcPlan plan = ff_tc_plan(p.kind, dests, m, p.n, kb_total, p.b_by_k);
+    const FfTcPlan plan = ff_tc_plan(p.planes, p.kind, dests, m, p.n, kb_total, p.b_by_k);
+    const int vec = 16 / (int)dtype_size(p.type);
     FfTc P = {};
     P.m = m;
     P.n = p.n;
@@ -561,62 +709,77 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
     P.items = (long long)P.live_tiles * P.n_tiles * P.splits;
     P.bias0 = p.bias0;
     P.bias1 = p.bias1;
+    P.bias_wide = aligned16(p.bias0) && aligned16(p.bias1);
     P.gate = p.gate;
     P.up = p.up;
+    P.saved_wide = aligned16(p.gate) && p.n % 4 == 0;
+    P.ldc = p.ldc;
     P.part = p.part;
     P.status = ctx->d_status;
+    // FF_STORE goes through TMA where the destination allows it
+    const bool c_wide = p.ldc % vec == 0 && aligned16(p.c0) && aligned16(p.c1);
+    const bool by_copies = p.kind != FF_STORE || (p.planes == 1 && c_wide);
+    if (!by_copies) {
+        P.c0 = p.c0;
+        P.c1 = p.c1;
+        P.c_wide = c_wide;
+    }
 
     FfMaps maps;
     memset(&maps, 0, sizeof maps);
+    const bool bf16 = p.type != FC_DTYPE_F16;
     const uint8_t *a = (const uint8_t *)p.a;
     const int second = dests == 2 || p.b_split < p.k;
     for (int i = 0; i <= second; ++i) {  // A's columns (K-major: the reduction; MN-major: the rows of one destination)
         const int cols = p.a_by_k ? (i ? p.k - p.b_split : p.b_split) : m;
-        const int skip = i == 0 ? 0 : p.a_by_k ? p.b_split : m;
-        FC_PROPAGATE(matrix_map(&maps.a[i], p.type, a + (size_t)skip * 2, cols, p.a_by_k ? p.m : p.k, p.lda, 64, p.a_by_k ? 128 : KB));
+        FC_PROPAGATE(matrix_map(&maps.a[i], bf16, a + (i ? (size_t)p.a_skip * 2 : 0), cols, p.a_by_k ? p.m : p.k, p.lda, p.planes,
+                                p.a_plane, 64, p.a_by_k ? 128 : KB));
     }
     const void *b[2] = {p.b0, p.b1};
     for (int i = 0; i < 2 && b[i]; ++i) {
         const int k = p.kind == FF_GATE ? p.k : i ? p.k - p.b_split : p.b_split;
-        FC_PROPAGATE(p.b_by_k ? matrix_map(&maps.b[i], p.type, b[i], k, p.n, p.ldb, 64, plan.bn / 2)
-                              : matrix_map(&maps.b[i], p.type, b[i], p.n, k, p.ldb, 64, KB));
+        FC_PROPAGATE(p.b_by_k ? matrix_map(&maps.b[i], bf16, b[i], k, p.n, p.ldb, p.planes, p.b_plane, 64, plan.bn / 2)
+                              : matrix_map(&maps.b[i], bf16, b[i], p.n, k, p.ldb, p.planes, p.b_plane, 64, KB));
     }
-    void *c[3] = {p.c0, p.c1, nullptr};
-    if (p.kind == FF_GATE_BACK) {
-        c[1] = (uint8_t *)p.c0 + (size_t)p.n * 2;
-        c[2] = p.c1;
-    }
-    if (P.splits == 1)
+    if (by_copies && P.splits == 1) {
+        const void *c[3] = {p.c0, p.c1, nullptr};
+        if (p.kind == FF_GATE_BACK) {
+            c[1] = (const uint8_t *)p.c0 + (size_t)p.a_skip * 2;
+            c[2] = p.c1;
+        }
         for (int i = 0; i < 3; ++i)
-            if (c[i]) FC_PROPAGATE(matrix_map(&maps.c[i], p.type, c[i], p.n, m, i == 2 ? p.n : p.ldc, 32, 32));
+            if (c[i])
+                FC_PROPAGATE(matrix_map(&maps.c[i], bf16, c[i], p.n, m, i == 2 ? p.ldc1 : p.ldc, p.kind == FF_STORE ? 1 : p.planes,
+                                        i == 2 ? p.c1_plane : p.c_plane, 32, 32));
+    }
 
     long long pairs = ctx->sm_count / 2;
     if (pairs > P.items) pairs = P.items;
-    return with_type(p.type, [&](auto t) -> int {
+    auto run = [&](auto ot, auto t, auto planes) -> int {
+        using OT = decltype(ot);
         using T = decltype(t);
-        if constexpr (std::is_same<T, float>::value) {
-            set_error("fp32 has no tensor-core product");
-            return FC_ERR_UNSUPPORTED;
-        } else {
-            auto go = [&](auto kernel) -> int {
-                FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FF_SMEM));
-                FC_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(2 * pairs)), dim3(FF_TC_THREADS), FF_SMEM, ctx->stream, maps, P));
-                return FC_OK;
-            };
-            if (p.kind == FF_GATE) return go(ff_tc_kernel<T, true, true, FF_GATE>);
-            if (p.kind == FF_GATE_BACK) return go(ff_tc_kernel<T, true, false, FF_GATE_BACK>);
-            FC_PROPAGATE(!p.a_by_k  ? go(ff_tc_kernel<T, false, false, FF_STORE>)
-                         : p.b_by_k ? go(ff_tc_kernel<T, true, true, FF_STORE>)
-                                    : go(ff_tc_kernel<T, true, false, FF_STORE>));
-            if (P.splits > 1) {
-                long long blocks = ceil_div((size_t)P.m_tiles * 8 * 4 * ceil_div(p.n, 16), 8);
-                if (blocks > 148 * 8) blocks = 148 * 8;
-                FC_CHECK_CUDA(launch_pdl(ff_tc_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, P, (T *)p.c0,
-                                         (T *)p.c1, p.ldc));
-            }
+        constexpr int PLANES = decltype(planes)::value, SMEM = Ring<PLANES>::kSmem;
+        auto go = [&](auto kernel) -> int {
+            FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+            FC_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(2 * pairs)), dim3(FF_TC_THREADS), SMEM, ctx->stream, maps, P));
             return FC_OK;
+        };
+        if (p.kind == FF_GATE) return go(ff_tc_kernel<OT, T, PLANES, true, true, FF_GATE>);
+        if (p.kind == FF_GATE_BACK) return go(ff_tc_kernel<OT, T, PLANES, true, false, FF_GATE_BACK>);
+        FC_PROPAGATE(!p.a_by_k  ? go(ff_tc_kernel<OT, T, PLANES, false, false, FF_STORE>)
+                     : p.b_by_k ? go(ff_tc_kernel<OT, T, PLANES, true, true, FF_STORE>)
+                                : go(ff_tc_kernel<OT, T, PLANES, true, false, FF_STORE>));
+        if (P.splits > 1) {
+            long long blocks = ceil_div((size_t)P.m_tiles * 8 * 4 * ceil_div(p.n, 16), 8);
+            if (blocks > 148 * 8) blocks = 148 * 8;
+            FC_CHECK_CUDA(launch_pdl(ff_tc_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, P, (T *)p.c0, (T *)p.c1,
+                                     (int)c_wide));
         }
-    });
+        return FC_OK;
+    };
+    const std::integral_constant<int, 1> one;
+    if (p.planes == 3) return run(__nv_bfloat16(), float(), std::integral_constant<int, 3>());
+    return p.type == FC_DTYPE_BF16 ? run(__nv_bfloat16(), __nv_bfloat16(), one) : run(__half(), __half(), one);
 }
 
 }  // namespace fc

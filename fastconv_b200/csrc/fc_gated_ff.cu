@@ -6,8 +6,9 @@
 //
 // Forward: one kernel for both projections, the activation and the product; one for the way down.  Backward: one product
 // whose epilogue turns dh into dg, du and h (dh itself is never stored), then dx over the joined reduction [dg du], both
-// input weights' gradients as one product over [dg du]^T, and dWd.  h, dg and du are rounded to the block's type between the kernels, as
-// the tensor cores take them; every sum is fp32.
+// input weights' gradients as one product over [dg du]^T, and dWd.  h, dg and du are rounded to the block's type between
+// the kernels, as the tensor cores take them (fp32: three bf16 parts that hold all its bits); every sum is fp32, and so are the
+// saved g and u: rounding them would add a second rounding to dg, du and h.
 #include <type_traits>
 
 #include "fc_gated_ff.h"
@@ -21,20 +22,67 @@ using namespace last;
 
 constexpr int JOIN_THREADS = 256;
 
-// ---- the shares of a split reduction, added in order --------------------------------------------------------------
+// ---- operands that the tensor cores' copies cannot take as they lie ------------------------------------------------
+// fp32, which is split into three bf16 planes, and rows that are no multiples of 16 bytes.  One launch for all of a call's.
+struct PackItem {
+    const void *src;
+    int64_t ld;
+    int rows, cols, wide;  // wide: the source can be read in 16-byte vectors
+    uint16_t *dst;
+    int64_t ldp, plane;
+    long long end;  // vectors of 8 of this item and those before it
+};
+struct PackList {
+    PackItem item[5];
+    int count;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(JOIN_THREADS) ff_join_kernel(const float *__restrict__ part, const FfProduct p) {
+__global__ void __launch_bounds__(256) ff_pack_kernel(const PackList list) {
+    constexpr int VEC = 16 / sizeof(T), PLANES = sizeof(T) == 4 ? 3 : 1;
     pdl_wait();
-    const int64_t total = (int64_t)p.m * p.n;
-    for (int64_t i = (int64_t)blockIdx.x * JOIN_THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * JOIN_THREADS) {
-        float v = 0.0f;
-        for (int s = 0; s < p.splits; ++s) v += part[s * total + i];
-        const int64_t m = i / p.n, n = i - m * p.n;
-        const bool second = m >= p.row_split;
-        T *c = (T *)(second ? p.c1 : p.c0);
-        if (c == nullptr) continue;
-        if (p.bias0) v += Elem<T>::load(((const T *)p.bias0)[n]);
-        c[(second ? m - p.row_split : m) * p.ldc + n] = Elem<T>::store(v);
+    const long long total = list.item[list.count - 1].end;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        int k = 0;
+        while (i >= list.item[k].end) ++k;
+        const PackItem &p = list.item[k];
+        const long long at = i - (k ? list.item[k - 1].end : 0);
+        const int per_row = (int)(p.ldp >> 3);
+        const long long row = at / per_row;
+        const int c = (int)(at - row * per_row) * 8;
+        const T *src = (const T *)p.src + row * p.ld + c;
+        float v[8];
+        if (p.wide && c + 8 <= p.cols) {
+#pragma unroll
+            for (int j = 0; j < 8; j += VEC) {
+                float f[VEC];
+                Vec<T, VEC>::load(src + j).unpack(f);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[j + e] = f[e];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = c + j < p.cols ? Elem<T>::load(src[j]) : 0.0f;
+        }
+        uint16_t *dst = p.dst + row * p.ldp + c;
+        if constexpr (PLANES == 1) {
+            Vec<T, 8> out;
+            out.pack(v);
+            out.store(dst);
+        } else {
+#pragma unroll
+            for (int z = 0; z < 3; ++z) {
+                Vec<__nv_bfloat16, 8> out;
+                float part[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    part[j] = z < 2 ? bf16_part(v[j]) : v[j];
+                    v[j] = fabsf(part[j]) <= 3.4028234e38f ? v[j] - part[j] : 0.0f;
+                }
+                out.pack(part);
+                out.store(dst + z * p.plane);
+            }
+        }
     }
 }
 
@@ -42,9 +90,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) ff_join_kernel(const float *__re
 constexpr int SUM_COLS = 32, SUM_ROWS = 8;
 
 // part[chunk][n]: the sum of the chunk's rows
-template <typename T>
-__global__ void __launch_bounds__(SUM_COLS *SUM_ROWS) ff_colsum_kernel(const T *__restrict__ a, int64_t lda, int rows, int n,
-                                                                      int chunk_rows, float *__restrict__ part) {
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(SUM_COLS *SUM_ROWS) ff_colsum_kernel(const T *__restrict__ a, int64_t lda, int64_t plane, int rows,
+                                                                      int n, int chunk_rows, float *__restrict__ part) {
     __shared__ float s[SUM_ROWS][SUM_COLS];
     pdl_wait();
     const int tx = threadIdx.x % SUM_COLS, ty = threadIdx.x / SUM_COLS;
@@ -52,7 +100,12 @@ __global__ void __launch_bounds__(SUM_COLS *SUM_ROWS) ff_colsum_kernel(const T *
     const int64_t r0 = (int64_t)blockIdx.y * chunk_rows, r1 = min((int64_t)rows, r0 + chunk_rows);
     float v = 0.0f;
     if (c < n)
-        for (int64_t r = r0 + ty; r < r1; r += SUM_ROWS) v += Elem<T>::load(a[r * lda + c]);
+        for (int64_t r = r0 + ty; r < r1; r += SUM_ROWS) {
+            float t = Elem<T>::load(a[r * lda + c]);
+#pragma unroll
+            for (int z = 1; z < PLANES; ++z) t += Elem<T>::load(a[z * plane + r * lda + c]);
+            v += t;
+        }
     s[ty][tx] = v;
     __syncthreads();
     if (ty == 0 && c < n) {
@@ -63,15 +116,14 @@ __global__ void __launch_bounds__(SUM_COLS *SUM_ROWS) ff_colsum_kernel(const T *
 }
 
 template <typename T>
-__global__ void __launch_bounds__(JOIN_THREADS) ff_colsum_join_kernel(const float *__restrict__ part, int n, int chunks, int split,
-                                                                     T *__restrict__ out0, T *__restrict__ out1) {
+__global__ void __launch_bounds__(JOIN_THREADS) ff_colsum_join_kernel(const float *__restrict__ part, int n, int chunks,
+                                                                     T *__restrict__ out) {
     pdl_wait();
     const int64_t c = (int64_t)blockIdx.x * JOIN_THREADS + threadIdx.x;
     if (c >= n) return;
     float v = 0.0f;
     for (int i = 0; i < chunks; ++i) v += part[(size_t)i * n + c];
-    T *out = c < split ? out0 : out1;
-    if (out) out[c < split ? c : c - split] = Elem<T>::store(v);
+    out[c] = Elem<T>::store(v);
 }
 
 int colsum_chunks(int rows, int n) {
@@ -82,18 +134,22 @@ int colsum_chunks(int rows, int n) {
     return chunks < 1 ? 1 : (int)chunks;
 }
 
-// out0[c] (c < split) and out1[c - split] = sums of a's columns; part: colsum_chunks * n floats
-int colsum(fc_context *ctx, int type, const void *a, int64_t lda, int rows, int n, int split, void *out0, void *out1, float *part) {
+// out[c] = the sum of column c of a, which is of `type` or, where plane > 0, the sum of three bf16 planes;
+// part: colsum_chunks * n floats
+int colsum(fc_context *ctx, int type, const void *a, int64_t lda, int64_t plane, int rows, int n, void *out, float *part) {
     const int want = colsum_chunks(rows, n);
-    const int chunk_rows = rows > 0 ? (int)ceil_div(rows, want) : 1;
-    const int chunks = rows > 0 ? (int)ceil_div(rows, chunk_rows) : 0;
+    const int chunk_rows = (int)ceil_div(rows, want), chunks = (int)ceil_div(rows, chunk_rows);
+    const dim3 grid((unsigned)ceil_div(n, SUM_COLS), chunks), block(SUM_COLS * SUM_ROWS);
     return with_type(type, [&](auto t) -> int {
         using T = decltype(t);
-        if (chunks > 0)
-            FC_CHECK_CUDA(launch_pdl(ff_colsum_kernel<T>, dim3((unsigned)ceil_div(n, SUM_COLS), chunks), dim3(SUM_COLS * SUM_ROWS), 0,
-                                     ctx->stream, (const T *)a, lda, rows, n, chunk_rows, part));
+        if (plane > 0)
+            FC_CHECK_CUDA(launch_pdl(ff_colsum_kernel<__nv_bfloat16, 3>, grid, block, 0, ctx->stream, (const __nv_bfloat16 *)a, lda,
+                                     plane, rows, n, chunk_rows, part));
+        else
+            FC_CHECK_CUDA(launch_pdl(ff_colsum_kernel<T, 1>, grid, block, 0, ctx->stream, (const T *)a, lda, plane, rows, n, chunk_rows,
+                                     part));
         FC_CHECK_CUDA(launch_pdl(ff_colsum_join_kernel<T>, dim3((unsigned)ceil_div(n, JOIN_THREADS)), dim3(JOIN_THREADS), 0, ctx->stream,
-                                 (const float *)part, n, chunks, split, (T *)out0, (T *)out1));
+                                 (const float *)part, n, chunks, (T *)out));
         return FC_OK;
     });
 }
@@ -120,67 +176,85 @@ int block_of(const fc_gated_ff_desc *d, Block *b) {
     return FC_OK;
 }
 
-FfProduct product(const Block &b, int kind, int m, int n, int k, const void *a, int64_t lda, bool a_by_k, const void *b0,
-                  int64_t ldb, bool b_by_k, void *c0, int64_t ldc) {
+// A matrix as a product reads it: 16-bit values in rows of a multiple of 8, one plane or three.
+struct Matrix {
+    const void *p;
+    int64_t ld, plane;
+};
+
+FfProduct product(const Block &b, int kind, int m, int n, int k, const Matrix &a, bool a_by_k, const Matrix &b0, bool b_by_k) {
     FfProduct p = {};
     p.type = b.type; p.act = b.act; p.kind = kind;
+    p.planes = b.type == FC_DTYPE_F32 ? 3 : 1;
     p.m = m; p.n = n; p.k = k;
-    p.a = a; p.lda = lda; p.a_by_k = a_by_k;
-    p.b0 = b0; p.ldb = ldb; p.b_by_k = b_by_k; p.b_split = k;
-    p.c0 = c0; p.ldc = ldc; p.row_split = m;
-    p.splits = 1;
+    p.a = a.p; p.lda = a.ld; p.a_plane = a.plane; p.a_by_k = a_by_k;
+    p.b0 = b0.p; p.ldb = b0.ld; p.b_plane = b0.plane; p.b_by_k = b_by_k;
+    p.b_split = k;
+    p.row_split = m;
     return p;
 }
 
 // the block's FF_STORE products
-FfProduct down_product(const Block &b, const void *h, const void *w_down, const void *bias, void *y) {
-    FfProduct p = product(b, FF_STORE, b.rows, b.out, b.hidden, h, b.hidden, true, w_down, b.hidden, true, y, b.ys);
+FfProduct down_product(const Block &b, const Matrix &h, const Matrix &w_down, const void *bias, void *y) {
+    FfProduct p = product(b, FF_STORE, b.rows, b.out, b.hidden, h, true, w_down, true);
     p.bias0 = bias;
+    p.c0 = y; p.ldc = b.ys;
     return p;
 }
-FfProduct dx_product(const Block &b, const void *dgu, const void *w_gate, const void *w_up, void *dx) {
-    FfProduct p = product(b, FF_STORE, b.rows, b.in, 2 * b.hidden, dgu, 2 * (int64_t)b.hidden, true, w_gate, b.in, false, dx, b.xs);
+FfProduct dx_product(const Block &b, const Matrix &dgu, const Matrix &w_gate, const void *w_up, void *dx) {
+    FfProduct p = product(b, FF_STORE, b.rows, b.in, 2 * b.hidden, dgu, true, w_gate, false);
+    p.a_skip = dgu.ld / 2;
     p.b1 = w_up;
     p.b_split = b.hidden;
+    p.c0 = dx; p.ldc = b.xs;
     return p;
 }
-FfProduct dw_in_product(const Block &b, const void *dgu, const void *x, void *dw_gate, void *dw_up) {
-    FfProduct p =
-        product(b, FF_STORE, 2 * b.hidden, b.in, b.rows, dgu, 2 * (int64_t)b.hidden, false, x, b.xs, false, dw_gate, b.in);
-    p.c1 = dw_up;
+FfProduct dw_in_product(const Block &b, const Matrix &dgu, const Matrix &x, void *dw_gate, void *dw_up) {
+    FfProduct p = product(b, FF_STORE, 2 * b.hidden, b.in, b.rows, dgu, false, x, false);
+    p.a_skip = dgu.ld / 2;
     p.row_split = b.hidden;
+    p.c0 = dw_gate; p.c1 = dw_up; p.ldc = b.in;
     return p;
 }
-FfProduct dw_down_product(const Block &b, const void *dy, const void *h, void *dw_down) {
-    return product(b, FF_STORE, b.out, b.hidden, b.rows, dy, b.ys, false, h, b.hidden, false, dw_down, b.hidden);
+FfProduct dw_down_product(const Block &b, const Matrix &dy, const Matrix &h, void *dw_down) {
+    FfProduct p = product(b, FF_STORE, b.out, b.hidden, b.rows, dy, false, h, false);
+    p.c0 = dw_down; p.ldc = b.hidden;
+    return p;
 }
 
+// The workspace: h, [dg du], packed copies of the operands (whether they are needed depends on the call's addresses too), and
+// the shares of split reductions and column sums.
 struct Work {
-    uint8_t *h, *dgu;
+    Matrix h, dgu, x, dy, w_gate, w_up, w_down;
     float *part;
     size_t bytes;
 };
 
 Work carve(const Block &b, void *base, bool backward) {
     Carver c = {(uint8_t *)base, 0};
-    const size_t e = dtype_size(b.type), rh = (size_t)b.rows * b.hidden;
+    const int planes = b.type == FC_DTYPE_F32 ? 3 : 1;
+    auto matrix = [&](int64_t rows, int64_t ld) {
+        const int64_t plane = rows * ld;
+        return Matrix{c.take<uint16_t>((size_t)plane * planes), ld, plane};
+    };
+    const int64_t in = round_up(b.in, 8), hidden = round_up(b.hidden, 8), out = round_up(b.out, 8);
     Work w = {};
     size_t part = 0;
     auto at_least = [&](size_t n) { if (n > part) part = n; };
-    auto shares = [&](const FfProduct &p) {  // of either kernel family: which one runs depends on the call's addresses too
-        const int s = ff_ffma_splits(p.m, p.n, p.k);
-        if (s > 1) at_least((size_t)s * p.m * p.n);
-        if (b.type != FC_DTYPE_F32 && p.k > 0) at_least(ff_tc_part_floats(p));
-    };
-    w.h = c.take<uint8_t>(rh * e);
+    w.h = matrix(b.rows, hidden);
+    w.x = matrix(b.rows, in);
+    w.w_gate = matrix(b.hidden, in);
+    w.w_up = matrix(b.hidden, in);
+    w.w_down = matrix(b.out, hidden);
     if (!backward) {
-        shares(down_product(b, nullptr, nullptr, nullptr, nullptr));
+        at_least(ff_tc_part_floats(down_product(b, w.h, w.w_down, nullptr, nullptr)));
     } else {
-        w.dgu = c.take<uint8_t>(2 * rh * e);
-        shares(dx_product(b, nullptr, nullptr, nullptr, nullptr));
-        shares(dw_in_product(b, nullptr, nullptr, nullptr, nullptr));
-        shares(dw_down_product(b, nullptr, nullptr, nullptr));
-        at_least((size_t)colsum_chunks(b.rows, 2 * b.hidden) * 2 * b.hidden);
+        w.dy = matrix(b.rows, out);
+        w.dgu = matrix(b.rows, 2 * hidden);
+        at_least(ff_tc_part_floats(dx_product(b, w.dgu, w.w_gate, nullptr, nullptr)));
+        at_least(ff_tc_part_floats(dw_in_product(b, w.dgu, w.x, nullptr, nullptr)));
+        at_least(ff_tc_part_floats(dw_down_product(b, w.dy, w.h, nullptr)));
+        at_least((size_t)colsum_chunks(b.rows, b.hidden) * b.hidden);
         at_least((size_t)colsum_chunks(b.rows, b.out) * b.out);
     }
     w.part = c.take<float>(part);
@@ -188,20 +262,37 @@ Work carve(const Block &b, void *base, bool backward) {
     return w;
 }
 
+// The operands of one call: as they lie where the copies can take them so, else packed.
+struct Packer {
+    const Block &b;
+    PackList list;
+    long long total;
+    explicit Packer(const Block &block) : b(block), list(), total(0) {}
+    static bool lies_well(const Block &b, const void *p, int64_t ld) { return b.type != FC_DTYPE_F32 && ld % 8 == 0 && aligned16(p); }
+    Matrix use(const void *p, int64_t ld, int rows, int cols, const Matrix &room, bool as_it_lies) {
+        if (as_it_lies) return Matrix{p, ld, 0};
+        const int vec = 16 / (int)dtype_size(b.type);
+        total += rows * (room.ld / 8);
+        list.item[list.count++] = PackItem{p, ld, rows, cols, ld % vec == 0 && aligned16(p), (uint16_t *)room.p, room.ld, room.plane, total};
+        return room;
+    }
+    Matrix use(const void *p, int64_t ld, int rows, int cols, const Matrix &room) {
+        return use(p, ld, rows, cols, room, lies_well(b, p, ld));
+    }
+    int run(fc_context *ctx) {
+        if (list.count == 0) return FC_OK;
+        return with_type(b.type, [&](auto t) -> int {
+            long long blocks = ceil_div((size_t)total, 256);
+            if (blocks > 148 * 16) blocks = 148 * 16;
+            FC_CHECK_CUDA(launch_pdl(ff_pack_kernel<decltype(t)>, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, list));
+            return FC_OK;
+        });
+    }
+};
+
 int multiply(fc_context *ctx, FfProduct p, float *part) {
     p.part = part;
-    if (p.kind != FF_GATE_BACK && ff_few_fits(p)) return launch_ff_few(ctx, p);
-    if (ff_tc_fits(p)) return launch_ff_tc(ctx, p);
-    if (p.kind == FF_STORE) p.splits = ff_ffma_splits(p.m, p.n, p.k);
-    FC_PROPAGATE(launch_ff_ffma(ctx, p));
-    if (p.splits == 1) return FC_OK;
-    return with_type(p.type, [&](auto t) -> int {
-        long long blocks = (long long)ceil_div((size_t)p.m * p.n, JOIN_THREADS);
-        if (blocks > 148 * 8) blocks = 148 * 8;
-        FC_CHECK_CUDA(launch_pdl(ff_join_kernel<decltype(t)>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, ctx->stream,
-                                 (const float *)part, p));
-        return FC_OK;
-    });
+    return launch_ff_tc(ctx, p);
 }
 
 int check_pointers(const Block &b, std::initializer_list<const void *> needed, std::initializer_list<const void *> optional) {
@@ -248,14 +339,33 @@ int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const voi
     FC_PROPAGATE(check_workspace(d_workspace, workspace_bytes, w.bytes));
     DeviceScope dev(ctx->device);
     FC_CHECK_CUDA(dev.status());
-    FfProduct p = product(b, FF_GATE, b.rows, b.hidden, b.in, d_x, b.xs, true, d_w_gate, b.in, true, w.h, b.hidden);
-    p.b1 = d_w_up;
-    p.bias0 = d_b_gate;
-    p.bias1 = d_b_up;
-    p.gate = d_saved;
-    p.up = d_saved ? d_saved + (size_t)b.rows * b.hidden : nullptr;
-    FC_PROPAGATE(multiply(ctx, p, nullptr));
-    return multiply(ctx, down_product(b, w.h, d_w_down, d_b_down, d_y), w.part);
+    float *up = d_saved ? d_saved + (size_t)b.rows * b.hidden : nullptr;
+    const Matrix x0 = {d_x, b.xs, 0}, wg0 = {d_w_gate, b.in, 0}, wd0 = {d_w_down, b.hidden, 0};
+    auto gate = [&](const Matrix &x, const Matrix &w_gate, const void *w_up) {
+        FfProduct p = product(b, FF_GATE, b.rows, b.hidden, b.in, x, true, w_gate, true);
+        p.b1 = w_up;
+        p.bias0 = d_b_gate;
+        p.bias1 = d_b_up;
+        p.gate = d_saved;
+        p.up = up;
+        p.c0 = const_cast<void *>(w.h.p); p.ldc = w.h.ld; p.c_plane = w.h.plane;
+        return p;
+    };
+    {
+        const FfProduct first = gate(x0, wg0, d_w_up), second = down_product(b, w.h, wd0, d_b_down, d_y);
+        if (ff_few_fits(first) && ff_few_fits(second)) {
+            FC_PROPAGATE(launch_ff_few(ctx, first));
+            return launch_ff_few(ctx, second);
+        }
+    }
+    Packer pack(b);
+    const bool w_in = Packer::lies_well(b, d_w_gate, b.in) && Packer::lies_well(b, d_w_up, b.in);
+    const Matrix x = pack.use(d_x, b.xs, b.rows, b.in, w.x), w_gate = pack.use(d_w_gate, b.in, b.hidden, b.in, w.w_gate, w_in),
+                 w_up = pack.use(d_w_up, b.in, b.hidden, b.in, w.w_up, w_in),
+                 w_down = pack.use(d_w_down, b.hidden, b.out, b.hidden, w.w_down);
+    FC_PROPAGATE(pack.run(ctx));
+    FC_PROPAGATE(multiply(ctx, gate(x, w_gate, w_up.p), nullptr));
+    return multiply(ctx, down_product(b, w.h, w_down, d_b_down, d_y), w.part);
 }
 
 int fc_gated_ff_backward(fc_context *ctx, const fc_gated_ff_desc *desc, const void *d_dy, const void *d_x, const void *d_w_gate,
@@ -272,20 +382,42 @@ int fc_gated_ff_backward(fc_context *ctx, const fc_gated_ff_desc *desc, const vo
     FC_PROPAGATE(check_workspace(d_workspace, workspace_bytes, w.bytes));
     DeviceScope dev(ctx->device);
     FC_CHECK_CUDA(dev.status());
-    const int64_t two = 2 * (int64_t)b.hidden;
-    if (b.rows > 0) {
-        FfProduct p = product(b, FF_GATE_BACK, b.rows, b.hidden, b.out, d_dy, b.ys, true, d_w_down, b.hidden, false, w.dgu, two);
-        p.gate = const_cast<float *>(d_saved);
-        p.up = p.gate + (size_t)b.rows * b.hidden;
-        p.c1 = w.h;
-        FC_PROPAGATE(multiply(ctx, p, nullptr));
-        if (d_dx) FC_PROPAGATE(multiply(ctx, dx_product(b, w.dgu, d_w_gate, d_w_up, d_dx), w.part));
+    const size_t e = dtype_size(b.type);
+    if (b.rows == 0) {  // sums of nothing
+        const struct { void *p; size_t n; } grads[] = {{d_dw_gate, (size_t)b.hidden * b.in}, {d_dw_up, (size_t)b.hidden * b.in},
+                                                       {d_dw_down, (size_t)b.out * b.hidden}, {d_db_gate, (size_t)b.hidden},
+                                                       {d_db_up, (size_t)b.hidden}, {d_db_down, (size_t)b.out}};
+        for (const auto &g : grads)
+            if (g.p) FC_CHECK_CUDA(cudaMemsetAsync(g.p, 0, g.n * e, ctx->stream));
+        return FC_OK;
     }
-    if (d_dw_gate || d_dw_up) FC_PROPAGATE(multiply(ctx, dw_in_product(b, w.dgu, d_x, d_dw_gate, d_dw_up), w.part));
-    if (d_dw_down) FC_PROPAGATE(multiply(ctx, dw_down_product(b, d_dy, w.h, d_dw_down), w.part));
-    if (d_db_gate || d_db_up)
-        FC_PROPAGATE(colsum(ctx, b.type, w.dgu, two, b.rows, (int)two, b.hidden, d_db_gate, d_db_up, w.part));
-    if (d_db_down) FC_PROPAGATE(colsum(ctx, b.type, d_dy, b.ys, b.rows, b.out, b.out, d_db_down, nullptr, w.part));
+    Packer pack(b);
+    const bool w_in = Packer::lies_well(b, d_w_gate, b.in) && Packer::lies_well(b, d_w_up, b.in);
+    const Matrix dy = pack.use(d_dy, b.ys, b.rows, b.out, w.dy), w_down = pack.use(d_w_down, b.hidden, b.out, b.hidden, w.w_down);
+    Matrix x = {}, w_gate = {}, w_up = {};
+    if (d_dw_gate || d_dw_up) x = pack.use(d_x, b.xs, b.rows, b.in, w.x);
+    if (d_dx) {
+        w_gate = pack.use(d_w_gate, b.in, b.hidden, b.in, w.w_gate, w_in);
+        w_up = pack.use(d_w_up, b.in, b.hidden, b.in, w.w_up, w_in);
+    }
+    FC_PROPAGATE(pack.run(ctx));
+
+    FfProduct p = product(b, FF_GATE_BACK, b.rows, b.hidden, b.out, dy, true, w_down, false);
+    p.gate = const_cast<float *>(d_saved);
+    p.up = p.gate + (size_t)b.rows * b.hidden;
+    p.a_skip = w.dgu.ld / 2;
+    p.c0 = const_cast<void *>(w.dgu.p); p.ldc = w.dgu.ld; p.c_plane = w.dgu.plane;
+    p.c1 = const_cast<void *>(w.h.p); p.ldc1 = w.h.ld; p.c1_plane = w.h.plane;
+    FC_PROPAGATE(multiply(ctx, p, nullptr));
+    if (d_dx) FC_PROPAGATE(multiply(ctx, dx_product(b, w.dgu, w_gate, w_up.p, d_dx), w.part));
+    if (d_dw_gate || d_dw_up) FC_PROPAGATE(multiply(ctx, dw_in_product(b, w.dgu, x, d_dw_gate, d_dw_up), w.part));
+    if (d_dw_down) FC_PROPAGATE(multiply(ctx, dw_down_product(b, dy, w.h, d_dw_down), w.part));
+
+    const int64_t plane = b.type == FC_DTYPE_F32 ? w.dgu.plane : 0;
+    const uint8_t *dgu = (const uint8_t *)w.dgu.p;
+    if (d_db_gate) FC_PROPAGATE(colsum(ctx, b.type, dgu, w.dgu.ld, plane, b.rows, b.hidden, d_db_gate, w.part));
+    if (d_db_up) FC_PROPAGATE(colsum(ctx, b.type, dgu + w.dgu.ld, w.dgu.ld, plane, b.rows, b.hidden, d_db_up, w.part));
+    if (d_db_down) FC_PROPAGATE(colsum(ctx, b.type, d_dy, b.ys, 0, b.rows, b.out, d_db_down, w.part));
     return FC_OK;
 }
 

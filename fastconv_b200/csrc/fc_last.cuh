@@ -96,6 +96,12 @@ inline bool dtype_ok(int type) { return type >= FC_DTYPE_F32 && type <= FC_DTYPE
 inline bool act_ok(int act) { return act >= FC_ACT_NONE && act <= FC_ACT_SIGMOID; }
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
+// The upper part of a value that is to be the sum of bf16 values: to nearest, but never up to infinity.
+__device__ __forceinline__ float bf16_part(float v) {
+    const float p = __bfloat162float(__float2bfloat16_rn(v));
+    return fabsf(v) <= 3.4028234e38f && !(fabsf(p) <= 3.4028234e38f) ? __uint_as_float(__float_as_uint(v) & 0xffff0000u) : p;
+}
+
 // ---- activations ------------------------------------------------------------------------------------------------
 // kExact: the library's functions, for results that are kept in fp32.  Otherwise the hardware's power of two and
 // reciprocal (a few units in the 23rd bit, subnormals as zero), for results that are rounded to 8 or 11 bits anyway: two
