@@ -36,17 +36,19 @@ constexpr int KB = 64;                    // reduction steps of a stage: 128 byt
 constexpr int HALF_BYTES = 128 * KB * 2;  // one CTA's A in a stage and plane
 constexpr int EPI_WARPS = 8;
 constexpr int PIECE = 32 * 32 * 2;        // 32 rows x 32 columns of 16 bits
-constexpr int PIECES = 4;                 // a warp's ring of pieces on their way out
+constexpr int PIECES = 2;                 // a warp's ring of pieces on their way out
 constexpr int FF_TC_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int OUT_BYTES = EPI_WARPS * PIECES * PIECE;
 constexpr int CHUNK = 4;                  // k-blocks whose sum stays in tensor memory, three planes
 
+// A stage takes some 2800 clocks from its request over the products to its release, and 512 of the matrix pipe at bn = 256: six
+// of them keep the pipe fed (five gave 597 clocks a k-block).  Narrower tiles have room for more.
 template <int PLANES>
 struct Ring {
-    static constexpr int kStages = PLANES == 1 ? 5 : 2;
-    static constexpr int kB = PLANES == 1 ? HALF_BYTES : HALF_BYTES / 2;  // the most of one CTA's B in a stage and plane
-    static constexpr int kStage = PLANES * (HALF_BYTES + kB);
-    static constexpr int kSmem = 1024 + kStages * kStage + OUT_BYTES + 256;
+    static constexpr int kBytes = PLANES == 1 ? 6 * 2 * HALF_BYTES : 2 * 3 * (HALF_BYTES + HALF_BYTES / 2);
+    static constexpr int kMost = 10;  // stages
+    static constexpr int kSmem = 1024 + kBytes + OUT_BYTES + 256;
+    __host__ __device__ static int stage_bytes(int bn) { return PLANES * (HALF_BYTES + bn * 64); }
 };
 
 struct FfMaps {
@@ -59,7 +61,7 @@ struct FfTc {
     int live_tiles, skip;     // those that are computed: live_tiles from `skip` on
     int n_tiles, splits;
     int kb_total, kb_first, kb_share;  // k-blocks; those before kb_first come from the first maps; of one share
-    int bn, act;
+    int bn, stages, act;
     long long items;
     const void *bias0, *bias1;
     int bias_wide;            // the biases can be read in 16-byte vectors
@@ -76,6 +78,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 __device__ __forceinline__ uint32_t first_cta(uint32_t addr) {  // the same place in the pair's first CTA
     uint32_t r;
@@ -140,6 +147,17 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr) {
     return d;
 }
 
+template <typename T>
+__device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        Vec<T, 2> two;
+        const float f[2] = {v[2 * i], v[2 * i + 1]};
+        two.pack(f);
+        w[i] = *reinterpret_cast<const uint32_t *>(&two);
+    }
+}
+
 // Sixteen-bit values of 32 neighbouring columns of this lane's row -> one piece (64-byte swizzle) -> TMA store.
 struct Outlet {
     uint32_t base;  // the warp's pieces
@@ -153,19 +171,18 @@ struct Outlet {
     }
     template <typename T>
     __device__ __forceinline__ void put(const CUtensorMap *map, const float (&v)[32], int x, int y, int z, int lane) {
+        uint32_t w[16];
+        pack_row<T>(v, w);
+        put(map, w, x, y, z, lane);
+    }
+    __device__ __forceinline__ void put(const CUtensorMap *map, const uint32_t (&w)[16], int x, int y, int z, int lane) {
         const uint32_t p = open();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                Vec<T, 2> two;
-                const float f[2] = {v[8 * i + 2 * j], v[8 * i + 2 * j + 1]};
-                two.pack(f);
-                w[j] = *reinterpret_cast<const uint32_t *>(&two);
-            }
             const uint32_t at = p + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]),
+                         "r"(w[4 * i + 3])
+                         : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -292,16 +309,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     ff_tc_kernel(const __grid_constant__ FfMaps maps, const FfTc P) {
     using R = Ring<PLANES>;
     constexpr bool kExact = PLANES == 3;
-    constexpr int kStages = R::kStages;
+    constexpr int kMost = R::kMost;
+    const int S = P.stages;
+    const uint32_t b_bytes = (uint32_t)P.bn * 64;  // this CTA's share of B in a stage and plane
+    const uint32_t stage_bytes = PLANES * (HALF_BYTES + b_bytes);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-    const uint32_t out_base = smem + kStages * R::kStage;
+    const uint32_t out_base = smem + R::kBytes;
     const uint32_t bars = out_base + OUT_BYTES;
     auto bar_full = [&](int s) { return bars + 8 * s; };
-    auto bar_empty = [&](int s) { return bars + 8 * (kStages + s); };
-    auto bar_acc_full = [&](int a) { return bars + 8 * (2 * kStages + a); };
-    auto bar_acc_empty = [&](int a) { return bars + 8 * (2 * kStages + 2 + a); };
-    auto bar_small_empty = [&](int a) { return bars + 8 * (2 * kStages + 4 + a); };  // three planes: the small products' accumulators
+    auto bar_empty = [&](int s) { return bars + 8 * (kMost + s); };
+    auto bar_acc_full = [&](int a) { return bars + 8 * (2 * kMost + a); };
+    auto bar_acc_empty = [&](int a) { return bars + 8 * (2 * kMost + 2 + a); };
+    auto bar_small_empty = [&](int a) { return bars + 8 * (2 * kMost + 4 + a); };  // three planes: the small products' accumulators
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
@@ -309,11 +329,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
-    const uint32_t b_bytes = (uint32_t)P.bn / 2 * 128;  // this CTA's share of B in a stage and plane
     const uint32_t tmem_cols = PLANES == 1 ? 2 * P.bn : 4 * P.bn;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < S; ++s) {
             mbar_init(bar_full(s), 1);
             mbar_init(bar_empty(s), 1);
         }
@@ -323,6 +342,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
             mbar_init(bar_small_empty(a), 2 * EPI_WARPS);
         }
         abort_word = 0;
+        for (int i = 0; i < 2; ++i) {  // descriptors on their way before the first copy wants them
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a[i]) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b[i]) : "memory");
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -344,24 +367,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
         share = (int)(rest / P.live_tiles);
     };
 
+    // Warps 0 and 1 run their loops with all lanes, on values that are the same in all of them, and one elected lane issues:
+    // matrix instructions and copies take their operands from uniform registers, and in a branch of one lane each of them
+    // costs some 150 clocks of moves.
     if (warp == 0) {
-        if (lane == 0) {
-            int g = 0;
-            bool ok = true;
-            for (long long item = first; item < P.items && ok; item += step) {
-                int mt, nt, share;
-                decode(item, mt, nt, share);
-                const int dest = mt / P.dest_tiles;
-                const int m0 = (mt - dest * P.dest_tiles) * 256 + (int)rank * 128;
-                const int n0 = KIND == FF_GATE ? nt * (P.bn / 2) : nt * P.bn + (int)rank * (P.bn / 2);
-                const int lo = share * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
-                for (int kb = lo; kb < hi; ++kb, ++g) {
-                    const int s = g % kStages;
-                    if (!mbar_wait(bar_empty(s), ((g / kStages) & 1) ^ 1, abort_flag, P.status)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t a_at = smem + s * R::kStage, b_at = a_at + PLANES * HALF_BYTES;
+        int s = 0;
+        uint32_t phase = 0;  // of the ring's current round
+        bool ok = true;
+        for (long long item = first; item < P.items && ok; item += step) {
+            int mt, nt, share;
+            decode(item, mt, nt, share);
+            const int dest = mt / P.dest_tiles;
+            const int m0 = (mt - dest * P.dest_tiles) * 256 + (int)rank * 128;
+            const int n0 = KIND == FF_GATE ? nt * (P.bn / 2) : nt * P.bn + (int)rank * (P.bn / 2);
+            const int lo = share * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
+            for (int kb = lo; kb < hi; ++kb) {
+                if (!mbar_wait(bar_empty(s), phase ^ 1, abort_flag, P.status)) {
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
+                    const uint32_t a_at = smem + s * stage_bytes, b_at = a_at + PLANES * HALF_BYTES;
                     const uint32_t full = first_cta(bar_full(s));
                     if (rank == 0) mbar_expect_tx(bar_full(s), 2 * PLANES * (HALF_BYTES + b_bytes));
                     const int second = kb >= P.kb_first;
@@ -370,7 +396,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                     const CUtensorMap *bm = &maps.b[KIND == FF_GATE ? (int)rank : second];
 #pragma unroll
                     for (int z = 0; z < PLANES; ++z) {
-                        const uint32_t az = a_at + z * HALF_BYTES, bz = b_at + z * R::kB;
+                        const uint32_t az = a_at + z * HALF_BYTES, bz = b_at + z * b_bytes;
                         if (A_BY_K) {
                             pair_load(az, am, full, k0, m0, z);
                         } else {
@@ -380,21 +406,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                         if (B_BY_K) {
                             pair_load(bz, bm, full, k0, n0, z);
                         } else {
-                            for (int i = 0; i < P.bn / 128; ++i) pair_load(bz + i * KB * 128, bm, full, n0 + 64 * i, k0, z);
+                            pair_load(bz, bm, full, n0, k0, z);
+                            if (P.bn > 128) pair_load(bz + KB * 128, bm, full, n0 + 64, k0, z);
                         }
                     }
                 }
+                __syncwarp();
+                if (++s == S) s = 0, phase ^= 1;
             }
-            // the other CTA's last releases have arrived here before this one may end
-            for (int i = 0; i < kStages && ok; ++i, ++g)
-                ok = mbar_wait(bar_empty(g % kStages), ((g / kStages) & 1) ^ 1, abort_flag, P.status);
+        }
+        // the other CTA's last releases have arrived here before this one may end
+        for (int i = 0; i < S && ok; ++i) {
+            ok = mbar_wait(bar_empty(s), phase ^ 1, abort_flag, P.status);
+            if (++s == S) s = 0, phase ^= 1;
         }
     } else if (warp == 1) {
-        if (rank == 0 && lane == 0) {
+        if (rank == 0) {
             constexpr uint32_t type = std::is_same<OT, __nv_bfloat16>::value ? 1 : 0;
             const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((A_BY_K ? 0u : 1u) << 15) | ((B_BY_K ? 0u : 1u) << 16) |
                                    ((uint32_t)(P.bn >> 3) << 17) | ((256u >> 4) << 24);
-            int g = 0, t = 0, c = 0;  // k-blocks, tiles and accumulators so far
+            int s = 0, t = 0, c = 0;  // stage; tiles and accumulators so far
+            uint32_t phase = 0;
             bool ok = true;
             for (long long item = first; item < P.items && ok; item += step, ++t) {
                 int mt, nt, share;
@@ -410,30 +442,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                     }
                     tc_fence_after();
                     const uint32_t d = tmem + acc * P.bn;
-                    for (int kb = k_lo; kb < k_hi; ++kb, ++g) {
-                        const int s = g % kStages;
-                        if (!mbar_wait(bar_full(s), (g / kStages) & 1, abort_flag, P.status)) {
+                    for (int kb = k_lo; kb < k_hi; ++kb) {
+                        if (!mbar_wait(bar_full(s), phase, abort_flag, P.status)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t a_at = smem + s * R::kStage, b_at = a_at + PLANES * HALF_BYTES;
+                        if (elect_one()) {
+                            const uint32_t a_at = smem + s * stage_bytes, b_at = a_at + PLANES * HALF_BYTES;
 #pragma unroll
-                        for (int k = 0; k < KB / 16; ++k) {  // 16 steps: 32 bytes along a row, or 16 rows
-                            auto a = [&](int z) { return operand<A_BY_K>(a_at + z * HALF_BYTES + k * (A_BY_K ? 32 : 2048)); };
-                            auto b = [&](int z) { return operand<B_BY_K>(b_at + z * R::kB + k * (B_BY_K ? 32 : 2048)); };
-                            pair_mma(d, a(0), b(0), idesc, kb > k_lo || k > 0);
-                            if (PLANES == 3) {
-                                pair_mma(small, a(0), b(1), idesc, kb > lo || k > 0);
-                                pair_mma(small, a(1), b(0), idesc, 1);
-                                pair_mma(small, a(0), b(2), idesc, 1);
-                                pair_mma(small, a(2), b(0), idesc, 1);
-                                pair_mma(small, a(1), b(1), idesc, 1);
+                            for (int k = 0; k < KB / 16; ++k) {  // 16 steps: 32 bytes along a row, or 16 rows
+                                auto a = [&](int z) { return operand<A_BY_K>(a_at + z * HALF_BYTES + k * (A_BY_K ? 32 : 2048)); };
+                                auto b = [&](int z) { return operand<B_BY_K>(b_at + z * b_bytes + k * (B_BY_K ? 32 : 2048)); };
+                                pair_mma(d, a(0), b(0), idesc, kb > k_lo || k > 0);
+                                if (PLANES == 3) {
+                                    pair_mma(small, a(0), b(1), idesc, kb > lo || k > 0);
+                                    pair_mma(small, a(1), b(0), idesc, 1);
+                                    pair_mma(small, a(0), b(2), idesc, 1);
+                                    pair_mma(small, a(2), b(0), idesc, 1);
+                                    pair_mma(small, a(1), b(1), idesc, 1);
+                                }
                             }
+                            pair_commit(bar_empty(s));
+                            if (kb == k_hi - 1) pair_commit(bar_acc_full(acc));
                         }
-                        pair_commit(bar_empty(s));
+                        __syncwarp();
+                        if (++s == S) s = 0, phase ^= 1;
                     }
-                    if (ok) pair_commit(bar_acc_full(acc));
                 }
             }
         }
@@ -457,6 +492,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = add ? v[j] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
             };
+            auto saved = [&](int x, float (&g)[32], float (&u)[32]) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) g[j] = u[j] = 0.0f;
+                if (row < P.m && x < P.n) {
+                    saved_row<false>(P, P.gate, y, lane, x, g);
+                    saved_row<false>(P, P.up, y, lane, x, u);
+                }
+            };
+            auto back = [&](float (&g)[32], float (&u)[32], float (&v)[32]) {  // in: g, u, dh; out: dg, du, h
+                switch (P.act) {
+                    case FC_ACT_RELU: gate_back_values<FC_ACT_RELU, kExact>(g, u, v); break;
+                    case FC_ACT_SILU: gate_back_values<FC_ACT_SILU, kExact>(g, u, v); break;
+                    case FC_ACT_GELU: gate_back_values<FC_ACT_GELU, kExact>(g, u, v); break;
+                    case FC_ACT_GELU_TANH: gate_back_values<FC_ACT_GELU_TANH, kExact>(g, u, v); break;
+                    case FC_ACT_SIGMOID: gate_back_values<FC_ACT_SIGMOID, kExact>(g, u, v); break;
+                    default: gate_back_values<FC_ACT_NONE, kExact>(g, u, v);
+                }
+            };
             // 32 columns from x on: v the product; FF_GATE: v the gate's, u the up projection's
             auto emit = [&](int x, float (&v)[32], float (&u)[32]) {
                 if (x >= P.n || y >= P.m) return;
@@ -478,20 +531,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                     put_planes<OT, PLANES>(out, &maps.c[0], v, x, y, lane);
                 } else if (KIND == FF_GATE_BACK) {
                     float g[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) g[j] = u[j] = 0.0f;
-                    if (row < P.m) {
-                        saved_row<false>(P, P.gate, y, lane, x, g);
-                        saved_row<false>(P, P.up, y, lane, x, u);
-                    }
-                    switch (P.act) {
-                        case FC_ACT_RELU: gate_back_values<FC_ACT_RELU, kExact>(g, u, v); break;
-                        case FC_ACT_SILU: gate_back_values<FC_ACT_SILU, kExact>(g, u, v); break;
-                        case FC_ACT_GELU: gate_back_values<FC_ACT_GELU, kExact>(g, u, v); break;
-                        case FC_ACT_GELU_TANH: gate_back_values<FC_ACT_GELU_TANH, kExact>(g, u, v); break;
-                        case FC_ACT_SIGMOID: gate_back_values<FC_ACT_SIGMOID, kExact>(g, u, v); break;
-                        default: gate_back_values<FC_ACT_NONE, kExact>(g, u, v);
-                    }
+                    saved(x, g, u);
+                    back(g, u, v);
                     put_planes<OT, PLANES>(out, &maps.c[0], g, x, y, lane);
                     put_planes<OT, PLANES>(out, &maps.c[1], u, x, y, lane);
                     put_planes<OT, PLANES>(out, &maps.c[2], v, x, y, lane);
@@ -516,11 +557,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
             };
             if constexpr (PLANES == 1) {
                 const int acc = c & 1;
+                float g[32], up[32];  // FF_GATE_BACK: the saved values, requested a piece ahead of their use
+                if (KIND == FF_GATE_BACK) saved(nt * cols + half * 32, g, up);
                 if (!mbar_wait(bar_acc_full(acc), (c >> 1) & 1, abort_flag, P.status)) break;
                 ++c;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * P.bn;
-                for (int j = half * 32; j < cols; j += 64) {
+                for (int j = half * 32; KIND == FF_GATE_BACK && j < cols; j += 64) {
+                    const int x = nt * cols + j;
+                    if (x >= P.n || y >= P.m) break;
+                    float v[32];
+                    fetch(d + j, v, false);
+                    back(g, up, v);
+                    uint32_t w[3][16];
+                    pack_row<OT>(g, w[0]);
+                    pack_row<OT>(up, w[1]);
+                    pack_row<OT>(v, w[2]);
+                    if (j + 64 < cols) saved(x + 64, g, up);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) out.put(&maps.c[i], w[i], x, y, 0, lane);
+                }
+                for (int j = half * 32; KIND != FF_GATE_BACK && j < cols; j += 64) {
                     if (nt * cols + j >= P.n || y >= P.m) break;
                     float v[32], u[32];
                     fetch(d + j, v, false);
@@ -700,6 +757,8 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
     P.skip = dests == 2 && p.c0 == nullptr ? P.dest_tiles : 0;
     P.live_tiles = dests == 2 && (p.c0 == nullptr || p.c1 == nullptr) ? P.dest_tiles : P.m_tiles;
     P.bn = plan.bn;
+    const int room = (p.planes == 1 ? Ring<1>::kBytes / Ring<1>::stage_bytes(plan.bn) : Ring<3>::kBytes / Ring<3>::stage_bytes(plan.bn));
+    P.stages = room < Ring<1>::kMost ? room : Ring<1>::kMost;
     P.n_tiles = (int)ceil_div(p.n, p.kind == FF_GATE ? plan.bn / 2 : plan.bn);
     P.splits = plan.splits;
     P.kb_total = kb_total;
