@@ -62,7 +62,7 @@ struct FfTc {
     int n_tiles, splits;
     int kb_total, kb_first, kb_share;  // k-blocks; those before kb_first come from the first maps; of one share
     int bn, stages, act;
-    long long items;
+    int items;                // tiles times shares
     const void *bias0, *bias1;
     int bias_wide;            // the biases can be read in 16-byte vectors
     float *gate, *up;         // saved: written (FF_GATE) or read (FF_GATE_BACK)
@@ -238,15 +238,21 @@ __device__ __forceinline__ void saved_row(const FfTc &P, float *base, int y, int
     const int block_rows = min(32, P.m - y);
     if (P.saved_wide) {
         float4 *p = (float4 *)(base + (size_t)y * P.n) + (size_t)(x / 4) * block_rows + lane;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (x + 4 * j >= P.n) break;
+        auto move = [&](int j, int at) {
             if (STORE) {
-                p[(size_t)j * block_rows] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                p[at] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             } else {
-                const float4 f = __ldg(p + (size_t)j * block_rows);
+                const float4 f = __ldg(p + at);
                 v[4 * j] = f.x, v[4 * j + 1] = f.y, v[4 * j + 2] = f.z, v[4 * j + 3] = f.w;
             }
+        };
+        if (x + 32 <= P.n && block_rows == 32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) move(j, j * 32);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (x + 4 * j < P.n) move(j, j * block_rows);
         }
     } else {
 #pragma unroll
@@ -328,7 +334,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
-    const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const uint32_t first = blockIdx.x >> 1, step = gridDim.x >> 1, items = P.items;
     const uint32_t tmem_cols = PLANES == 1 ? 2 * P.bn : 4 * P.bn;
 
     if (threadIdx.x == 0) {
@@ -360,11 +366,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     const uint32_t tmem = tmem_slot;
     pdl_wait();
 
-    auto decode = [&](long long item, int &mt, int &nt, int &share) {
-        nt = (int)(item % P.n_tiles);
-        const long long rest = item / P.n_tiles;
-        mt = P.skip + (int)(rest % P.live_tiles);
-        share = (int)(rest / P.live_tiles);
+    auto decode = [&](uint32_t item, int &mt, int &nt, int &share) {
+        const uint32_t rest = item / (uint32_t)P.n_tiles;
+        nt = (int)(item - rest * P.n_tiles);
+        share = (int)(P.splits > 1 ? rest / (uint32_t)P.live_tiles : 0);
+        mt = P.skip + (int)(rest - share * P.live_tiles);
     };
 
     // Warps 0 and 1 run their loops with all lanes, on values that are the same in all of them, and one elected lane issues:
@@ -374,10 +380,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
         int s = 0;
         uint32_t phase = 0;  // of the ring's current round
         bool ok = true;
-        for (long long item = first; item < P.items && ok; item += step) {
+        for (uint32_t item = first; item < items && ok; item += step) {
             int mt, nt, share;
             decode(item, mt, nt, share);
-            const int dest = mt / P.dest_tiles;
+            const int dest = mt >= P.dest_tiles;
             const int m0 = (mt - dest * P.dest_tiles) * 256 + (int)rank * 128;
             const int n0 = KIND == FF_GATE ? nt * (P.bn / 2) : nt * P.bn + (int)rank * (P.bn / 2);
             const int lo = share * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
@@ -428,7 +434,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
             int s = 0, t = 0, c = 0;  // stage; tiles and accumulators so far
             uint32_t phase = 0;
             bool ok = true;
-            for (long long item = first; item < P.items && ok; item += step, ++t) {
+            for (uint32_t item = first; item < items && ok; item += step, ++t) {
                 int mt, nt, share;
                 decode(item, mt, nt, share);
                 const int lo = share * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
@@ -478,10 +484,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
         const int cols = KIND == FF_GATE ? P.bn / 2 : P.bn;  // output columns of a tile
         int t = 0, c = 0;
         bool ok = true;
-        for (long long item = first; item < P.items && ok; item += step, ++t) {
+        for (uint32_t item = first; item < items && ok; item += step, ++t) {
             int mt, nt, share;
             decode(item, mt, nt, share);
-            const int dest = mt / P.dest_tiles;
+            const int dest = mt >= P.dest_tiles;
             const int y = (mt - dest * P.dest_tiles) * 256 + (int)rank * 128 + quad * 32;  // the warp's first row
             const int row = y + lane;
             const uint32_t lanes = (uint32_t)(quad * 32) << 16;
@@ -493,8 +499,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                 for (int j = 0; j < 32; ++j) v[j] = add ? v[j] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
             };
             auto saved = [&](int x, float (&g)[32], float (&u)[32]) {
+                if (row >= P.m || x + 32 > P.n) {  // what is past the edge is computed with zeros and not stored
 #pragma unroll
-                for (int j = 0; j < 32; ++j) g[j] = u[j] = 0.0f;
+                    for (int j = 0; j < 32; ++j) g[j] = u[j] = 0.0f;
+                }
                 if (row < P.m && x < P.n) {
                     saved_row<false>(P, P.gate, y, lane, x, g);
                     saved_row<false>(P, P.up, y, lane, x, u);
@@ -650,7 +658,7 @@ __global__ void __launch_bounds__(256) ff_tc_join_kernel(const FfTc P, T *c0, T 
         const int q = (int)(rest % col_blocks) * 4 + (lane >> 3);
         const long long block = rest / col_blocks;
         const int r = r8 * 8 + (lane & 7);
-        const int mt = (int)(block >> 3), dest = mt / P.dest_tiles;
+        const int mt = (int)(block >> 3), dest = mt >= P.dest_tiles;
         const int row = (mt - dest * P.dest_tiles) * 256 + (int)(block & 7) * 32 + r;
         T *c = dest ? c1 : c0;
         if (q >= quads || row >= P.m || c == nullptr) continue;
@@ -765,7 +773,9 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
     P.kb_first = kb_first;
     P.kb_share = (int)ceil_div(kb_total, plan.splits);
     P.act = p.act;
-    P.items = (long long)P.live_tiles * P.n_tiles * P.splits;
+    const long long items = (long long)P.live_tiles * P.n_tiles * P.splits;
+    FC_REQUIRE(items < (1ll << 31) - 4096, FC_ERR_UNSUPPORTED, "product of %lld tiles", items);  // item + step stays in 32 bits
+    P.items = (int)items;
     P.bias0 = p.bias0;
     P.bias1 = p.bias1;
     P.bias_wide = aligned16(p.bias0) && aligned16(p.bias1);
@@ -812,7 +822,7 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
                                         i == 2 ? p.c1_plane : p.c_plane, 32, 32));
     }
 
-    long long pairs = ctx->sm_count / 2;
+    int pairs = ctx->sm_count / 2;
     if (pairs > P.items) pairs = P.items;
     auto run = [&](auto ot, auto t, auto planes) -> int {
         using OT = decltype(ot);
