@@ -36,20 +36,22 @@ constexpr int KB = 64;                    // reduction steps of a stage: 128 byt
 constexpr int HALF_BYTES = 128 * KB * 2;  // one CTA's A in a stage and plane
 constexpr int EPI_WARPS = 8;
 constexpr int PIECE = 32 * 32 * 2;        // 32 rows x 32 columns of 16 bits
-constexpr int PIECES = 2;                 // a warp's ring of pieces on their way out
 constexpr int FF_TC_THREADS = 64 + 32 * EPI_WARPS;
-constexpr int OUT_BYTES = EPI_WARPS * PIECES * PIECE;
 constexpr int CHUNK = 4;                  // k-blocks whose sum stays in tensor memory, three planes
 
-// A stage takes some 2800 clocks from its request over the products to its release, and 512 of the matrix pipe at bn = 256: six
-// of them keep the pipe fed (five gave 597 clocks a k-block).  Narrower tiles have room for more.
-template <int PLANES>
+// The ring of stages and, for every epilogue warp, of pieces on their way out.  Six stages of bn = 256 (narrower tiles have room
+// for more); FF_GATE_BACK, which waits for memory and not for the matrix pipe, gives one for the three pieces that it writes at
+// a time.
+template <int PLANES, int KIND>
 struct Ring {
-    static constexpr int kBytes = PLANES == 1 ? 6 * 2 * HALF_BYTES : 2 * 3 * (HALF_BYTES + HALF_BYTES / 2);
+    static constexpr int kPieces = KIND == FF_GATE_BACK ? 4 : 2;
+    static constexpr int kBytes =
+        PLANES == 1 ? (KIND == FF_GATE_BACK ? 5 : 6) * 2 * HALF_BYTES : 2 * 3 * (HALF_BYTES + HALF_BYTES / 2);
+    static constexpr int kOut = EPI_WARPS * kPieces * PIECE;
     static constexpr int kMost = 10;  // stages
-    static constexpr int kSmem = 1024 + kBytes + OUT_BYTES + 256;
-    __host__ __device__ static int stage_bytes(int bn) { return PLANES * (HALF_BYTES + bn * 64); }
+    static constexpr int kSmem = 1024 + kBytes + kOut + 256;
 };
+__host__ __device__ constexpr int ff_stage_bytes(int planes, int bn) { return planes * (HALF_BYTES + bn * 64); }
 
 struct FfMaps {
     CUtensorMap a[2], b[2], c[3];
@@ -93,7 +95,9 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    // relaxed: what it stands for are reads of tensor memory, ordered by the tcgen05 fences; a release would wait for the
+    // warp's global stores too
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // into this CTA's shared memory, reported to the first CTA's barrier
 __device__ __forceinline__ void pair_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
@@ -159,35 +163,40 @@ __device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]
 }
 
 // Sixteen-bit values of 32 neighbouring columns of this lane's row -> one piece (64-byte swizzle) -> TMA store.
+template <int PIECES>
 struct Outlet {
     uint32_t base;  // the warp's pieces
     int next;
-    __device__ __forceinline__ uint32_t open() {  // a piece that is free again
-        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PIECES - 1) : "memory");
+    // N pieces at once: one wait until as many are free, one fence
+    template <int N>
+    __device__ __forceinline__ void put(const CUtensorMap *map, int map_step, const uint32_t (&w)[N][16], int x, int y, int z, int z_step,
+                                        int lane) {
+        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PIECES - N) : "memory");
         __syncwarp();
-        const uint32_t p = base + next * PIECE;
-        next = (next + 1) % PIECES;
-        return p;
-    }
-    template <typename T>
-    __device__ __forceinline__ void put(const CUtensorMap *map, const float (&v)[32], int x, int y, int z, int lane) {
-        uint32_t w[16];
-        pack_row<T>(v, w);
-        put(map, w, x, y, z, lane);
-    }
-    __device__ __forceinline__ void put(const CUtensorMap *map, const uint32_t (&w)[16], int x, int y, int z, int lane) {
-        const uint32_t p = open();
+        uint32_t at[N];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t at = p + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]),
-                         "r"(w[4 * i + 3])
-                         : "memory");
+        for (int k = 0; k < N; ++k) {
+            at[k] = base + next * PIECE;
+            next = (next + 1) & (PIECES - 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at[k] + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)),
+                             "r"(w[k][4 * i]), "r"(w[k][4 * i + 1]), "r"(w[k][4 * i + 2]), "r"(w[k][4 * i + 3])
+                             : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) store_3d(map, p, x, y, z);
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // one group a piece in every lane, so that all count alike
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (lane == 0) store_3d(map + k * map_step, at[k], x, y, z + k * z_step);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // one group a piece in every lane, so that all count alike
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void put(const CUtensorMap *map, const float (&v)[32], int x, int y, int z, int lane) {
+        uint32_t w[1][16];
+        pack_row<T>(v, w[0]);
+        put<1>(map, 0, w, x, y, z, 0, lane);
     }
 };
 
@@ -268,10 +277,10 @@ __device__ __forceinline__ void saved_row(const FfTc &P, float *base, int y, int
 }
 
 // to a matrix that a product will read again: one plane of 16 bits, or the three bf16 parts
-template <typename OT, int PLANES>
-__device__ __forceinline__ void put_planes(Outlet &out, const CUtensorMap *map, float (&v)[32], int x, int y, int lane) {
+template <typename OT, int PLANES, int PIECES>
+__device__ __forceinline__ void put_planes(Outlet<PIECES> &out, const CUtensorMap *map, float (&v)[32], int x, int y, int lane) {
     if constexpr (PLANES == 1) {
-        out.put<OT>(map, v, x, y, 0, lane);
+        out.template put<OT>(map, v, x, y, 0, lane);
     } else {
         float part[32];
 #pragma unroll
@@ -281,7 +290,7 @@ __device__ __forceinline__ void put_planes(Outlet &out, const CUtensorMap *map, 
                 part[j] = z < 2 ? bf16_part(v[j]) : v[j];
                 v[j] = fabsf(part[j]) <= 3.4028234e38f ? v[j] - part[j] : 0.0f;
             }
-            out.put<OT>(map, part, x, y, z, lane);
+            out.template put<OT>(map, part, x, y, z, lane);
         }
     }
 }
@@ -313,7 +322,7 @@ __device__ __forceinline__ void gate_back_values(float (&g)[32], float (&u)[32],
 template <typename OT, typename T, int PLANES, bool A_BY_K, bool B_BY_K, int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     ff_tc_kernel(const __grid_constant__ FfMaps maps, const FfTc P) {
-    using R = Ring<PLANES>;
+    using R = Ring<PLANES, KIND>;
     constexpr bool kExact = PLANES == 3;
     constexpr int kMost = R::kMost;
     const int S = P.stages;
@@ -322,7 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const uint32_t out_base = smem + R::kBytes;
-    const uint32_t bars = out_base + OUT_BYTES;
+    const uint32_t bars = out_base + R::kOut;
     auto bar_full = [&](int s) { return bars + 8 * s; };
     auto bar_empty = [&](int s) { return bars + 8 * (kMost + s); };
     auto bar_acc_full = [&](int a) { return bars + 8 * (2 * kMost + a); };
@@ -480,7 +489,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
         }
     } else {
         const int quad = warp & 3, half = (warp - 2) >> 2;  // tensor memory lanes of this warp; every second column piece
-        Outlet out = {out_base + (uint32_t)(warp - 2) * PIECES * PIECE, 0};
+        Outlet<R::kPieces> out = {out_base + (uint32_t)(warp - 2) * R::kPieces * PIECE, 0};
         const int cols = KIND == FF_GATE ? P.bn / 2 : P.bn;  // output columns of a tile
         int t = 0, c = 0;
         bool ok = true;
@@ -536,14 +545,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                         case FC_ACT_SIGMOID: gate_values<FC_ACT_SIGMOID, kExact>(v, u); break;
                         default: gate_values<FC_ACT_NONE, kExact>(v, u);
                     }
-                    put_planes<OT, PLANES>(out, &maps.c[0], v, x, y, lane);
+                    put_planes<OT, PLANES, R::kPieces>(out, &maps.c[0], v, x, y, lane);
                 } else if (KIND == FF_GATE_BACK) {
                     float g[32];
                     saved(x, g, u);
                     back(g, u, v);
-                    put_planes<OT, PLANES>(out, &maps.c[0], g, x, y, lane);
-                    put_planes<OT, PLANES>(out, &maps.c[1], u, x, y, lane);
-                    put_planes<OT, PLANES>(out, &maps.c[2], v, x, y, lane);
+                    put_planes<OT, PLANES, R::kPieces>(out, &maps.c[0], g, x, y, lane);
+                    put_planes<OT, PLANES, R::kPieces>(out, &maps.c[1], u, x, y, lane);
+                    put_planes<OT, PLANES, R::kPieces>(out, &maps.c[2], v, x, y, lane);
                 } else if (P.splits > 1) {  // [share][block of 32 rows][4 columns][row]
                     const int quads = (P.n + 3) / 4;
                     const size_t block = ((size_t)share * P.m_tiles + mt) * 8 + rank * 4 + quad;
@@ -559,7 +568,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                     if (c != nullptr) {
                         if (row < P.m) store_row(c + (size_t)row * P.ldc, P.c_wide, x, P.n, v);
                     } else if constexpr (PLANES == 1) {
-                        out.put<OT>(&maps.c[dest], v, x, y, 0, lane);
+                        out.template put<OT>(&maps.c[dest], v, x, y, 0, lane);
                     }
                 }
             };
@@ -582,8 +591,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                     pack_row<OT>(up, w[1]);
                     pack_row<OT>(v, w[2]);
                     if (j + 64 < cols) saved(x + 64, g, up);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) out.put(&maps.c[i], w[i], x, y, 0, lane);
+                    if constexpr (KIND == FF_GATE_BACK) out.template put<3>(&maps.c[0], 1, w, x, y, 0, 0, lane);
                 }
                 for (int j = half * 32; KIND != FF_GATE_BACK && j < cols; j += 64) {
                     if (nt * cols + j >= P.n || y >= P.m) break;
@@ -765,8 +773,6 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
     P.skip = dests == 2 && p.c0 == nullptr ? P.dest_tiles : 0;
     P.live_tiles = dests == 2 && (p.c0 == nullptr || p.c1 == nullptr) ? P.dest_tiles : P.m_tiles;
     P.bn = plan.bn;
-    const int room = (p.planes == 1 ? Ring<1>::kBytes / Ring<1>::stage_bytes(plan.bn) : Ring<3>::kBytes / Ring<3>::stage_bytes(plan.bn));
-    P.stages = room < Ring<1>::kMost ? room : Ring<1>::kMost;
     P.n_tiles = (int)ceil_div(p.n, p.kind == FF_GATE ? plan.bn / 2 : plan.bn);
     P.splits = plan.splits;
     P.kb_total = kb_total;
@@ -827,17 +833,22 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
     auto run = [&](auto ot, auto t, auto planes) -> int {
         using OT = decltype(ot);
         using T = decltype(t);
-        constexpr int PLANES = decltype(planes)::value, SMEM = Ring<PLANES>::kSmem;
-        auto go = [&](auto kernel) -> int {
+        constexpr int PLANES = decltype(planes)::value;
+        auto go = [&](auto kernel, auto ring) -> int {
+            using R = decltype(ring);
+            constexpr int SMEM = R::kSmem;
+            const int room = R::kBytes / ff_stage_bytes(PLANES, P.bn);
+            P.stages = room < R::kMost ? room : R::kMost;
             FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
             FC_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(2 * pairs)), dim3(FF_TC_THREADS), SMEM, ctx->stream, maps, P));
             return FC_OK;
         };
-        if (p.kind == FF_GATE) return go(ff_tc_kernel<OT, T, PLANES, true, true, FF_GATE>);
-        if (p.kind == FF_GATE_BACK) return go(ff_tc_kernel<OT, T, PLANES, true, false, FF_GATE_BACK>);
-        FC_PROPAGATE(!p.a_by_k  ? go(ff_tc_kernel<OT, T, PLANES, false, false, FF_STORE>)
-                     : p.b_by_k ? go(ff_tc_kernel<OT, T, PLANES, true, true, FF_STORE>)
-                                : go(ff_tc_kernel<OT, T, PLANES, true, false, FF_STORE>));
+        if (p.kind == FF_GATE) return go(ff_tc_kernel<OT, T, PLANES, true, true, FF_GATE>, Ring<PLANES, FF_GATE>());
+        if (p.kind == FF_GATE_BACK) return go(ff_tc_kernel<OT, T, PLANES, true, false, FF_GATE_BACK>, Ring<PLANES, FF_GATE_BACK>());
+        const Ring<PLANES, FF_STORE> ring;
+        FC_PROPAGATE(!p.a_by_k  ? go(ff_tc_kernel<OT, T, PLANES, false, false, FF_STORE>, ring)
+                     : p.b_by_k ? go(ff_tc_kernel<OT, T, PLANES, true, true, FF_STORE>, ring)
+                                : go(ff_tc_kernel<OT, T, PLANES, true, false, FF_STORE>, ring));
         if (P.splits > 1) {
             long long blocks = ceil_div((size_t)P.m_tiles * 8 * 4 * ceil_div(p.n, 16), 8);
             if (blocks > 148 * 8) blocks = 148 * 8;
