@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(FEW_THREADS) ff_few_kernel(const FfProduct p, 
     const int shares = 1 << log_shares, share = warp & (shares - 1);
     const long long n0 = ((long long)blockIdx.x * (FEW_WARPS >> log_shares) + (warp >> log_shares)) * STEP;
     pdl_wait();
+    pdl_next();
     const T *w[NW];
 #pragma unroll
     for (int j = 0; j < NW; ++j) {

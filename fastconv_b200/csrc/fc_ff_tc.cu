@@ -374,6 +374,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     pdl_wait();
+    pdl_next();
 
     auto decode = [&](uint32_t item, int &mt, int &nt, int &share) {
         const uint32_t rest = item / (uint32_t)P.n_tiles;
@@ -657,6 +658,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
 template <typename T>
 __global__ void __launch_bounds__(256) ff_tc_join_kernel(const FfTc P, T *c0, T *c1, int wide) {
     pdl_wait();
+    pdl_next();
     const int quads = (P.n + 3) / 4, col_blocks = (quads + 3) / 4;
     const long long blocks = (long long)P.m_tiles * 8 * col_blocks * 4;  // of 8 rows x 4 quads: a warp each
     for (long long w = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5; w < blocks; w += (long long)gridDim.x * 8) {

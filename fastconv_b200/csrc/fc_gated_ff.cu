@@ -20,8 +20,6 @@ namespace {
 
 using namespace last;
 
-constexpr int JOIN_THREADS = 256;
-
 // ---- operands that the tensor cores' copies cannot take as they lie ------------------------------------------------
 // fp32, which is split into three bf16 planes, and rows that are no multiples of 16 bytes.  One launch for all of a call's.
 struct PackItem {
@@ -41,6 +39,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) ff_pack_kernel(const PackList list) {
     constexpr int VEC = 16 / sizeof(T), PLANES = sizeof(T) == 4 ? 3 : 1;
     pdl_wait();
+    pdl_next();
     const long long total = list.item[list.count - 1].end;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         int k = 0;
@@ -87,72 +86,103 @@ __global__ void __launch_bounds__(256) ff_pack_kernel(const PackList list) {
 }
 
 // ---- column sums: the biases' gradients ---------------------------------------------------------------------------
-constexpr int SUM_COLS = 32, SUM_ROWS = 8;
+// One launch for the three of a call where a block can add up all rows of its 32 columns; with more rows shares of them, and a
+// second launch that adds the shares in order.
+constexpr int SUM_COLS = 32, SUM_ROWS = 32;
 
-// part[chunk][n]: the sum of the chunk's rows
-template <typename T, int PLANES>
-__global__ void __launch_bounds__(SUM_COLS *SUM_ROWS) ff_colsum_kernel(const T *__restrict__ a, int64_t lda, int64_t plane, int rows,
-                                                                      int n, int chunk_rows, float *__restrict__ part) {
-    __shared__ float s[SUM_ROWS][SUM_COLS];
+struct SumItem {
+    const void *a;
+    int64_t lda, plane;  // plane > 0: the sum of three bf16 planes
+    int n, first;        // columns; the item's first block of columns
+    float *part;         // [chunks][n]
+    void *out;
+};
+struct SumList {
+    SumItem item[3];
+    int count, blocks, rows, chunks, chunk_rows;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(SUM_COLS *SUM_ROWS) ff_colsum_kernel(const SumList list) {
+    __shared__ float s[SUM_ROWS][SUM_COLS + 1];
     pdl_wait();
+    pdl_next();
+    int k = 0;
+    while (k + 1 < list.count && (int)blockIdx.x >= list.item[k + 1].first) ++k;
+    const SumItem &p = list.item[k];
     const int tx = threadIdx.x % SUM_COLS, ty = threadIdx.x / SUM_COLS;
-    const int64_t c = (int64_t)blockIdx.x * SUM_COLS + tx;
-    const int64_t r0 = (int64_t)blockIdx.y * chunk_rows, r1 = min((int64_t)rows, r0 + chunk_rows);
+    const int64_t c = (int64_t)(blockIdx.x - p.first) * SUM_COLS + tx;
+    const int64_t r0 = (int64_t)blockIdx.y * list.chunk_rows, r1 = min((int64_t)list.rows, r0 + list.chunk_rows);
     float v = 0.0f;
-    if (c < n)
-        for (int64_t r = r0 + ty; r < r1; r += SUM_ROWS) {
-            float t = Elem<T>::load(a[r * lda + c]);
-#pragma unroll
-            for (int z = 1; z < PLANES; ++z) t += Elem<T>::load(a[z * plane + r * lda + c]);
-            v += t;
+    if (c < p.n) {
+        if (p.plane > 0) {
+            const __nv_bfloat16 *a = (const __nv_bfloat16 *)p.a + c;
+#pragma unroll 4
+            for (int64_t r = r0 + ty; r < r1; r += SUM_ROWS)
+                v += __bfloat162float(a[r * p.lda]) + __bfloat162float(a[p.plane + r * p.lda]) +
+                     __bfloat162float(a[2 * p.plane + r * p.lda]);
+        } else {
+            const T *a = (const T *)p.a + c;
+#pragma unroll 8
+            for (int64_t r = r0 + ty; r < r1; r += SUM_ROWS) v += Elem<T>::load(a[r * p.lda]);
         }
+    }
     s[ty][tx] = v;
     __syncthreads();
-    if (ty == 0 && c < n) {
+    v = s[tx][ty];  // the sums of column ty, one to a lane
 #pragma unroll
-        for (int i = 1; i < SUM_ROWS; ++i) v += s[i][tx];
-        part[(size_t)blockIdx.y * n + c] = v;
-    }
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int64_t col = (int64_t)(blockIdx.x - p.first) * SUM_COLS + ty;
+    if (tx > 0 || col >= p.n) return;
+    if (list.chunks > 1)
+        p.part[(size_t)blockIdx.y * p.n + col] = v;
+    else
+        ((T *)p.out)[col] = Elem<T>::store(v);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(JOIN_THREADS) ff_colsum_join_kernel(const float *__restrict__ part, int n, int chunks,
-                                                                     T *__restrict__ out) {
+__global__ void __launch_bounds__(SUM_COLS) ff_colsum_join_kernel(const SumList list) {
     pdl_wait();
-    const int64_t c = (int64_t)blockIdx.x * JOIN_THREADS + threadIdx.x;
-    if (c >= n) return;
+    pdl_next();
+    int k = 0;
+    while (k + 1 < list.count && (int)blockIdx.x >= list.item[k + 1].first) ++k;
+    const SumItem &p = list.item[k];
+    const int64_t c = (int64_t)(blockIdx.x - p.first) * SUM_COLS + threadIdx.x;
+    if (c >= p.n) return;
     float v = 0.0f;
-    for (int i = 0; i < chunks; ++i) v += part[(size_t)i * n + c];
-    out[c] = Elem<T>::store(v);
+#pragma unroll 8
+    for (int i = 0; i < list.chunks; ++i) v += p.part[(size_t)i * p.n + c];
+    ((T *)p.out)[c] = Elem<T>::store(v);
 }
 
-int colsum_chunks(int rows, int n) {
-    const long long cols = ceil_div(n, SUM_COLS);
-    long long chunks = ceil_div(148 * 8, cols > 0 ? cols : 1);
-    const long long most = ceil_div(rows, 4 * SUM_ROWS);
-    if (chunks > most) chunks = most;
-    return chunks < 1 ? 1 : (int)chunks;
+// shares of the rows: none up to 2048 of them, else blocks for every SM, of at least 512 rows
+int colsum_chunks(int rows) {
+    if (rows <= 2048) return 1;
+    const long long c = ceil_div(rows, 512);
+    return c > 64 ? 64 : (int)c;
 }
 
-// out[c] = the sum of column c of a, which is of `type` or, where plane > 0, the sum of three bf16 planes;
-// part: colsum_chunks * n floats
-int colsum(fc_context *ctx, int type, const void *a, int64_t lda, int64_t plane, int rows, int n, void *out, float *part) {
-    const int want = colsum_chunks(rows, n);
-    const int chunk_rows = (int)ceil_div(rows, want), chunks = (int)ceil_div(rows, chunk_rows);
-    const dim3 grid((unsigned)ceil_div(n, SUM_COLS), chunks), block(SUM_COLS * SUM_ROWS);
-    return with_type(type, [&](auto t) -> int {
-        using T = decltype(t);
-        if (plane > 0)
-            FC_CHECK_CUDA(launch_pdl(ff_colsum_kernel<__nv_bfloat16, 3>, grid, block, 0, ctx->stream, (const __nv_bfloat16 *)a, lda,
-                                     plane, rows, n, chunk_rows, part));
-        else
-            FC_CHECK_CUDA(launch_pdl(ff_colsum_kernel<T, 1>, grid, block, 0, ctx->stream, (const T *)a, lda, plane, rows, n, chunk_rows,
-                                     part));
-        FC_CHECK_CUDA(launch_pdl(ff_colsum_join_kernel<T>, dim3((unsigned)ceil_div(n, JOIN_THREADS)), dim3(JOIN_THREADS), 0, ctx->stream,
-                                 (const float *)part, n, chunks, (T *)out));
-        return FC_OK;
-    });
-}
+struct Sums {
+    SumList list;
+    void add(const void *a, int64_t lda, int64_t plane, int n, void *out, float *part) {
+        if (out == nullptr) return;
+        list.item[list.count++] = SumItem{a, lda, plane, n, list.blocks, part, out};
+        list.blocks += (int)ceil_div(n, SUM_COLS);
+    }
+    int run(fc_context *ctx, int type, int rows) {
+        if (list.count == 0) return FC_OK;
+        list.rows = rows;
+        list.chunk_rows = (int)ceil_div(rows, colsum_chunks(rows));
+        list.chunks = (int)ceil_div(rows, list.chunk_rows);
+        return with_type(type, [&](auto t) -> int {
+            using T = decltype(t);
+            FC_CHECK_CUDA(launch_pdl(ff_colsum_kernel<T>, dim3(list.blocks, list.chunks), dim3(SUM_COLS * SUM_ROWS), 0, ctx->stream, list));
+            if (list.chunks > 1)
+                FC_CHECK_CUDA(launch_pdl(ff_colsum_join_kernel<T>, dim3(list.blocks), dim3(SUM_COLS), 0, ctx->stream, list));
+            return FC_OK;
+        });
+    }
+};
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 
@@ -254,8 +284,7 @@ Work carve(const Block &b, void *base, bool backward) {
         at_least(ff_tc_part_floats(dx_product(b, w.dgu, w.w_gate, nullptr, nullptr)));
         at_least(ff_tc_part_floats(dw_in_product(b, w.dgu, w.x, nullptr, nullptr)));
         at_least(ff_tc_part_floats(dw_down_product(b, w.dy, w.h, nullptr)));
-        at_least((size_t)colsum_chunks(b.rows, b.hidden) * b.hidden);
-        at_least((size_t)colsum_chunks(b.rows, b.out) * b.out);
+        at_least((size_t)colsum_chunks(b.rows) * (2 * (size_t)b.hidden + b.out));
     }
     w.part = c.take<float>(part);
     w.bytes = c.used;
@@ -415,9 +444,12 @@ int fc_gated_ff_backward(fc_context *ctx, const fc_gated_ff_desc *desc, const vo
 
     const int64_t plane = b.type == FC_DTYPE_F32 ? w.dgu.plane : 0;
     const uint8_t *dgu = (const uint8_t *)w.dgu.p;
-    if (d_db_gate) FC_PROPAGATE(colsum(ctx, b.type, dgu, w.dgu.ld, plane, b.rows, b.hidden, d_db_gate, w.part));
-    if (d_db_up) FC_PROPAGATE(colsum(ctx, b.type, dgu + w.dgu.ld, w.dgu.ld, plane, b.rows, b.hidden, d_db_up, w.part));
-    if (d_db_down) FC_PROPAGATE(colsum(ctx, b.type, d_dy, b.ys, 0, b.rows, b.out, d_db_down, w.part));
+    const size_t chunks = colsum_chunks(b.rows);
+    Sums sums = {};
+    sums.add(dgu, w.dgu.ld, plane, b.hidden, d_db_gate, w.part);
+    sums.add(dgu + w.dgu.ld, w.dgu.ld, plane, b.hidden, d_db_up, w.part + chunks * b.hidden);
+    sums.add(d_dy, b.ys, 0, b.out, d_db_down, w.part + 2 * chunks * b.hidden);
+    FC_PROPAGATE(sums.run(ctx, b.type, b.rows));
     return FC_OK;
 }
 

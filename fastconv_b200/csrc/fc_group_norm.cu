@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_part_kernel(const T *__rest
                                                                 const NormShape s) {
     __shared__ float2 stat[NORM_THREADS * VEC];
     pdl_wait();
+    pdl_next();
     const Place b = place_of<VEC>(s);
     float k[VEC], sum[VEC], sq[VEC];
     int n = 0;
@@ -166,6 +167,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_join_kernel(const float2 *_
                                                                 float *__restrict__ rstd, const NormShape s) {
     __shared__ float scratch[NORM_THREADS / 32];
     pdl_wait();
+    pdl_next();
     const int img = blockIdx.x / s.groups, g = blockIdx.x % s.groups;
     const float2 *src = part + (size_t)img * s.chunks * s.channels + g * s.cpg;
     const int items = s.chunks * s.cpg;
@@ -198,6 +200,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_apply_kernel(const T *__res
                                                                  const NormShape s) {
     constexpr bool kExact = std::is_same<T, float>::value;
     pdl_wait();
+    pdl_next();
     const Place b = place_of<VEC>(s);
     if (!b.live) return;
     float m[VEC], a[VEC], o[VEC];
@@ -265,6 +268,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_part_kernel(const T *_
                                                                      const NormShape s) {
     __shared__ float2 stat[NORM_THREADS * VEC];
     pdl_wait();
+    pdl_next();
     const Place b = place_of<VEC>(s);
     float s1[VEC], s2[VEC];
 #pragma unroll
@@ -308,6 +312,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_join_kernel(const floa
                                                                      float2 *__restrict__ ab, const NormShape s) {
     __shared__ float scratch[NORM_THREADS / 32];
     pdl_wait();
+    pdl_next();
     const int img = blockIdx.x / s.groups, g = blockIdx.x % s.groups;
     float a = 0.0f, q = 0.0f;
     for (int i = threadIdx.x; i < s.cpg; i += NORM_THREADS) {
@@ -338,6 +343,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_apply_kernel(const T *
                                                                       const float2 *__restrict__ ab, T *__restrict__ dx,
                                                                       const NormShape s) {
     pdl_wait();
+    pdl_next();
     const Place b = place_of<VEC>(s);
     if (!b.live) return;
     const BackChannels<T, VEC> ch(gamma, beta, mean, rstd, b.img, b.c0, s);
@@ -548,6 +554,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
     V *mine = data + b.row * f.vectors + b.col;
     const int hop = f.rows * f.vectors;
     pdl_wait();
+    pdl_next();
     if (b.live) {
         const T *src = x + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.xs + b.c0;
         const int64_t src_hop = f.rows * s.xs;
@@ -698,6 +705,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
     const FusedPlace b = fused_place(s, f, VEC);
     const int hop = f.rows * f.vectors, start = b.row * f.vectors + b.col;
     pdl_wait();
+    pdl_next();
     if (b.live) {
         const T *sx = x + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.xs + b.c0;
         const T *sd = dy + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.ys + b.c0;
@@ -861,6 +869,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_params_kernel(const fl
                                                                        const NormShape s) {
     __shared__ float2 shares[8][32];
     pdl_wait();
+    pdl_next();
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
     float2 t = make_float2(0.0f, 0.0f);
     if (c < s.channels)

@@ -335,6 +335,11 @@ class DeviceScope {
     cudaError_t status_;
 };
 
+// Lets the next kernel of the stream begin its set-up (barriers, tensor memory, descriptors) on SMs that this one leaves
+// free or has left; it touches nothing of this one's before its own pdl_wait().  Every block says so after its own wait, which
+// keeps the chain: a kernel ends only after the one before it.
+__device__ __forceinline__ void pdl_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // A launch of clusters of `cluster` blocks, in stream order like every other (programmatic dependent launch).
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, unsigned threads, unsigned cluster, size_t smem,

@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) map_move_kernel(float *__restric
                                                                const MoveShape s) {
     __shared__ float tile[TILE][TILE + 1];  // [channel][pixel]
     pdl_wait();
+    pdl_next();
     const long long id = blockIdx.x;
     const int ct = (int)(id % s.ctiles);
     const long long rest = id / s.ctiles;
