@@ -94,6 +94,10 @@ __device__ __forceinline__ uint32_t first_cta(uint32_t addr) {  // the same plac
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// both CTAs are done with each other's barriers; nothing in memory is handed over
+__device__ __forceinline__ void cluster_leave() {
+    asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
+}
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
     // relaxed: what it stands for are reads of tensor memory, ordered by the tcgen05 fences; a release would wait for the
     // warp's global stores too
@@ -135,6 +139,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
+}
+// what was loaded is there after the wait and not before: keeps its uses behind it
+template <int N>
+__device__ __forceinline__ void tmem_landed(uint32_t (&r)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
@@ -505,6 +515,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                 uint32_t r[32];
                 tmem_ld32(at + lanes, r);
                 tmem_ld_wait();
+                tmem_landed(r);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = add ? v[j] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
             };
@@ -647,7 +658,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
         for (int i = 0; i < 64; ++i) __nanosleep(1000);
     }
     tc_fence_before();
-    cluster_sync();
+    cluster_leave();
     if (warp == 1) {
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");

@@ -21,33 +21,68 @@ struct MoveShape {
     int ctiles, ptiles;
 };
 
-template <typename T, bool kToLast>
+// kPairs: two neighbouring channels of the channels-last map move as one word (16-bit types, even stride, 4-byte aligned).
+template <typename T, bool kToLast, bool kPairs>
 __global__ void __launch_bounds__(MOVE_THREADS) map_move_kernel(float *__restrict__ planes, T *__restrict__ last_map,
                                                                const MoveShape s) {
     __shared__ float tile[TILE][TILE + 1];  // [channel][pixel]
-    pdl_wait();
-    pdl_next();
-    const long long id = blockIdx.x;
-    const int ct = (int)(id % s.ctiles);
-    const long long rest = id / s.ctiles;
-    const int pt = (int)(rest % s.ptiles), img = (int)(rest / s.ptiles);
-    const int c0 = ct * TILE, p0 = pt * TILE;
-    const int tx = threadIdx.x & (TILE - 1), ty = threadIdx.x / TILE;
+    const uint32_t rest = blockIdx.x / (uint32_t)s.ctiles, ct = blockIdx.x - rest * s.ctiles;
+    const uint32_t img = rest / (uint32_t)s.ptiles, pt = rest - img * s.ptiles;
+    const int c0 = (int)ct * TILE, p0 = (int)pt * TILE;
+    const int nc = min(TILE, s.channels - c0), np = min(TILE, s.pixels - p0);
     float *plane = planes + ((size_t)img * s.channels + c0) * s.pixels + p0;
     T *row = last_map + ((size_t)img * s.pixels + p0) * s.stride + c0;
-    const int nc = min(TILE, s.channels - c0), np = min(TILE, s.pixels - p0);
+    const bool whole = nc == TILE && np == TILE;
+    // one side walks over pixels with 64 threads, a channel a step; the other over channels, a pixel a step
+    const int px = threadIdx.x & (TILE - 1), cy = threadIdx.x / TILE;
+    constexpr int C_LANES = kPairs ? TILE / 2 : TILE, P_STEP = MOVE_THREADS / C_LANES, C_STEP = MOVE_THREADS / TILE;
+    const int cx = threadIdx.x % C_LANES, py = threadIdx.x / C_LANES;
+    auto plane_side = [&](auto &&one) {
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < TILE / C_STEP; ++i) one(cy + i * C_STEP);
+        } else if (px < np) {
+            for (int c = cy; c < nc; c += C_STEP) one(c);
+        }
+    };
+    auto last_side = [&](auto &&one) {
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < TILE / P_STEP; ++i) one(py + i * P_STEP);
+        } else {
+            for (int p = py; p < np; p += P_STEP) one(p);
+        }
+    };
+    pdl_wait();
+    pdl_next();
     if (kToLast) {
-        if (tx < np)
-            for (int c = ty; c < nc; c += MOVE_THREADS / TILE) tile[c][tx] = plane[(size_t)c * s.pixels + tx];
+        plane_side([&](int c) { tile[c][px] = __ldg(plane + (size_t)c * s.pixels + px); });
         __syncthreads();
-        if (tx < nc)
-            for (int p = ty; p < np; p += MOVE_THREADS / TILE) row[(size_t)p * s.stride + tx] = Elem<T>::store(tile[tx][p]);
+        last_side([&](int p) {
+            T *to = row + (size_t)p * s.stride;
+            if constexpr (kPairs) {
+                if (2 * cx + 1 < nc)
+                    Elem<T>::store2(to + 2 * cx, tile[2 * cx][p], tile[2 * cx + 1][p]);
+                else if (2 * cx < nc)
+                    to[2 * cx] = Elem<T>::store(tile[2 * cx][p]);
+            } else if (cx < nc) {
+                to[cx] = Elem<T>::store(tile[cx][p]);
+            }
+        });
     } else {
-        if (tx < nc)
-            for (int p = ty; p < np; p += MOVE_THREADS / TILE) tile[tx][p] = Elem<T>::load(row[(size_t)p * s.stride + tx]);
+        last_side([&](int p) {
+            const T *from = row + (size_t)p * s.stride;
+            if constexpr (kPairs) {
+                if (2 * cx + 1 < nc)
+                    Elem<T>::load2(from + 2 * cx, tile[2 * cx][p], tile[2 * cx + 1][p]);
+                else if (2 * cx < nc)
+                    tile[2 * cx][p] = Elem<T>::load(from[2 * cx]);
+            } else if (cx < nc) {
+                tile[cx][p] = Elem<T>::load(from[cx]);
+            }
+        });
         __syncthreads();
-        if (tx < np)
-            for (int c = ty; c < nc; c += MOVE_THREADS / TILE) plane[(size_t)c * s.pixels + tx] = tile[c][tx];
+        plane_side([&](int c) { plane[(size_t)c * s.pixels + px] = tile[c][px]; });
     }
 }
 
@@ -71,9 +106,14 @@ int move(fc_context *ctx, float *planes, void *last_map, int batch, int channels
     FC_CHECK_CUDA(dev.status());
     return with_type(type, [&](auto t) -> int {
         using T = decltype(t);
-        FC_CHECK_CUDA(launch_pdl(to_last ? map_move_kernel<T, true> : map_move_kernel<T, false>, dim3((unsigned)blocks),
-                                 dim3(MOVE_THREADS), 0, ctx->stream, planes, (T *)last_map, s));
-        return FC_OK;
+        auto go = [&](auto kernel) -> int {
+            FC_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)blocks), dim3(MOVE_THREADS), 0, ctx->stream, planes, (T *)last_map, s));
+            return FC_OK;
+        };
+        if constexpr (sizeof(T) == 2)
+            if (stride % 2 == 0 && (uintptr_t)last_map % 4 == 0)
+                return to_last ? go(map_move_kernel<T, true, true>) : go(map_move_kernel<T, false, true>);
+        return to_last ? go(map_move_kernel<T, true, false>) : go(map_move_kernel<T, false, false>);
     });
 }
 
