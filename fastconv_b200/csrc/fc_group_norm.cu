@@ -410,9 +410,9 @@ __device__ __forceinline__ FusedPlace fused_place(const NormShape &s, const Fuse
     return b;
 }
 // use(i, group of the block that the thread's channel i belongs to)
-template <int VEC, typename F>
-__device__ __forceinline__ void over_groups(const NormShape &s, const Fused &f, const FusedPlace &b, F &&use) {
-    if (f.width == VEC) {
+template <int VEC, bool UNI, typename F>
+__device__ __forceinline__ void over_groups(const NormShape &s, const FusedPlace &b, F &&use) {
+    if (UNI) {  // a vector lies in one group
 #pragma unroll
         for (int i = 0; i < VEC; ++i) use(i, b.g0);
         return;
@@ -467,13 +467,12 @@ __device__ __forceinline__ void copy_parts(int np, int part, F &&f) {
 // `tg` neighbouring threads (a power of two) add them without index arithmetic.
 struct GroupSums {
     int groups, slots, log_tg;  // groups of the block; slots of a group in all rows; 2^log_tg threads to a group
-    int width;              // channels of a slot
     float *stat, *scratch, *red;  // [planes][rows * cb], [planes][8], [planes][groups]
     int plane, per_row;
-    template <int VEC>
+    template <int VEC, bool UNI>
     __device__ __forceinline__ void put(const NormShape &s, const FusedPlace &b, int which, const float (&v)[VEC]) const {
         float *to = stat + which * plane + b.row * per_row;
-        if (width == VEC) {
+        if (UNI) {
             float t = 0.0f;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) t += v[i];
@@ -526,12 +525,13 @@ struct GroupSums {
 // Squares are taken around one value of the group, its first in the block.  Where that turns out to be more than four standard
 // deviations from the mean, they are taken once more around the mean, so the variance never loses more than some four of
 // its 24 bits, however far the map is from zero.  The blocks of a cluster are joined by the means' distances.
-template <typename T, int ACT>
-__global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__restrict__ x, const void *__restrict__ gamma,
+template <typename T, int ACT, bool UNI>
+__global__ void __launch_bounds__(FUSED_THREADS, UNI ? 4 : 2) norm_fused_kernel(const T *__restrict__ x, const void *__restrict__ gamma,
                                                                   const void *__restrict__ beta, T *__restrict__ y,
                                                                   float *__restrict__ mean, float *__restrict__ rstd,
                                                                   const NormShape s, const Fused f) {
     constexpr int VEC = 16 / sizeof(T);
+    constexpr int OF_GROUP = UNI ? 1 : VEC / 2;  // pairs of what belongs to a group
     constexpr bool kExact = std::is_same<T, float>::value;
     using V = Vec<T, VEC>;
     namespace cg = cooperative_groups;
@@ -540,7 +540,6 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
     V *data = (V *)smem;  // [pc][vectors]
     GroupSums gs;
     gs.groups = f.groups;
-    gs.width = f.width;
     gs.per_row = f.per_row;
     gs.slots = f.rows * f.per_row;
     gs.log_tg = f.log_tg;
@@ -568,13 +567,13 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
     const bool sums = threadIdx.x < gs.groups;
     float level = sums ? Elem<T>::load(corner[threadIdx.x * s.cpg]) : 0.0f;
     float v[VEC], u[VEC];
-    over_groups<VEC>(s, f, b, [&](int i, int g) { v[i] = b.live ? -Elem<T>::load(corner[g * s.cpg]) : 0.0f; });
+    over_groups<VEC, UNI>(s, b, [&](int i, int g) { v[i] = b.live ? -Elem<T>::load(corner[g * s.cpg]) : 0.0f; });
     const float n_inv = quick_inverse((float)b.np * (float)s.cpg);
     auto deviations = [&](auto &&passes) {  // from -v; their sums and squares' sums to gs.red
-        Pair from[VEC / 2], sum[VEC / 2], sq[VEC / 2];
+        Pair from[OF_GROUP], sum[VEC / 2], sq[VEC / 2];
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) {
-            from[i] = pair(v[2 * i], v[2 * i + 1]);
+            if (i < OF_GROUP) from[i] = pair(v[2 * i], v[2 * i + 1]);
             sum[i] = sq[i] = 0;
         }
         const V *at = mine;
@@ -586,7 +585,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
                 unpack_pairs(V::load(at), q);
 #pragma unroll
                 for (int i = 0; i < VEC / 2; ++i) {
-                    const Pair d = add2(q[i], from[i]);
+                    const Pair d = add2(q[i], from[UNI ? 0 : i]);
                     sum[i] = add2(sum[i], d);
                     sq[i] = fma2(d, d, sq[i]);
                 }
@@ -599,8 +598,8 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
                 a[2 * i] = split(sum[i]).x, a[2 * i + 1] = split(sum[i]).y;
                 c[2 * i] = split(sq[i]).x, c[2 * i + 1] = split(sq[i]).y;
             }
-            gs.put<VEC>(s, b, 0, a);
-            gs.put<VEC>(s, b, 1, c);
+            gs.put<VEC, UNI>(s, b, 0, a);
+            gs.put<VEC, UNI>(s, b, 1, c);
         }
         gs.template add<2>();
     };
@@ -613,7 +612,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
         share[threadIdx.x] = make_float2(level, fmaxf(q, 0.0f));
     }
     if (__syncthreads_or(sums && !(gs.red[threadIdx.x] * d <= 16.0f * q) && d != 0.0f)) {
-        over_groups<VEC>(s, f, b, [&](int i, int g) { v[i] = b.live ? -share[g].x : 0.0f; });
+        over_groups<VEC, UNI>(s, b, [&](int i, int g) { v[i] = b.live ? -share[g].x : 0.0f; });
         deviations([&](auto &&part) { part(0, b.np); });
         if (sums) {
             d = gs.red[threadIdx.x] * n_inv;
@@ -652,18 +651,18 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
     __syncthreads();
     if (f.cluster > 1) cluster_arrive();
     if (b.live) {
-        Pair m[VEC / 2], a[VEC / 2], o[VEC / 2];
+        Pair m[OF_GROUP], a[VEC / 2], o[VEC / 2];
         float w[VEC];
         params<T, VEC>(gamma, b.c0, s.params_f32, 1.0f, u);
         params<T, VEC>(beta, b.c0, s.params_f32, 0.0f, v);
-        over_groups<VEC>(s, f, b, [&](int i, int g) {
+        over_groups<VEC, UNI>(s, b, [&](int i, int g) {
             const float2 t = total[g];
             u[i] *= t.y;
             w[i] = -t.x;
         });
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) {
-            m[i] = pair(w[2 * i], w[2 * i + 1]);
+            if (i < OF_GROUP) m[i] = pair(w[2 * i], w[2 * i + 1]);
             a[i] = pair(u[2 * i], u[2 * i + 1]);
             o[i] = pair(v[2 * i], v[2 * i + 1]);
         }
@@ -676,7 +675,7 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
             unpack_pairs(V::load(at), q);
 #pragma unroll
             for (int i = 0; i < VEC / 2; ++i)
-                q[i] = act_value2<ACT, kExact>(fma2(add2(q[i], m[i]), a[i], o[i]));
+                q[i] = act_value2<ACT, kExact>(fma2(add2(q[i], m[UNI ? 0 : i]), a[i], o[i]));
             V out;
             pack_pairs(out, q);
             out.store(dst);
@@ -686,8 +685,8 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_fused_kernel(const T *__re
 }
 
 // sums[img * channels + c]: the image's (sum dz, sum dz xhat)
-template <typename T, int ACT>
-__global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T *__restrict__ dy, const T *__restrict__ x,
+template <typename T, int ACT, bool UNI>
+__global__ void __launch_bounds__(FUSED_THREADS, UNI ? 4 : 2) norm_back_fused_kernel(const T *__restrict__ dy, const T *__restrict__ x,
                                                                        const void *__restrict__ gamma,
                                                                        const void *__restrict__ beta,
                                                                        const float *__restrict__ mean,
@@ -719,29 +718,31 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
         });
     }
     constexpr bool kExact = std::is_same<T, float>::value;
-    Pair m[VEC / 2], r[VEC / 2], gm[VEC / 2], bt[VEC / 2];  // -mean, rstd, gamma, beta
+    // With xm = x - mean:  z = (gamma rstd) xm + beta,  dx = (gamma rstd) dz - rstd A - xm (rstd^2 B).  What belongs to a group
+    // is one pair where a vector lies in one (UNI).
+    constexpr int PAIRS = VEC / 2, OF_GROUP = UNI ? 1 : PAIRS;
+    Pair m[OF_GROUP], gr[PAIRS], bt[PAIRS];  // -mean, gamma rstd, beta
     if (b.live) {
-        float fm[VEC], fr[VEC], fg[VEC], fb[VEC];
-        over_groups<VEC>(s, f, b, [&](int i, int g) {
-            const int at = b.img * s.groups + b.cblk * f.groups + g;
-            fr[i] = rstd[at];
-            fm[i] = -mean[at];
-        });
+        float fm[VEC], fg[VEC], fb[VEC];
         params<T, VEC>(gamma, b.c0, s.params_f32, 1.0f, fg);
         params<T, VEC>(beta, b.c0, s.params_f32, 0.0f, fb);
+        over_groups<VEC, UNI>(s, b, [&](int i, int g) {
+            const int at = b.img * s.groups + b.cblk * f.groups + g;
+            fm[i] = -mean[at];
+            fg[i] *= rstd[at];
+        });
 #pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) {
-            m[i] = pair(fm[2 * i], fm[2 * i + 1]);
-            r[i] = pair(fr[2 * i], fr[2 * i + 1]);
-            gm[i] = pair(fg[2 * i], fg[2 * i + 1]);
+        for (int i = 0; i < PAIRS; ++i) {
+            if (i < OF_GROUP) m[i] = pair(fm[2 * i], fm[2 * i + 1]);
+            gr[i] = pair(fg[2 * i], fg[2 * i + 1]);
             bt[i] = pair(fb[2 * i], fb[2 * i + 1]);
         }
     }
-    // dz and xhat of a pair of channels
-    auto one = [&](int i, Pair v, Pair d, Pair &dz, Pair &xhat) {
-        xhat = mul2(add2(v, m[i]), r[i]);
+    // dz and x - mean of a pair of channels
+    auto one = [&](int i, Pair v, Pair d, Pair &dz, Pair &xm) {
+        xm = add2(v, m[UNI ? 0 : i]);
         Pair a, slope;
-        act_both2<ACT, kExact>(fma2(xhat, gm[i], bt[i]), a, slope);
+        act_both2<ACT, kExact>(fma2(xm, gr[i], bt[i]), a, slope);
         dz = mul2(d, slope);
     };
     {
@@ -751,25 +752,28 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
         int at = start;
         as_they_land(b.np, f.part, [&](int from, int upto) {
             if (!b.live) return;
+#pragma unroll 1
             for (int p = from + b.row; p < upto; p += f.rows, at += hop) {
                 Pair v[VEC / 2], d[VEC / 2];
                 unpack_pairs(V::load(xs + at), v);
                 unpack_pairs(V::load(ds + at), d);
 #pragma unroll
                 for (int i = 0; i < VEC / 2; ++i) {
-                    Pair dz, xhat;
-                    one(i, v[i], d[i], dz, xhat);
+                    Pair dz, xm;
+                    one(i, v[i], d[i], dz, xm);
                     s1[i] = add2(s1[i], dz);
-                    s2[i] = fma2(dz, xhat, s2[i]);
+                    s2[i] = fma2(dz, xm, s2[i]);
                 }
             }
         });
         if (b.live) {
+            float fr[VEC];
+            over_groups<VEC, UNI>(s, b, [&](int i, int g) { fr[i] = rstd[b.img * s.groups + b.cblk * f.groups + g]; });
 #pragma unroll
             for (int i = 0; i < VEC / 2; ++i) {
                 const float2 p = split(s1[i]), q = split(s2[i]);
-                stat[b.row * f.cb + b.col * VEC + 2 * i] = make_float2(p.x, q.x);
-                stat[b.row * f.cb + b.col * VEC + 2 * i + 1] = make_float2(p.y, q.y);
+                stat[b.row * f.cb + b.col * VEC + 2 * i] = make_float2(p.x, q.x * fr[2 * i]);
+                stat[b.row * f.cb + b.col * VEC + 2 * i + 1] = make_float2(p.y, q.y * fr[2 * i + 1]);
             }
         }
     }
@@ -832,27 +836,31 @@ __global__ void __launch_bounds__(FUSED_THREADS) norm_back_fused_kernel(const T 
                 a += __shfl_xor_sync(0xffffffffu, a, o);
                 q += __shfl_xor_sync(0xffffffffu, q, o);
             }
-            if (lane == 0) ab[g] = make_float2(a * inv, q * inv);
+            if (lane == 0) {
+                const float r = rstd[b.img * s.groups + b.cblk * f.groups + g];
+                ab[g] = make_float2(-a * inv * r, -q * inv * r * r);
+            }
         }
         __syncthreads();
         if (b.live) {
             float fa[VEC], fb[VEC];
-            over_groups<VEC>(s, f, b, [&](int i, int g) { fa[i] = -ab[g].x, fb[i] = -ab[g].y; });
-            Pair ta[VEC / 2], tb[VEC / 2];
+            over_groups<VEC, UNI>(s, b, [&](int i, int g) { fa[i] = ab[g].x, fb[i] = ab[g].y; });
+            Pair ta[OF_GROUP], tb[OF_GROUP];
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) ta[i] = pair(fa[2 * i], fa[2 * i + 1]), tb[i] = pair(fb[2 * i], fb[2 * i + 1]);
+            for (int i = 0; i < OF_GROUP; ++i) ta[i] = pair(fa[2 * i], fa[2 * i + 1]), tb[i] = pair(fb[2 * i], fb[2 * i + 1]);
             T *dst = dx + ((size_t)b.img * s.pixels + b.p0 + b.row) * s.xs + b.c0;
             const int64_t dst_hop = f.rows * s.xs;
             int at = start;
+#pragma unroll 1
             for (int p = b.row; p < b.np; p += f.rows, at += hop, dst += dst_hop) {
                 Pair v[VEC / 2], d[VEC / 2];
                 unpack_pairs(V::load(xs + at), v);
                 unpack_pairs(V::load(ds + at), d);
 #pragma unroll
                 for (int i = 0; i < VEC / 2; ++i) {
-                    Pair dz, xhat;
-                    one(i, v[i], d[i], dz, xhat);
-                    v[i] = mul2(r[i], fma2(xhat, tb[i], fma2(dz, gm[i], ta[i])));
+                    Pair dz, xm;
+                    one(i, v[i], d[i], dz, xm);
+                    v[i] = fma2(dz, gr[i], fma2(xm, tb[UNI ? 0 : i], ta[UNI ? 0 : i]));
                 }
                 V out;
                 pack_pairs(out, v);
@@ -933,9 +941,11 @@ void norm_split(NormShape *s, int vec) {
 }
 
 // The one-kernel form for vectors of 16 bytes, or false where an image's smallest block of channels is more than eight
-// blocks' shared memory holds.  Chosen by an estimate in nanoseconds: `waves` rounds of blocks of about 2.5 us (3.5 in a
-// cluster), which two or more blocks of an SM overlap; 0.7 us of instructions that a block takes whatever it holds; and the bytes at 6500 a nanosecond, less where the runs of a pixel are
-// short (memory moves 32 bytes, and is quick from 128 on) or where there are fewer blocks than SMs.
+// blocks' shared memory holds.  Chosen by an estimate in nanoseconds: `waves` rounds of blocks of about 2.5 us, in a cluster 350
+// ns a block more, which several blocks of an SM overlap; 0.7 us of instructions that a block takes whatever it holds; and
+// the bytes at 6500 a nanosecond, less where the runs of a pixel are shorter than the 32 bytes that memory moves or where
+// there are fewer blocks than SMs.  64 x 56x56x256 bf16 forward: runs of 64 bytes in clusters of 4 57 us, of 32 in 2 60, of 128 in
+// 8 63, of 64 in 8 71, of 32 in one block 79; in three kernels 103 (backward 124 against 187).
 bool fused_plan(const NormShape &s, int esize, bool backward, Fused *best) {
     const int vec = 16 / esize, arrays = backward ? 2 : 1;
     if (s.channels % vec || s.batch > 65535) return false;
@@ -961,9 +971,9 @@ bool fused_plan(const NormShape &s, int esize, bool backward, Fused *best) {
             double per_sm = 220.0 * 1024 / (f.smem + 1024.0);
             per_sm = per_sm > 6 ? 6 : (double)(int)per_sm;
             const double waves = (double)(long long)((blocks + 148 * per_sm - 1) / (148 * per_sm));
-            const double eff = (run >= 128 ? 1.0 : run >= 64 ? 0.85 : run >= 32 ? 0.6 : 0.3) * (blocks < 148 ? blocks / 148 : 1.0) *
+            const double eff = (run >= 64 ? 1.0 : run >= 32 ? 0.95 : 0.6) * (blocks < 148 ? blocks / 148 : 1.0) *
                                (per_sm < 2 ? 0.75 : 1.0);
-            const double cost = waves * (cluster > 1 ? 3500.0 : 2500.0) / (waves > 1 ? per_sm : 1.0) + blocks / 148 * 700.0 +
+            const double cost = waves * (2500.0 + (cluster > 1 ? 350.0 * cluster : 0.0)) / (waves > 1 ? per_sm : 1.0) + blocks / 148 * 700.0 +
                                 bytes / (6500.0 * eff);
             if (cost < best_cost) {
                 best_cost = cost;
@@ -1071,7 +1081,8 @@ int fc_group_norm_forward(fc_context *ctx, const fc_group_norm_desc *desc, const
         if constexpr (VEC > 1) {
             if (fused_plan(s, sizeof(T), false, &f))
                 return with_act(desc->act, [&](auto a) -> int {
-                    auto kernel = norm_fused_kernel<T, decltype(a)::value>;
+                    constexpr int A = decltype(a)::value;
+                    auto kernel = f.width > 1 ? norm_fused_kernel<T, A, true> : norm_fused_kernel<T, A, false>;
                     FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
                     FC_CHECK_CUDA(launch_clusters(kernel, dim3(f.blocks * f.cluster, s.batch), FUSED_THREADS, f.cluster, f.smem,
                                                   ctx->stream, (const T *)d_x, d_gamma, d_beta, (T *)d_y, d_mean, d_rstd, s, f));
@@ -1124,7 +1135,8 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
         if (fused) {
             if constexpr (VEC > 1)
                 FC_PROPAGATE(with_act(desc->act, [&](auto a) -> int {
-                    auto kernel = norm_back_fused_kernel<T, decltype(a)::value>;
+                    constexpr int A = decltype(a)::value;
+                    auto kernel = f.width > 1 ? norm_back_fused_kernel<T, A, true> : norm_back_fused_kernel<T, A, false>;
                     FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
                     FC_CHECK_CUDA(launch_clusters(kernel, dim3(f.blocks * f.cluster, s.batch), FUSED_THREADS, f.cluster, f.smem,
                                                   ctx->stream, (const T *)d_dy, (const T *)d_x, d_gamma, d_beta, d_mean, d_rstd,
