@@ -71,7 +71,6 @@ struct FfTc {
     int saved_wide;           // in float4
     void *c0, *c1;            // FF_STORE: destinations that are stored to without TMA (else null)
     int64_t ldc;
-    int c_wide;               // in 16-byte vectors
     float *part;
     int *status;
 };
@@ -230,25 +229,19 @@ __device__ __forceinline__ void add_bias(const void *bias, int wide, int n, int 
     }
 }
 
-// 32 columns of one row, from n on
+// 32 rows x 32 columns that lie in registers a row a lane -> rows y.. and columns x.. of c, turned in the warp's 4 KB of shared
+// memory so that a warp writes a row's neighbouring columns: for destinations that TMA cannot address, and fp32.
 template <typename T>
-__device__ __forceinline__ void store_row(T *row, int wide, int n, int n_end, const float (&v)[32]) {
-    constexpr int VEC = 16 / sizeof(T);
-    if (wide && n + 32 <= n_end) {
+__device__ __forceinline__ void store_block(float *turn, T *c, int64_t ldc, int y, int m, int x, int n, const float (&v)[32], int lane) {
 #pragma unroll
-        for (int i = 0; i < 32; i += VEC) {
-            float f[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) f[j] = v[i + j];
-            Vec<T, VEC> w;
-            w.pack(f);
-            w.store(row + n + i);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (n + i < n_end) row[n + i] = Elem<T>::store(v[i]);
-    }
+    for (int j = 0; j < 32; ++j) turn[lane * 32 + (j ^ lane)] = v[j];
+    __syncwarp();
+    const int rows = min(32, m - y);
+    T *to = c + (size_t)y * ldc + x + lane;
+    if (x + lane < n)
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r, to += ldc) *to = Elem<T>::store(turn[r * 32 + (lane ^ r)]);
+    __syncwarp();
 }
 
 // 32 saved values of the row y + lane, from column x on (ff_saved_at)
@@ -293,11 +286,11 @@ __device__ __forceinline__ void put_planes(Outlet<PIECES> &out, const CUtensorMa
         out.template put<OT>(map, v, x, y, 0, lane);
     } else {
         float part[32];
-#pragma unroll
+#pragma unroll 1
         for (int z = 0; z < 3; ++z) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-                part[j] = z < 2 ? bf16_part(v[j]) : v[j];
+                part[j] = bf16_part(v[j]);  // the last part is what is left: 8 bits, kept as it is
                 v[j] = fabsf(part[j]) <= 3.4028234e38f ? v[j] - part[j] : 0.0f;
             }
             out.template put<OT>(map, part, x, y, z, lane);
@@ -305,21 +298,55 @@ __device__ __forceinline__ void put_planes(Outlet<PIECES> &out, const CUtensorMa
     }
 }
 
-template <int ACT, bool kExact>
+// fp32: a call for two values at a time (act, act' of both), and not 32 copies of the library's functions, whose 80 KB of
+// straight code a tile would wait for
+__device__ __noinline__ float4 exact_act(int act, float y, float z) {
+    float4 r;
+    switch (act) {
+        case FC_ACT_GELU: act_both<FC_ACT_GELU, true>(y, r.x, r.y), act_both<FC_ACT_GELU, true>(z, r.z, r.w); break;
+        case FC_ACT_GELU_TANH: act_both<FC_ACT_GELU_TANH, true>(y, r.x, r.y), act_both<FC_ACT_GELU_TANH, true>(z, r.z, r.w); break;
+        case FC_ACT_SILU: act_both<FC_ACT_SILU, true>(y, r.x, r.y), act_both<FC_ACT_SILU, true>(z, r.z, r.w); break;
+        default: act_both_rt(act, y, r.x, r.y), act_both_rt(act, z, r.z, r.w);
+    }
+    return r;
+}
+__device__ __forceinline__ void gate_values_exact(int act, float (&g)[32], const float (&u)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        const float4 f = exact_act(act, g[j], g[j + 1]);
+        g[j] = f.x * u[j];
+        g[j + 1] = f.z * u[j + 1];
+    }
+}
+__device__ __forceinline__ void gate_back_values_exact(int act, float (&g)[32], float (&u)[32], float (&dh)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        const float4 f = exact_act(act, g[j], g[j + 1]);
+        const float h0 = f.x * u[j], h1 = f.z * u[j + 1];
+        g[j] = dh[j] * u[j] * f.y;
+        g[j + 1] = dh[j + 1] * u[j + 1] * f.w;
+        u[j] = dh[j] * f.x;
+        u[j + 1] = dh[j + 1] * f.z;
+        dh[j] = h0;
+        dh[j + 1] = h1;
+    }
+}
+
+template <int ACT>
 __device__ __forceinline__ void gate_values(float (&g)[32], const float (&u)[32]) {  // in: g, u; out: h in g
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-        const float2 h = split(mul2(act_value2<ACT, kExact>(pair(g[j], g[j + 1])), pair(u[j], u[j + 1])));
+        const float2 h = split(mul2(act_value2<ACT, false>(pair(g[j], g[j + 1])), pair(u[j], u[j + 1])));
         g[j] = h.x, g[j + 1] = h.y;
     }
 }
-template <int ACT, bool kExact>
+template <int ACT>
 __device__ __forceinline__ void gate_back_values(float (&g)[32], float (&u)[32], float (&dh)[32]) {
     // in: g, u, dh; out: dg, du, h
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
         Pair a, d;
-        act_both2<ACT, kExact>(pair(g[j], g[j + 1]), a, d);
+        act_both2<ACT, false>(pair(g[j], g[j + 1]), a, d);
         const Pair up = pair(u[j], u[j + 1]), e = pair(dh[j], dh[j + 1]);
         const float2 dg = split(mul2(mul2(e, up), d)), du = split(mul2(e, a)), h = split(mul2(a, up));
         g[j] = dg.x, g[j + 1] = dg.y;
@@ -501,6 +528,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     } else {
         const int quad = warp & 3, half = (warp - 2) >> 2;  // tensor memory lanes of this warp; every second column piece
         Outlet<R::kPieces> out = {out_base + (uint32_t)(warp - 2) * R::kPieces * PIECE, 0};
+        float *turn = reinterpret_cast<float *>(smem_raw + (out.base - smem_u32(smem_raw)));
         const int cols = KIND == FF_GATE ? P.bn / 2 : P.bn;  // output columns of a tile
         int t = 0, c = 0;
         bool ok = true;
@@ -530,13 +558,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                 }
             };
             auto back = [&](float (&g)[32], float (&u)[32], float (&v)[32]) {  // in: g, u, dh; out: dg, du, h
-                switch (P.act) {
-                    case FC_ACT_RELU: gate_back_values<FC_ACT_RELU, kExact>(g, u, v); break;
-                    case FC_ACT_SILU: gate_back_values<FC_ACT_SILU, kExact>(g, u, v); break;
-                    case FC_ACT_GELU: gate_back_values<FC_ACT_GELU, kExact>(g, u, v); break;
-                    case FC_ACT_GELU_TANH: gate_back_values<FC_ACT_GELU_TANH, kExact>(g, u, v); break;
-                    case FC_ACT_SIGMOID: gate_back_values<FC_ACT_SIGMOID, kExact>(g, u, v); break;
-                    default: gate_back_values<FC_ACT_NONE, kExact>(g, u, v);
+                if constexpr (kExact) {
+                    gate_back_values_exact(P.act, g, u, v);
+                } else {
+                    switch (P.act) {
+                        case FC_ACT_RELU: gate_back_values<FC_ACT_RELU>(g, u, v); break;
+                        case FC_ACT_SILU: gate_back_values<FC_ACT_SILU>(g, u, v); break;
+                        case FC_ACT_GELU: gate_back_values<FC_ACT_GELU>(g, u, v); break;
+                        case FC_ACT_GELU_TANH: gate_back_values<FC_ACT_GELU_TANH>(g, u, v); break;
+                        case FC_ACT_SIGMOID: gate_back_values<FC_ACT_SIGMOID>(g, u, v); break;
+                        default: gate_back_values<FC_ACT_NONE>(g, u, v);
+                    }
                 }
             };
             // 32 columns from x on: v the product; FF_GATE: v the gate's, u the up projection's
@@ -549,13 +581,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                         saved_row<true>(P, P.gate, y, lane, x, v);
                         saved_row<true>(P, P.up, y, lane, x, u);
                     }
-                    switch (P.act) {
-                        case FC_ACT_RELU: gate_values<FC_ACT_RELU, kExact>(v, u); break;
-                        case FC_ACT_SILU: gate_values<FC_ACT_SILU, kExact>(v, u); break;
-                        case FC_ACT_GELU: gate_values<FC_ACT_GELU, kExact>(v, u); break;
-                        case FC_ACT_GELU_TANH: gate_values<FC_ACT_GELU_TANH, kExact>(v, u); break;
-                        case FC_ACT_SIGMOID: gate_values<FC_ACT_SIGMOID, kExact>(v, u); break;
-                        default: gate_values<FC_ACT_NONE, kExact>(v, u);
+                    if constexpr (kExact) {
+                        gate_values_exact(P.act, v, u);
+                    } else {
+                        switch (P.act) {
+                            case FC_ACT_RELU: gate_values<FC_ACT_RELU>(v, u); break;
+                            case FC_ACT_SILU: gate_values<FC_ACT_SILU>(v, u); break;
+                            case FC_ACT_GELU: gate_values<FC_ACT_GELU>(v, u); break;
+                            case FC_ACT_GELU_TANH: gate_values<FC_ACT_GELU_TANH>(v, u); break;
+                            case FC_ACT_SIGMOID: gate_values<FC_ACT_SIGMOID>(v, u); break;
+                            default: gate_values<FC_ACT_NONE>(v, u);
+                        }
                     }
                     put_planes<OT, PLANES, R::kPieces>(out, &maps.c[0], v, x, y, lane);
                 } else if (KIND == FF_GATE_BACK) {
@@ -578,7 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                     add_bias<T>(P.bias0, P.bias_wide, x, P.n, v);
                     T *c = (T *)(dest ? P.c1 : P.c0);
                     if (c != nullptr) {
-                        if (row < P.m) store_row(c + (size_t)row * P.ldc, P.c_wide, x, P.n, v);
+                        store_block(turn, c, P.ldc, y, P.m, x, P.n, v, lane);
                     } else if constexpr (PLANES == 1) {
                         out.template put<OT>(&maps.c[dest], v, x, y, 0, lane);
                     }
@@ -810,7 +846,6 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
     if (!by_copies) {
         P.c0 = p.c0;
         P.c1 = p.c1;
-        P.c_wide = c_wide;
     }
 
     FfMaps maps;
