@@ -195,7 +195,8 @@ int block_of(const fc_gated_ff_desc *d, Block *b) {
     FC_REQUIRE(d != nullptr, FC_ERR_INVALID_ARG, "descriptor is NULL");
     FC_REQUIRE(d->rows >= 0 && d->in_channels > 0 && d->hidden > 0 && d->out_channels > 0, FC_ERR_INVALID_ARG,
                "rows %d, channels in %d, hidden %d, out %d", d->rows, d->in_channels, d->hidden, d->out_channels);
-    FC_REQUIRE(d->hidden < (1 << 30), FC_ERR_UNSUPPORTED, "%d hidden channels", d->hidden);
+    FC_REQUIRE(d->in_channels < (1 << 30) && d->hidden < (1 << 30) && d->out_channels < (1 << 30), FC_ERR_UNSUPPORTED,
+               "channels in %d, hidden %d, out %d", d->in_channels, d->hidden, d->out_channels);
     FC_REQUIRE(dtype_ok(d->type), FC_ERR_INVALID_ARG, "unknown element type %d", d->type);
     FC_REQUIRE(act_ok(d->act), FC_ERR_INVALID_ARG, "unknown activation %d", d->act);
     const int64_t xs = d->x_stride ? d->x_stride : d->in_channels, ys = d->y_stride ? d->y_stride : d->out_channels;
@@ -364,6 +365,7 @@ int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const voi
     if (b.rows == 0) return FC_OK;
     FC_PROPAGATE(check_pointers(b, {d_x, d_w_gate, d_w_up, d_w_down, d_y}, {d_b_gate, d_b_up, d_b_down}));
     FC_REQUIRE((uintptr_t)d_saved % 4 == 0, FC_ERR_INVALID_ARG, "the saved values' address is no multiple of 4");
+    FC_REQUIRE(d_y != d_x, FC_ERR_INVALID_ARG, "the output is the input");
     const Work w = carve(b, d_workspace, false);
     FC_PROPAGATE(check_workspace(d_workspace, workspace_bytes, w.bytes));
     DeviceScope dev(ctx->device);
@@ -407,6 +409,7 @@ int fc_gated_ff_backward(fc_context *ctx, const fc_gated_ff_desc *desc, const vo
     if (b.rows > 0) FC_PROPAGATE(check_pointers(b, {d_dy, d_x, d_w_gate, d_w_up, d_w_down, d_saved}, {}));
     FC_REQUIRE((uintptr_t)d_saved % 4 == 0, FC_ERR_INVALID_ARG, "the saved values' address is no multiple of 4");
     FC_PROPAGATE(check_pointers(b, {}, {d_dx, d_dw_gate, d_dw_up, d_dw_down, d_db_gate, d_db_up, d_db_down}));
+    FC_REQUIRE(d_dx == nullptr || (d_dx != d_x && d_dx != d_dy), FC_ERR_INVALID_ARG, "an output is an input");
     const Work w = carve(b, d_workspace, true);
     FC_PROPAGATE(check_workspace(d_workspace, workspace_bytes, w.bytes));
     DeviceScope dev(ctx->device);

@@ -910,6 +910,7 @@ int norm_shape(const fc_group_norm_desc *d, NormShape *s) {
     FC_REQUIRE(d != nullptr, FC_ERR_INVALID_ARG, "descriptor is NULL");
     FC_REQUIRE(d->batch >= 0 && d->pixels > 0 && d->channels > 0 && d->groups > 0, FC_ERR_INVALID_ARG,
                "batch %d, pixels %d, channels %d, groups %d", d->batch, d->pixels, d->channels, d->groups);
+    FC_REQUIRE(d->pixels < (1 << 30) && d->channels <= (1 << 20), FC_ERR_UNSUPPORTED, "%d pixels of %d channels", d->pixels, d->channels);
     FC_REQUIRE(d->channels % d->groups == 0, FC_ERR_INVALID_ARG, "%d groups do not divide %d channels", d->groups, d->channels);
     FC_REQUIRE(dtype_ok(d->type), FC_ERR_INVALID_ARG, "unknown element type %d", d->type);
     FC_REQUIRE(d->param_type == FC_DTYPE_F32 || d->param_type == d->type, FC_ERR_INVALID_ARG,
@@ -1068,6 +1069,7 @@ int fc_group_norm_forward(fc_context *ctx, const fc_group_norm_desc *desc, const
     FC_PROPAGATE(norm_shape(desc, &s));
     if (s.batch == 0) return FC_OK;
     FC_PROPAGATE(check_maps(desc, {d_x, d_y}, {d_gamma, d_beta}));
+    FC_REQUIRE(d_y != d_x, FC_ERR_INVALID_ARG, "the output is the input");
     size_t need;
     FC_PROPAGATE(fc_group_norm_workspace(desc, &need, nullptr));
     FC_REQUIRE(d_workspace != nullptr && aligned16(d_workspace) && workspace_bytes >= need, FC_ERR_INVALID_ARG,
@@ -1114,6 +1116,7 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
     NormShape s;
     FC_PROPAGATE(norm_shape(desc, &s));
     if (s.batch > 0) FC_PROPAGATE(check_maps(desc, {d_dy, d_x, d_dx ? d_dx : d_x}, {d_gamma, d_beta, d_dgamma, d_dbeta}));
+    FC_REQUIRE(d_dx == nullptr || (d_dx != d_x && d_dx != d_dy), FC_ERR_INVALID_ARG, "an output is an input");
     FC_REQUIRE(s.batch == 0 || (d_mean != nullptr && d_rstd != nullptr), FC_ERR_INVALID_ARG,
                "the gradient needs the forward pass's mean and rstd");
     size_t need;

@@ -91,6 +91,7 @@ int move(fc_context *ctx, float *planes, void *last_map, int batch, int channels
     FC_REQUIRE(ctx != nullptr, FC_ERR_INVALID_ARG, "context is NULL");
     FC_REQUIRE(batch >= 0 && channels > 0 && pixels > 0, FC_ERR_INVALID_ARG, "batch %d, channels %d, pixels %d", batch,
                channels, pixels);
+    FC_REQUIRE(channels < (1 << 30) && pixels < (1 << 30), FC_ERR_UNSUPPORTED, "%d channels, %d pixels", channels, pixels);
     FC_REQUIRE(dtype_ok(type), FC_ERR_INVALID_ARG, "unknown element type %d", type);
     if (stride == 0) stride = channels;
     FC_REQUIRE(stride >= channels, FC_ERR_INVALID_ARG, "pixel stride %lld is less than the %d channels", (long long)stride,

@@ -445,7 +445,9 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
  *   y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd
  * with the weights of 1x1 convolutions, contiguous: w_gate, w_up [hidden][in_channels], w_down [out_channels][hidden];
  * one row is a single token or pixel.  Weights, biases, gradients and maps are of one type; between the kernels the
- * products act(.) * (.), and in the backward pass the gradients of gate and up, are rounded to that type. */
+ * products act(.) * (.), and in the backward pass the gradients of gate and up, are rounded to that type (in fp32 they
+ * keep 24 bits).  fp32 values are multiplied as sums of three bf16 parts: where an operand or an intermediate is infinite,
+ * fp32 results that depend on it are NaN. */
 typedef struct fc_gated_ff_desc {
     int32_t rows, in_channels, hidden, out_channels; /* rows 0: nothing to do (the weights' gradients are then zero) */
     int32_t type;                                    /* fc_dtype */

@@ -55,6 +55,15 @@ def test_null_contexts_and_descriptors_are_refused():
     assert lib.fc_gated_ff_workspace(C.byref(ffd(hidden=1 << 30)), None, None) == _lib.FC_ERR_UNSUPPORTED
 
 
+def test_sizes_that_indices_do_not_hold_are_refused():
+    lib, unsupported = fc.load(), _lib.FC_ERR_UNSUPPORTED
+    assert lib.fc_group_norm_workspace(C.byref(gn(pixels=1 << 30)), None, None) == unsupported
+    assert lib.fc_group_norm_workspace(C.byref(gn(channels=1 << 21)), None, None) == unsupported
+    assert lib.fc_group_norm_workspace(C.byref(gn(batch=1 << 30, groups=4)), None, None) == unsupported
+    for name in ("in_channels", "hidden", "out_channels"):
+        assert lib.fc_gated_ff_workspace(C.byref(ffd(**{name: 1 << 30})), None, None) == unsupported
+
+
 def test_names_are_checked():
     with pytest.raises(ValueError, match="act"):
         fc.GroupNorm(1, 1, 8, 2, act="swish", ctx=object())

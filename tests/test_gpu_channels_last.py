@@ -463,3 +463,185 @@ def test_two_plans_interleave_on_one_stream(lctx):
             plan.forward(at(x), at(y), **{k: at(v) for k, v in w.items()})
     done(lctx)
     assert all(torch.equal(a, b) for a, b in zip(*ys)) and torch.equal(ys[0][0], ys[0][2])
+
+
+# ---- refusals that need a context -----------------------------------------------------------------------------------
+
+def test_calls_that_are_refused(lctx):
+    """Nothing is launched: the checks are the host's."""
+    lib, bad = fc.load(), -1
+    a = torch.full((4096,), GUARD, device="cuda")
+    p, q, w, h = a.data_ptr(), a.data_ptr() + 4096, a.data_ptr() + 8192, lctx.handle
+    torch.cuda.synchronize()
+    assert lib.fc_map_to_channels_last(h, None, q, 1, 4, 4, 0, 0) == bad
+    assert lib.fc_map_to_channels_last(h, p + 2, q, 1, 4, 4, 0, 0) == bad
+    assert lib.fc_map_from_channels_last(h, p + 1, q, 1, 4, 4, 0, 1) == bad
+    assert lib.fc_map_to_channels_last(h, p, q, 1, 4, 4, 3, 0) == bad
+    assert lib.fc_map_to_channels_last(h, p, q, 1, 4, 4, 0, 7) == bad
+    assert lib.fc_map_to_channels_last(h, p, q, -1, 4, 4, 0, 0) == bad
+    assert lib.fc_map_to_channels_last(h, p, q, 1, 1 << 30, 4, 0, 0) == -2
+    gn = fc.GroupNorm(1, 16, 8, 2, ctx=lctx)
+    d, n = gn._ref, gn.workspace_bytes
+    fwd = lib.fc_group_norm_forward
+    assert fwd(h, d, p, None, None, None, None, None, w, n) == bad
+    assert fwd(h, d, p, None, None, p, None, None, w, n) == bad
+    assert fwd(h, d, p + 2, None, None, q, None, None, w, n) == bad
+    assert fwd(h, d, p, p + 1, None, q, None, None, w, n) == bad
+    assert fwd(h, d, p, None, None, q, None, None, None, n) == bad
+    assert fwd(h, d, p, None, None, q, None, None, w + 4, n) == bad
+    assert fwd(h, d, p, None, None, q, None, None, w, 16) == bad
+    bwd = lib.fc_group_norm_backward
+    assert bwd(h, d, p, p + 512, None, None, None, None, q, None, None, w, n) == bad  # no mean and rstd
+    assert bwd(h, d, p, q, None, None, p, p, q, None, None, w, n) == bad
+    assert bwd(h, d, p, q, None, None, p, p, w, None, None, w, 16) == bad
+    ff = fc.GatedFeedForward(4, 8, 16, dtype="fp32", train=True, ctx=lctx)
+    d, n = ff._ref, ff.workspace_bytes
+    fwd, bwd = lib.fc_gated_ff_forward, lib.fc_gated_ff_backward
+    ops = [p, p, p, p, None, None, None, q, None, w, n]
+    for i, v in ((0, None), (1, None), (2, None), (3, None), (7, None), (7, p), (0, p + 2), (4, p + 1), (8, p + 2), (9, None), (9, w + 8),
+                 (10, 64)):
+        assert fwd(h, d, *[v if j == i else o for j, o in enumerate(ops)]) == bad, i
+    ops = [p, p, p, p, p, p, q, None, None, None, None, None, None, w, n]
+    for i, v in ((0, None), (1, None), (2, None), (3, None), (4, None), (5, None), (6, p), (6, q + 1), (7, q + 2), (5, p + 2), (13, None),
+                 (14, 64)):
+        assert bwd(h, d, *[v if j == i else o for j, o in enumerate(ops)]) == bad, i
+    with pytest.raises(RuntimeError, match="train"):
+        fc.GatedFeedForward(4, 8, 16, dtype="fp32", ctx=lctx).backward(p, p, w_gate=p, w_up=p, w_down=p, saved=p)
+    gn.release()
+    with pytest.raises(RuntimeError, match="released"):
+        gn.forward(p, q)
+    done(lctx)
+    assert bool((a == GUARD).all())
+
+
+# ---- far offsets, far levels ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("channels", [16, 15])
+def test_offsets_past_32_bits(lctx, channels):
+    """Rows so far apart that the last ones' offsets pass 2^31 elements."""
+    rows, stride = 40000, 1 << 16
+    flat = torch.empty(rows * stride, dtype=torch.bfloat16, device="cuda")
+    view = flat.view(rows, stride)
+    x = torch.randn(rows, channels, generator=gen(61)).cuda().bfloat16()
+    view[:, :channels] = x
+    near = torch.empty_like(x)
+    for kind in ("norm", "ff", "move"):
+        torch.cuda.synchronize()
+        if kind == "norm":
+            for xs, ys, src, dst in ((0, 0, x, near), (stride, stride, view, view[:, 64:])):
+                fc.GroupNorm(1, rows, channels, 1, act="silu", dtype="bf16", x_stride=xs, y_stride=ys, ctx=lctx).forward(at(src), at(dst))
+        elif kind == "ff":
+            w = {k: (0.2 * torch.randn(*s, generator=gen(62))).cuda().bfloat16() for k, s in
+                 (("w_gate", (24, channels)), ("w_up", (24, channels)), ("w_down", (channels, 24)))}
+            torch.cuda.synchronize()
+            for xs, ys, src, dst in ((0, 0, x, near), (stride, stride, view, view[:, 64:])):
+                fc.GatedFeedForward(rows, channels, 24, dtype="bf16", x_stride=xs, y_stride=ys, ctx=lctx).forward(
+                    at(src), at(dst), **{k: at(v) for k, v in w.items()})
+        else:
+            planes = torch.empty(channels, rows, device="cuda")
+            torch.cuda.synchronize()
+            fc.from_channels_last(at(view), at(planes), 1, channels, rows, dtype="bf16", stride=stride, ctx=lctx)
+            fc.to_channels_last(at(planes), at(view[:, 64:]), 1, channels, rows, dtype="bf16", stride=stride, ctx=lctx)
+            near = x
+        done(lctx)
+        assert torch.equal(view[:, 64:64 + channels], near), kind
+    assert torch.equal(view[:, :channels], x)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("p,c,groups", [(196, 64, 8), (5000, 64, 4), (777, 33, 3)])
+def test_norm_where_a_groups_first_value_is_far_off(lctx, dtype, p, c, groups):
+    """The value that squares are taken around is an outlier of 3000 standard deviations."""
+    n = 2
+    x = torch.randn(n, p, c, generator=gen(71))
+    x[:, 0, ::c // groups] = 3000.0
+    x[:, p // 2, 1::c // groups] = -2000.0
+    x = x.cuda().to(DTYPES[dtype])
+    y, mean, rstd = torch.empty_like(x), torch.empty(n, groups, device="cuda"), torch.empty(n, groups, device="cuda")
+    plan = fc.GroupNorm(n, p, c, groups, dtype=dtype, ctx=lctx)
+    torch.cuda.synchronize()
+    plan.forward(at(x), at(y), mean=at(mean), rstd=at(rstd))
+    done(lctx)
+    one, zero = torch.ones(c, dtype=torch.float64), torch.zeros(c, dtype=torch.float64)
+    want = norm(x.double().cpu(), groups, 1e-5, one, zero, "none", dtype)
+    check(y, *want["y"], dtype, "y")
+    check(rstd, *want["rstd"], "fp32", "rstd")
+
+
+def test_ff_of_very_large_and_very_small_fp32(lctx):
+    """Operands of 1e20 and 1e-20: each is split by its own size."""
+    rows, k, f = 140, 72, 136
+    g = gen(81)
+    t = {"x": 1e20 * torch.randn(rows, k, generator=g), "w_gate": 1e-20 * torch.randn(f, k, generator=g) * k ** -0.5,
+         "w_up": 1e-20 * torch.randn(f, k, generator=g) * k ** -0.5, "w_down": 1e18 * torch.randn(k, f, generator=g) * f ** -0.5}
+    t = {n: v.cuda() for n, v in t.items()}
+    y = torch.empty(rows, k, device="cuda")
+    plan = fc.GatedFeedForward(rows, k, f, dtype="fp32", ctx=lctx)
+    torch.cuda.synchronize()
+    plan.forward(at(t["x"]), at(y), **{n: at(v) for n, v in t.items() if n != "x"})
+    done(lctx)
+    want = ff({**{n: v.double().cpu() for n, v in t.items()}, "b_gate": None, "b_up": None, "b_down": None}, "silu", "fp32")
+    check(y, *want["y"], "fp32", "y")
+
+
+def test_a_nan_stays_in_its_row(lctx):
+    rows, k, f = 300, 64, 128
+    for dtype in ("fp32", "bf16"):
+        dt = DTYPES[dtype]
+        g = gen(91)
+        x = torch.randn(rows, k, generator=g).to(dt).cuda()
+        x[137, 5] = float("nan")
+        x[299, 63] = float("inf")
+        w = {n: (0.1 * torch.randn(*s, generator=g)).to(dt).cuda() for n, s in
+             (("w_gate", (f, k)), ("w_up", (f, k)), ("w_down", (k, f)))}
+        y = torch.empty_like(x)
+        plan = fc.GatedFeedForward(rows, k, f, dtype=dtype, ctx=lctx)
+        torch.cuda.synchronize()
+        plan.forward(at(x), at(y), **{n: at(v) for n, v in w.items()})
+        done(lctx)
+        bad = ~torch.isfinite(y)
+        assert bool(torch.isnan(y[137]).all()) and bool(bad[299].all()) and int(bad.sum()) == 2 * k
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_a_training_step_replayed_from_a_graph(lctx, dtype):
+    """Norm and block, forward and backward, captured once and replayed on other inputs: the bits of the calls."""
+    n, p, c, f, groups = 3, 150, 64, 136, 8
+    dt = DTYPES[dtype]
+    g = gen(101)
+    rnd = lambda *s: (0.5 * torch.randn(*s, generator=g)).to(dt).cuda()  # noqa: E731
+    x, dy, w = rnd(n * p, c), rnd(n * p, c), {"w_gate": rnd(f, c), "w_up": rnd(f, c), "w_down": rnd(c, f)}
+    gamma, beta = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda")
+    mean, rstd, saved = torch.empty(n, groups, device="cuda"), torch.empty(n, groups, device="cuda"), torch.empty(2, n * p, f, device="cuda")
+    outs = {"mid": torch.empty_like(x), "y": torch.empty_like(x), "dmid": torch.empty_like(x), "dx": torch.empty_like(x),
+            "dgamma": torch.empty_like(gamma), "dbeta": torch.empty_like(beta), **{"d" + k: torch.empty_like(v) for k, v in w.items()}}
+    gn = fc.GroupNorm(n, p, c, groups, act="gelu", dtype=dtype, ctx=lctx)
+    block = fc.GatedFeedForward(n * p, c, f, dtype=dtype, train=True, ctx=lctx)
+
+    def step():
+        gn.forward(at(x), at(outs["mid"]), gamma=at(gamma), beta=at(beta), mean=at(mean), rstd=at(rstd))
+        block.forward(at(outs["mid"]), at(outs["y"]), **{k: at(v) for k, v in w.items()}, saved=at(saved))
+        block.backward(at(dy), at(outs["mid"]), at(outs["dmid"]), **{k: at(v) for k, v in w.items()}, saved=at(saved),
+                       **{"d" + k: at(outs["d" + k]) for k in w})
+        gn.backward(at(outs["dmid"]), at(x), at(outs["dx"]), gamma=at(gamma), beta=at(beta), mean=at(mean), rstd=at(rstd),
+                    dgamma=at(outs["dgamma"]), dbeta=at(outs["dbeta"]))
+
+    stream, graph = torch.cuda.ExternalStream(lctx.stream.value), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for _ in range(2):
+        x.copy_(rnd(n * p, c))
+        torch.cuda.synchronize()
+        step()
+        done(lctx)
+        called = {k: v.clone() for k, v in outs.items()}
+        for v in outs.values():
+            v.fill_(GUARD)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        done(lctx)
+        for k, v in outs.items():
+            assert torch.equal(v, called[k]), k
+    del graph
