@@ -763,10 +763,11 @@ int matrix_map(CUtensorMap *map, bool bf16, const void *base, long long cols, lo
 
 }  // namespace
 
-// Tile width and shares of the reduction, by an estimate in SM clocks: a k-block of 256 x bn takes 2 bn clocks of the matrix
-// pipe and (16 KB + 64 bn bytes) at about 56 bytes a clock of operand copies; the first tile's latency and a tile's epilogue
-// that nothing hides, about 2500; a split result is written and read once more by every share (about 3000 bytes a clock, all SMs),
-// and joined by a kernel of its own (about 4000).
+// Tile width and shares of the reduction, by an estimate in SM clocks.  A k-block of 256 x 256 takes 512 clocks of the matrix pipe
+// and is measured at 560; one of 128 or 64 columns takes 435 all the same (an instruction takes some 108 clocks to read its
+// 256 rows of A), so narrow tiles only serve to occupy more SMs; of three planes 24 instructions, 2600.  Operand copies run at
+// about 60 bytes a clock.  The first tile's latency and a last epilogue that nothing hides come to about 5000; a split result is
+// written and read once more by every share (about 3000 bytes a clock, all SMs) and joined by a kernel of its own (about 4000).
 struct FfTcPlan {
     int bn, splits;
 };
@@ -781,9 +782,9 @@ static FfTcPlan ff_tc_plan(int planes, int kind, int dests, int m, int n, int kb
             if (s > 1 && kb_total / s < 4) break;
             const int share = (int)ceil_div(kb_total, s);
             if (s > 1 && (s - 1) * share >= kb_total) continue;  // the last share would be empty
-            const double copies = planes * (16384.0 + 64.0 * bn) / 56.0, mma = (planes == 1 ? 2.0 : 12.0) * bn;
+            const double copies = planes * (16384.0 + 64.0 * bn) / 60.0, mma = planes == 3 ? 2600.0 : bn > 128 ? 560.0 : 435.0;
             const double waves = (double)ceil_div((size_t)(tiles * s), pairs);
-            double cost = waves * share * (copies > mma ? copies : mma) + 2500.0;
+            double cost = waves * share * (copies > mma ? copies : mma) + 5000.0;
             if (s > 1) cost += 4000.0 + (double)s * dests * m * n * 8.0 / 3000.0;
             if (cost < best_cost * 0.999) {
                 best_cost = cost;
