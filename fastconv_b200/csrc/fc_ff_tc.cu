@@ -51,7 +51,9 @@ struct Ring {
     static constexpr int kMost = 10;  // stages
     static constexpr int kSmem = 1024 + kBytes + kOut + 256;
 };
-__host__ __device__ constexpr int ff_stage_bytes(int planes, int bn) { return planes * (HALF_BYTES + bn * 64); }
+// A stage holds one k-block of bn = 256 (512 clocks of the matrix pipe) or of three planes, else two: a stage's round of wait,
+// commit and release takes some 430 clocks, which one k-block of a narrower tile does not fill.
+__host__ __device__ constexpr int ff_kb_bytes(int planes, int bn) { return planes * (HALF_BYTES + bn * 64); }
 
 struct FfMaps {
     CUtensorMap a[2], b[2], c[3];
@@ -64,6 +66,7 @@ struct FfTc {
     int n_tiles, splits;
     int kb_total, kb_first, kb_share;  // k-blocks; those before kb_first come from the first maps; of one share
     int bn, stages, act;
+    int kbs;                  // k-blocks of a stage
     int items;                // tiles times shares
     const void *bias0, *bias1;
     int bias_wide;            // the biases can be read in 16-byte vectors
@@ -364,7 +367,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
     constexpr int kMost = R::kMost;
     const int S = P.stages;
     const uint32_t b_bytes = (uint32_t)P.bn * 64;  // this CTA's share of B in a stage and plane
-    const uint32_t stage_bytes = PLANES * (HALF_BYTES + b_bytes);
+    const uint32_t kb_bytes = PLANES * (HALF_BYTES + b_bytes);
+    const int kbs = PLANES == 1 ? P.kbs : 1;
+    const uint32_t stage_bytes = kbs * kb_bytes;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const uint32_t out_base = smem + R::kBytes;
@@ -434,33 +439,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
             const int m0 = (mt - dest * P.dest_tiles) * 256 + (int)rank * 128;
             const int n0 = KIND == FF_GATE ? nt * (P.bn / 2) : nt * P.bn + (int)rank * (P.bn / 2);
             const int lo = share * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
-            for (int kb = lo; kb < hi; ++kb) {
+            for (int k_lo = lo; k_lo < hi; k_lo += kbs) {
                 if (!mbar_wait(bar_empty(s), phase ^ 1, abort_flag, P.status)) {
                     ok = false;
                     break;
                 }
                 if (elect_one()) {
-                    const uint32_t a_at = smem + s * stage_bytes, b_at = a_at + PLANES * HALF_BYTES;
+                    const int k_hi = min(hi, k_lo + kbs);
                     const uint32_t full = first_cta(bar_full(s));
-                    if (rank == 0) mbar_expect_tx(bar_full(s), 2 * PLANES * (HALF_BYTES + b_bytes));
-                    const int second = kb >= P.kb_first;
-                    const int k0 = (second ? kb - P.kb_first : kb) * KB;
-                    const CUtensorMap *am = &maps.a[A_BY_K ? second : dest];
-                    const CUtensorMap *bm = &maps.b[KIND == FF_GATE ? (int)rank : second];
+                    if (rank == 0) mbar_expect_tx(bar_full(s), 2 * (k_hi - k_lo) * kb_bytes);
+                    uint32_t a_at = smem + s * stage_bytes;
+                    for (int kb = k_lo; kb < k_hi; ++kb, a_at += kb_bytes) {
+                        const uint32_t b_at = a_at + PLANES * HALF_BYTES;
+                        const int second = kb >= P.kb_first;
+                        const int k0 = (second ? kb - P.kb_first : kb) * KB;
+                        const CUtensorMap *am = &maps.a[A_BY_K ? second : dest];
+                        const CUtensorMap *bm = &maps.b[KIND == FF_GATE ? (int)rank : second];
 #pragma unroll
-                    for (int z = 0; z < PLANES; ++z) {
-                        const uint32_t az = a_at + z * HALF_BYTES, bz = b_at + z * b_bytes;
-                        if (A_BY_K) {
-                            pair_load(az, am, full, k0, m0, z);
-                        } else {
+                        for (int z = 0; z < PLANES; ++z) {
+                            const uint32_t az = a_at + z * HALF_BYTES, bz = b_at + z * b_bytes;
+                            if (A_BY_K) {
+                                pair_load(az, am, full, k0, m0, z);
+                            } else {
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) pair_load(az + i * KB * 128, am, full, m0 + 64 * i, k0, z);
-                        }
-                        if (B_BY_K) {
-                            pair_load(bz, bm, full, k0, n0, z);
-                        } else {
-                            pair_load(bz, bm, full, n0, k0, z);
-                            if (P.bn > 128) pair_load(bz + KB * 128, bm, full, n0 + 64, k0, z);
+                                for (int i = 0; i < 2; ++i) pair_load(az + i * KB * 128, am, full, m0 + 64 * i, k0, z);
+                            }
+                            if (B_BY_K) {
+                                pair_load(bz, bm, full, k0, n0, z);
+                            } else {
+                                pair_load(bz, bm, full, n0, k0, z);
+                                if (P.bn > 128) pair_load(bz + KB * 128, bm, full, n0 + 64, k0, z);
+                            }
                         }
                     }
                 }
@@ -495,29 +504,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                     }
                     tc_fence_after();
                     const uint32_t d = tmem + acc * P.bn;
-                    for (int kb = k_lo; kb < k_hi; ++kb) {
+                    for (int kb = k_lo; kb < k_hi; kb += kbs) {
                         if (!mbar_wait(bar_full(s), phase, abort_flag, P.status)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
                         if (elect_one()) {
-                            const uint32_t a_at = smem + s * stage_bytes, b_at = a_at + PLANES * HALF_BYTES;
+                            uint32_t a_at = smem + s * stage_bytes;
+                            const int upto = min(k_hi, kb + kbs);
+                            for (int j = kb; j < upto; ++j, a_at += kb_bytes) {
+                                const uint32_t b_at = a_at + PLANES * HALF_BYTES;
 #pragma unroll
-                            for (int k = 0; k < KB / 16; ++k) {  // 16 steps: 32 bytes along a row, or 16 rows
-                                auto a = [&](int z) { return operand<A_BY_K>(a_at + z * HALF_BYTES + k * (A_BY_K ? 32 : 2048)); };
-                                auto b = [&](int z) { return operand<B_BY_K>(b_at + z * b_bytes + k * (B_BY_K ? 32 : 2048)); };
-                                pair_mma(d, a(0), b(0), idesc, kb > k_lo || k > 0);
-                                if (PLANES == 3) {
-                                    pair_mma(small, a(0), b(1), idesc, kb > lo || k > 0);
-                                    pair_mma(small, a(1), b(0), idesc, 1);
-                                    pair_mma(small, a(0), b(2), idesc, 1);
-                                    pair_mma(small, a(2), b(0), idesc, 1);
-                                    pair_mma(small, a(1), b(1), idesc, 1);
+                                for (int k = 0; k < KB / 16; ++k) {  // 16 steps: 32 bytes along a row, or 16 rows
+                                    auto a = [&](int z) { return operand<A_BY_K>(a_at + z * HALF_BYTES + k * (A_BY_K ? 32 : 2048)); };
+                                    auto b = [&](int z) { return operand<B_BY_K>(b_at + z * b_bytes + k * (B_BY_K ? 32 : 2048)); };
+                                    pair_mma(d, a(0), b(0), idesc, j > k_lo || k > 0);
+                                    if (PLANES == 3) {
+                                        pair_mma(small, a(0), b(1), idesc, j > lo || k > 0);
+                                        pair_mma(small, a(1), b(0), idesc, 1);
+                                        pair_mma(small, a(0), b(2), idesc, 1);
+                                        pair_mma(small, a(2), b(0), idesc, 1);
+                                        pair_mma(small, a(1), b(1), idesc, 1);
+                                    }
                                 }
                             }
                             pair_commit(bar_empty(s));
-                            if (kb == k_hi - 1) pair_commit(bar_acc_full(acc));
+                            if (kb + kbs >= k_hi) pair_commit(bar_acc_full(acc));
                         }
                         __syncwarp();
                         if (++s == S) s = 0, phase ^= 1;
@@ -764,10 +777,10 @@ int matrix_map(CUtensorMap *map, bool bf16, const void *base, long long cols, lo
 }  // namespace
 
 // Tile width and shares of the reduction, by an estimate in SM clocks.  A k-block of 256 x 256 takes 512 clocks of the matrix pipe
-// and is measured at 560; one of 128 or 64 columns takes 435 all the same (an instruction takes some 108 clocks to read its
-// 256 rows of A), so narrow tiles only serve to occupy more SMs; of three planes 24 instructions, 2600.  Operand copies run at
-// about 60 bytes a clock.  The first tile's latency and a last epilogue that nothing hides come to about 5000; a split result is
-// written and read once more by every share (about 3000 bytes a clock, all SMs) and joined by a kernel of its own (about 4000).
+// and is measured at 560, one of 128 columns at 275 and of 64 at 215 (two to a stage; 435 each with one); of three planes, 24
+// instructions of 128 columns, at 1600.  Operand copies run at about 60 bytes a clock.  The first tile's latency and a last
+// epilogue that nothing hides come to about 5000; a split result is written and read once more by every share (about
+// 3000 bytes a clock, all SMs) and joined by a kernel of its own (about 4000).
 struct FfTcPlan {
     int bn, splits;
 };
@@ -782,7 +795,7 @@ static FfTcPlan ff_tc_plan(int planes, int kind, int dests, int m, int n, int kb
             if (s > 1 && kb_total / s < 4) break;
             const int share = (int)ceil_div(kb_total, s);
             if (s > 1 && (s - 1) * share >= kb_total) continue;  // the last share would be empty
-            const double copies = planes * (16384.0 + 64.0 * bn) / 60.0, mma = planes == 3 ? 2600.0 : bn > 128 ? 560.0 : 435.0;
+            const double copies = planes * (16384.0 + 64.0 * bn) / 60.0, mma = planes == 3 ? 1600.0 : bn == 256 ? 560.0 : bn == 128 ? 275.0 : 215.0;
             const double waves = (double)ceil_div((size_t)(tiles * s), pairs);
             double cost = waves * share * (copies > mma ? copies : mma) + 5000.0;
             if (s > 1) cost += 4000.0 + (double)s * dests * m * n * 8.0 / 3000.0;
@@ -886,7 +899,8 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
         auto go = [&](auto kernel, auto ring) -> int {
             using R = decltype(ring);
             constexpr int SMEM = R::kSmem;
-            const int room = R::kBytes / ff_stage_bytes(PLANES, P.bn);
+            P.kbs = PLANES == 1 && P.bn < 256 ? 2 : 1;
+            const int room = R::kBytes / (P.kbs * ff_kb_bytes(PLANES, P.bn));
             P.stages = room < R::kMost ? room : R::kMost;
             FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
             FC_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(2 * pairs)), dim3(FF_TC_THREADS), SMEM, ctx->stream, maps, P));
