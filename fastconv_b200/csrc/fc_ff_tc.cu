@@ -3,7 +3,7 @@
 // A pair of CTAs computes 256 x bn outputs (bn = 64, 128 or 256) with tcgen05.mma.cta_group::2: each CTA stages its own 128
 // rows of A and half of B's columns, so an operand byte is fetched into shared memory once for 256 rows or bn columns.
 // Persistent; per CTA
-//   warp 0      producer: TMA boxes of 64 reduction steps into a ring of stages
+//   warp 0      producer: TMA boxes of 64 reduction steps (a k-block) into a ring of stages
 //   warp 1      of the pair's first CTA: the matrix instructions, into one of two accumulators in tensor memory
 //   warps 2..9  epilogue of the other accumulator: 32 rows x 32 columns at a time, from tensor memory through registers and
 //               a swizzled 2 KB piece of shared memory to a TMA store, which also cuts off what lies outside the matrix
@@ -17,7 +17,13 @@
 // values the six largest are taken, hh, hm, mh, hl, lh, mm; the others are below 2^-25 of the result.  The tensor cores' fp32
 // additions round toward zero, which over a long reduction adds up to a bias of some 2e-8 an instruction: the five small
 // products, where that does not matter, have an accumulator of their own, and the sum of hh is taken over into registers,
-// rounded to nearest, every 256 steps.  Six times the work of a bf16 product, and still four times the FP32 pipe's rate.
+// rounded to nearest, every 256 steps.  Six times the work of a bf16 product; 95 TFLOP/s at 3137 rows 256->1024->256, where
+// products on the FP32 pipe gave 29.
+//
+// What bounds them, measured on one B200 in bf16: a plain product of 210 GFLOP takes 126 to 144 us by the clock that the power
+// cap leaves, the matrix pipe active 0.94 of the time; the gate's of 50176 rows 512->2048 (210 GFLOP) 136 us, 0.91.  With 12544
+// rows 1024->4096 the gate that also writes 0.41 GB of saved values takes 177 us, and the backward gate (105 GFLOP) 150 us for
+// 0.75 GB, 5 TB/s: memory.  Small products are bound by a tile's way through set-up, first copies and epilogue, 5 us.
 #include <cstring>
 #include <type_traits>
 
@@ -32,8 +38,8 @@ namespace {
 using namespace last;
 using namespace tc;
 
-constexpr int KB = 64;                    // reduction steps of a stage: 128 bytes, one swizzle span
-constexpr int HALF_BYTES = 128 * KB * 2;  // one CTA's A in a stage and plane
+constexpr int KB = 64;                    // reduction steps of a k-block: 128 bytes, one swizzle span
+constexpr int HALF_BYTES = 128 * KB * 2;  // one CTA's A in a k-block and plane
 constexpr int EPI_WARPS = 8;
 constexpr int PIECE = 32 * 32 * 2;        // 32 rows x 32 columns of 16 bits
 constexpr int FF_TC_THREADS = 64 + 32 * EPI_WARPS;

@@ -10,7 +10,10 @@
 // so that a level far from zero costs no digits.  No atomics: results are the same from run to run.
 //
 // One kernel where a cluster's shared memory holds an image's block of channels (then a map is read once); otherwise
-// three each way: sums of a chunk of pixels per channel, their join per group, the map itself.
+// three each way: sums of a chunk of pixels per channel, their join per group, the map itself.  The bound is memory: 64 x
+// 28x28x512 fp32 takes 46 us (4.5 TB/s, 0.68 of the measured copy rate; two blocks of 100 KB to an SM leave memory waiting
+// between a block's loads and its stores), 64 x 56x56x256 bf16 57 us forward and 124 us backward (3.6 and 2.5 TB/s), where
+// instructions and the special-function unit are as busy as memory.
 #include <cooperative_groups.h>
 
 #include <numeric>
