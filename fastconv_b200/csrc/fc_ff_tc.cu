@@ -860,9 +860,10 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
     P.ldc = p.ldc;
     P.part = p.part;
     P.status = ctx->d_status;
-    // FF_STORE goes through TMA where the destination allows it
+    // FF_STORE goes through TMA where the destination allows it.  A store is cut off at 16 bytes: where the columns end inside
+    // such a piece, zeros would go to what lies behind them.  (In the workspace they may.)
     const bool c_wide = p.ldc % vec == 0 && aligned16(p.c0) && aligned16(p.c1);
-    const bool by_copies = p.kind != FF_STORE || (p.planes == 1 && c_wide);
+    const bool by_copies = p.kind != FF_STORE || (p.planes == 1 && c_wide && p.n % vec == 0);
     if (!by_copies) {
         P.c0 = p.c0;
         P.c1 = p.c1;

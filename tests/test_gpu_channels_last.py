@@ -645,3 +645,79 @@ def test_a_training_step_replayed_from_a_graph(lctx, dtype):
         for k, v in outs.items():
             assert torch.equal(v, called[k]), k
     del graph
+
+
+def test_norm_of_very_many_images(lctx):
+    """More images than a launch has rows of blocks."""
+    run_norm(lctx, 70000, 4, 8, 2, "silu", "fp32")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("k", [64, 65])
+def test_what_lies_between_rows_does_not_matter(lctx, dtype, k):
+    """NaN between the channels of the maps: the same bits as from maps without gaps, in the block and in the norm."""
+    rows, f, wide = 200, 72, 80
+    dt = DTYPES[dtype]
+    g = gen(111)
+    rnd = lambda *s: (0.5 * torch.randn(*s, generator=g)).to(dt).cuda()  # noqa: E731
+    x, dy = rnd(rows, k), rnd(rows, k)
+    w = {"w_gate": rnd(f, k), "w_up": rnd(f, k), "w_down": rnd(k, f)}
+    gapped = {n: torch.full((rows, wide), float("nan"), dtype=dt, device="cuda") for n in ("x", "dy", "y", "dx", "n", "ndx")}
+    gapped["x"][:, :k], gapped["dy"][:, :k] = x, dy
+    results = []
+    for stride, t in ((0, {"x": x, "dy": dy, **{n: torch.empty_like(x) for n in ("y", "dx", "n", "ndx")}}), (wide, gapped)):
+        saved, mean, rstd = torch.empty(2, rows, f, device="cuda"), torch.empty(2, 1, device="cuda"), torch.empty(2, 1, device="cuda")
+        grads = {"d" + n: torch.empty_like(v) for n, v in w.items()}
+        block = fc.GatedFeedForward(rows, k, f, dtype=dtype, x_stride=stride, y_stride=stride, train=True, ctx=lctx)
+        gn = fc.GroupNorm(2, rows // 2, k, 1, act="silu", dtype=dtype, x_stride=stride, y_stride=stride, ctx=lctx)
+        dgamma, dbeta = torch.empty(2, k, device="cuda")
+        torch.cuda.synchronize()
+        block.forward(at(t["x"]), at(t["y"]), **{n: at(v) for n, v in w.items()}, saved=at(saved))
+        block.backward(at(t["dy"]), at(t["x"]), at(t["dx"]), **{n: at(v) for n, v in w.items()}, saved=at(saved),
+                       **{n: at(v) for n, v in grads.items()})
+        gn.forward(at(t["x"]), at(t["n"]), mean=at(mean), rstd=at(rstd))
+        gn.backward(at(t["dy"]), at(t["x"]), at(t["ndx"]), mean=at(mean), rstd=at(rstd), dgamma=at(dgamma), dbeta=at(dbeta))
+        done(lctx)
+        for n in ("y", "dx", "n", "ndx"):
+            assert torch.isnan(t[n][:, k:]).all()
+        results.append([t[n][:, :k].clone() for n in ("y", "dx")] + list(grads.values()))
+        norms = [t["n"][:, :k], t["ndx"][:, :k], dgamma, dbeta, mean, rstd]
+        assert all(bool(torch.isfinite(v).all()) for v in norms)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_two_contexts_at_once(lctx):
+    """Calls of two contexts overlap on the GPU; each has its own stream and workspaces, and gets the bits it gets alone."""
+    other = fc.Context(0, arena_bytes=512 << 20)
+    try:
+        g = gen(121)
+        jobs = []
+        for ctx, (rows, k, f) in ((lctx, (3000, 256, 520)), (other, (2000, 320, 264))):
+            t = {"x": torch.randn(rows, k, generator=g).cuda().bfloat16()}
+            for n, s in (("w_gate", (f, k)), ("w_up", (f, k)), ("w_down", (k, f))):
+                t[n] = (0.05 * torch.randn(*s, generator=g)).cuda().bfloat16()
+            jobs.append((fc.GatedFeedForward(rows, k, f, dtype="bf16", ctx=ctx), fc.GroupNorm(4, rows // 4, k, 8, act="silu", dtype="bf16", ctx=ctx),
+                         t, torch.empty_like(t["x"]), torch.empty_like(t["x"])))
+
+        def run(job):
+            plan, gn, t, mid, y = job
+            gn.forward(at(t["x"]), at(mid))
+            plan.forward(at(mid), at(y), **{n: at(v) for n, v in t.items() if n != "x"})
+
+        torch.cuda.synchronize()
+        alone = []
+        for job in jobs:
+            run(job)
+            lctx.synchronize()
+            other.synchronize()
+            alone.append(job[4].clone())
+            job[4].fill_(GUARD)
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for job in jobs:
+                run(job)
+        lctx.synchronize()
+        other.synchronize()
+        assert all(torch.equal(job[4], a) for job, a in zip(jobs, alone))
+    finally:
+        other.close()
