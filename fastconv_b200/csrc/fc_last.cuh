@@ -111,6 +111,17 @@ __device__ __forceinline__ float fast_exp(float z) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(z * 1.44269504088896341f));
     return r;
 }
+// the larger and the smaller of two; a NaN stays one
+__device__ __forceinline__ float at_least(float z, float low) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(low));
+    return r;
+}
+__device__ __forceinline__ float at_most(float z, float high) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(high));
+    return r;
+}
 template <bool kExact>
 __device__ __forceinline__ float sigmoid(float z) {
     // exp(-z) = inf for very negative z: the quotient is then 0, as it should be
@@ -253,7 +264,8 @@ __device__ __forceinline__ void pack_pairs(Vec<T, N> &v, const Pair (&p)[N / 2])
     v.pack(f);
 }
 // Two sigmoids with one reciprocal: 1/a = b/(ab), 1/b = a/(ab).  The exponentials are bounded by 2^60 so that the product is
-// finite (and a NaN stays in its half: z itself is multiplied in later); a sigmoid below 2^-60 comes out as 2^-60.  The
+// finite (and a NaN stays in its half: z itself is multiplied in later); a sigmoid below 2^-60 comes out as 2^-60, and what is
+// multiplied by it is bounded from below (low_bounded) so that the product stays at nothing for any z.  The
 // special-function unit, which gives four results a clock to a quarter of an SM, is what the activations wait for.
 __device__ __forceinline__ Pair sigmoid_fast2(Pair z) {
     const float2 t = split(mul2(z, pair(-1.44269504088896341f, -1.44269504088896341f)));
@@ -264,6 +276,10 @@ __device__ __forceinline__ Pair sigmoid_fast2(Pair z) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u.x * u.y));
     return mul2(pair(r, r), pair(u.y, u.x));
 }
+__device__ __forceinline__ Pair low_bounded(Pair z) {
+    const float2 f = split(z);
+    return pair(at_least(f.x, -64.0f), at_least(f.y, -64.0f));
+}
 __device__ __forceinline__ Pair gelu_tanh_argument(Pair z) {  // sqrt(8 / pi) (z + 0.044715 z^3), |z| bounded in the cube
     const float2 q = split(mul2(z, z));
     const Pair t = pair(fminf(q.x, 1e6f), fminf(q.y, 1e6f));
@@ -273,8 +289,8 @@ __device__ __forceinline__ Pair gelu_tanh_argument(Pair z) {  // sqrt(8 / pi) (z
 template <int kAct, bool kExact>
 __device__ __forceinline__ Pair act_value2(Pair z) {
     if (kAct == FC_ACT_NONE) return z;
-    if (kAct == FC_ACT_SILU && !kExact) return mul2(z, sigmoid_fast2(z));
-    if (kAct == FC_ACT_GELU_TANH && !kExact) return mul2(z, sigmoid_fast2(gelu_tanh_argument(z)));
+    if (kAct == FC_ACT_SILU && !kExact) return mul2(low_bounded(z), sigmoid_fast2(z));
+    if (kAct == FC_ACT_GELU_TANH && !kExact) return mul2(low_bounded(z), sigmoid_fast2(gelu_tanh_argument(z)));
     const float2 f = split(z);
     return pair(act_value<kAct, kExact>(f.x), act_value<kAct, kExact>(f.y));
 }
@@ -282,7 +298,7 @@ template <int kAct, bool kExact>
 __device__ __forceinline__ void act_both2(Pair z, Pair &a, Pair &d) {
     if (kAct == FC_ACT_SILU && !kExact) {
         const Pair s = sigmoid_fast2(z), one = pair(1.0f, 1.0f), minus = pair(-1.0f, -1.0f);
-        a = mul2(z, s);
+        a = mul2(low_bounded(z), s);
         d = fma2(a, fma2(s, minus, one), s);
         return;
     }

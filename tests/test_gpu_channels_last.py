@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import fastconv_b200 as fc
-from _last_ref import DTYPES, check, ff, norm, stored
+from _last_ref import DTYPES, act, check, ff, norm, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -582,6 +582,40 @@ def test_ff_of_very_large_and_very_small_fp32(lctx):
     done(lctx)
     want = ff({**{n: v.double().cpu() for n, v in t.items()}, "b_gate": None, "b_up": None, "b_down": None}, "silu", "fp32")
     check(y, *want["y"], "fp32", "y")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 200])
+@pytest.mark.parametrize("kind", ["silu", "gelu_tanh", "sigmoid"])
+def test_ff_activations_of_huge_arguments(lctx, rows, dtype, kind):
+    """Gates that are exact powers of two, up to 2^100 of either sign: act(z) goes to 0 or z, act'(z) to 0 or 1.
+
+    up and the down matrix are ones and the identity, so that y is act(z), rounded once, and the first column of the gate's
+    gradient is act'(z), rounded once.  Beside the half step: the exponential's argument, up to 87 in size where its result
+    is one that counts, is off by some four roundings, 2^-15 of the result at most; the types of 16 bits bound the sigmoid at
+    2^-60, 64 times of which is 5.6e-17.  act' has 1 - s, off by two steps of 1 where it is not 0, times up to 8 (|z|) in SiLU
+    and less in the others: 2^-19."""
+    dt = DTYPES[dtype]
+    z = [0.0] + [s * 2.0 ** e for s in (1, -1) for e in (-1, 1, 3, 5, 6, 9, 40, 66, 100)]
+    f = 64
+    z = (z * 4)[:f]
+    w_gate, w_up = torch.zeros(f, f), torch.zeros(f, f)
+    w_gate[:, 0], w_up[:, 0] = torch.tensor(z), 1.0
+    x, dy = torch.zeros(rows, f), torch.zeros(rows, f)
+    x[:, 0], dy[rows - 1] = 1.0, 1.0
+    x, dy, w_gate, w_up, w_down = (t.to(dt).cuda() for t in (x, dy, w_gate, w_up, torch.eye(f)))
+    y, dw, saved = torch.empty_like(x), torch.empty_like(w_gate), torch.empty(2, rows, f, device="cuda")
+    plan = fc.GatedFeedForward(rows, f, f, act=kind, dtype=dtype, train=True, ctx=lctx)
+    torch.cuda.synchronize()
+    ws = {"w_gate": at(w_gate), "w_up": at(w_up), "w_down": at(w_down)}
+    plan.forward(at(x), at(y), **ws, saved=at(saved))
+    plan.backward(at(dy), at(x), **ws, saved=at(saved), dw_gate=at(dw))
+    done(lctx)
+    v, d = act(torch.tensor(z, dtype=torch.float64), kind)
+    rel = torch.finfo(dt).eps / 2 + 2.0 ** -15
+    for got, want, tiny, what in ((y, v.expand(rows, f), 1e-35 if dtype == "fp32" else 1e-16, "y"), (dw[:, 0], d, 2.0 ** -19, "dw_gate")):
+        off = (got.double().cpu() - want).abs()
+        assert bool((off <= rel * want.abs() + tiny).all()), (what, off.max())
 
 
 def test_a_nan_stays_in_its_row(lctx):
