@@ -50,7 +50,7 @@ constexpr int CHUNK = 4;                  // k-blocks whose sum stays in tensor 
 // a time.
 template <int PLANES, int KIND>
 struct Ring {
-    static constexpr int kPieces = KIND == FF_GATE_BACK ? 4 : 2;
+    static constexpr int kPieces = KIND == FF_GATE_BACK || PLANES == 3 ? 4 : 2;
     static constexpr int kBytes =
         PLANES == 1 ? (KIND == FF_GATE_BACK ? 5 : 6) * 2 * HALF_BYTES : 2 * 3 * (HALF_BYTES + HALF_BYTES / 2);
     static constexpr int kOut = EPI_WARPS * kPieces * PIECE;
@@ -294,51 +294,101 @@ __device__ __forceinline__ void put_planes(Outlet<PIECES> &out, const CUtensorMa
     if constexpr (PLANES == 1) {
         out.template put<OT>(map, v, x, y, 0, lane);
     } else {
-        float part[32];
 #pragma unroll 1
-        for (int z = 0; z < 3; ++z) {
+        for (int z = 0; z < 3; ++z) {  // a loop, as the pieces are: a launch of one tile a CTA waits for the instructions themselves
+            uint32_t w[1][16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                part[j] = bf16_part(v[j]);  // the last part is what is left: 8 bits, kept as it is
-                v[j] = fabsf(part[j]) <= 3.4028234e38f ? v[j] - part[j] : 0.0f;
+            for (int j = 0; j < 16; ++j) {
+                const float p = bf16_part(v[2 * j]), q = bf16_part(v[2 * j + 1]);  // of the third part: all that is left
+                const float two[2] = {p, q};
+                Vec<OT, 2> pair16;
+                pair16.pack(two);
+                w[0][j] = *reinterpret_cast<const uint32_t *>(&pair16);
+                v[2 * j] = fabsf(p) <= 3.4028234e38f ? v[2 * j] - p : 0.0f;
+                v[2 * j + 1] = fabsf(q) <= 3.4028234e38f ? v[2 * j + 1] - q : 0.0f;
             }
-            out.template put<OT>(map, part, x, y, z, lane);
+            out.template put<1>(map, 0, w, x, y, z, 0, lane);
         }
     }
 }
 
-// fp32: a call for two values at a time (act, act' of both), and not 32 copies of the library's functions, whose 80 KB of
-// straight code a tile would wait for
-__device__ __noinline__ float4 exact_act(int act, float y, float z) {
+// fp32: GELU by the library's erfc, in a call for two values at a time (act, act' of both), because 32 copies of it are 50 KB of
+// straight code that a tile would wait for.
+__device__ __noinline__ float4 exact_gelu(float y, float z) {
     float4 r;
-    switch (act) {
-        case FC_ACT_GELU: act_both<FC_ACT_GELU, true>(y, r.x, r.y), act_both<FC_ACT_GELU, true>(z, r.z, r.w); break;
-        case FC_ACT_GELU_TANH: act_both<FC_ACT_GELU_TANH, true>(y, r.x, r.y), act_both<FC_ACT_GELU_TANH, true>(z, r.z, r.w); break;
-        case FC_ACT_SILU: act_both<FC_ACT_SILU, true>(y, r.x, r.y), act_both<FC_ACT_SILU, true>(z, r.z, r.w); break;
-        default: act_both_rt(act, y, r.x, r.y), act_both_rt(act, z, r.z, r.w);
-    }
+    act_both<FC_ACT_GELU, true>(y, r.x, r.y);
+    act_both<FC_ACT_GELU, true>(z, r.z, r.w);
     return r;
 }
-__device__ __forceinline__ void gate_values_exact(int act, float (&g)[32], const float (&u)[32]) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-        const float4 f = exact_act(act, g[j], g[j + 1]);
-        g[j] = f.x * u[j];
-        g[j + 1] = f.z * u[j + 1];
+// The other activations in line: exp(-z) = 2^t (1 + ln 2 * rest) with the rounding of t = -z log2(e) made good, and a
+// reciprocal with one Newton step; a few units in the 23rd bit.  z is bounded so that no step overflows: below -87 the result is
+// that of -87, 1.6e-38.
+__device__ __forceinline__ float fine_sigmoid(float z) {
+    z = at_most(at_least(z, -87.0f), 128.0f);
+    const float t = z * -1.44269504088896341f;
+    const float rest = fmaf(z, -1.44269504088896341f, -t) + z * -1.92596299e-8f;  // log2(e) = 1.44269502162933350 + 1.92596299e-8
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    const float x = 1.0f + fmaf(e, rest * 0.69314718055994531f, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return fmaf(r, fmaf(-x, r, 1.0f), r);
+}
+template <int ACT>
+__device__ __forceinline__ void fine_both(float z, float &a, float &d) {
+    if (ACT == FC_ACT_SILU) {
+        const float s = fine_sigmoid(z);
+        a = at_least(z, -87.0f) * s;
+        d = fmaf(a, 1.0f - s, s);
+    } else if (ACT == FC_ACT_GELU_TANH) {
+        z = at_least(z, -87.0f);
+        const float t = fminf(z * z, 1e6f);
+        const float s = fine_sigmoid(1.59576912160573071f * z * fmaf(0.044715f, t, 1.0f));
+        a = z * s;
+        d = fmaf(a * (1.0f - s), 1.59576912160573071f * fmaf(0.134145f, t, 1.0f), s);
+    } else if (ACT == FC_ACT_SIGMOID) {
+        a = fine_sigmoid(z);
+        d = a * (1.0f - a);
+    } else {
+        act_both<ACT, true>(z, a, d);  // none, ReLU
     }
 }
-__device__ __forceinline__ void gate_back_values_exact(int act, float (&g)[32], float (&u)[32], float (&dh)[32]) {
+// use(j, act(g[j]), act'(g[j])) for all 32
+template <typename F>
+__device__ __forceinline__ void exact_acts(int act, const float (&g)[32], F &&use) {
+    auto all = [&](auto kind) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-        const float4 f = exact_act(act, g[j], g[j + 1]);
-        const float h0 = f.x * u[j], h1 = f.z * u[j + 1];
-        g[j] = dh[j] * u[j] * f.y;
-        g[j + 1] = dh[j + 1] * u[j + 1] * f.w;
-        u[j] = dh[j] * f.x;
-        u[j + 1] = dh[j + 1] * f.z;
-        dh[j] = h0;
-        dh[j + 1] = h1;
+        for (int j = 0; j < 32; ++j) {
+            float a, d;
+            fine_both<decltype(kind)::value>(g[j], a, d);
+            use(j, a, d);
+        }
+    };
+    switch (act) {
+        case FC_ACT_GELU:
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                const float4 f = exact_gelu(g[j], g[j + 1]);
+                use(j, f.x, f.y);
+                use(j + 1, f.z, f.w);
+            }
+            break;
+        case FC_ACT_SILU: all(std::integral_constant<int, FC_ACT_SILU>()); break;
+        case FC_ACT_GELU_TANH: all(std::integral_constant<int, FC_ACT_GELU_TANH>()); break;
+        case FC_ACT_SIGMOID: all(std::integral_constant<int, FC_ACT_SIGMOID>()); break;
+        case FC_ACT_RELU: all(std::integral_constant<int, FC_ACT_RELU>()); break;
+        default: all(std::integral_constant<int, FC_ACT_NONE>());
     }
+}
+__device__ __forceinline__ void gate_values_exact(int act, float (&g)[32], const float (&u)[32]) {
+    exact_acts(act, g, [&](int j, float a, float) { g[j] = a * u[j]; });
+}
+__device__ __forceinline__ void gate_back_values_exact(int act, float (&g)[32], float (&u)[32], float (&dh)[32]) {
+    exact_acts(act, g, [&](int j, float a, float d) {
+        const float h = a * u[j];
+        g[j] = dh[j] * u[j] * d;
+        u[j] = dh[j] * a;
+        dh[j] = h;
+    });
 }
 
 template <int ACT>
@@ -700,8 +750,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                     emit(nt * cols + p0, v, u);
                 } else {
                     float w[32];
-                    emit(nt * cols + p0, v, w);
-                    emit(nt * cols + p1, u, w);
+#pragma unroll 1
+                    for (int i = 0; i < 2; ++i) {
+                        emit(nt * cols + (i ? p1 : p0), v, w);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = u[j];
+                    }
                 }
             }
         }
