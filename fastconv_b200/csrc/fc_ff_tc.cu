@@ -17,7 +17,7 @@
 // values the six largest are taken, hh, hm, mh, hl, lh, mm; the others are below 2^-25 of the result.  The tensor cores' fp32
 // additions round toward zero, which over a long reduction adds up to a bias of some 2e-8 an instruction: the five small
 // products, where that does not matter, have an accumulator of their own, and the sum of hh is taken over into registers,
-// rounded to nearest, every 256 steps.  Six times the work of a bf16 product; 95 TFLOP/s at 3137 rows 256->1024->256, where
+// rounded to nearest, every 256 steps.  Six times the work of a bf16 product; 98 TFLOP/s at 3137 rows 256->1024->256, where
 // products on the FP32 pipe gave 29.
 //
 // What bounds them, measured on one B200 in bf16: a plain product of 210 GFLOP takes 126 to 144 us by the clock that the power
