@@ -1029,7 +1029,8 @@ int with_vectors(const NormShape &s, int type, std::initializer_list<const void 
     });
 }
 
-int check_maps(const fc_group_norm_desc *d, std::initializer_list<const void *> maps, std::initializer_list<const void *> params) {
+int check_maps(const fc_group_norm_desc *d, std::initializer_list<const void *> maps, std::initializer_list<const void *> params,
+               const float *mean, const float *rstd) {
     for (const void *p : maps) {
         FC_REQUIRE(p != nullptr, FC_ERR_INVALID_ARG, "NULL map");
         FC_REQUIRE((uintptr_t)p % dtype_size(d->type) == 0, FC_ERR_INVALID_ARG, "a map's address is no multiple of its element size");
@@ -1037,6 +1038,7 @@ int check_maps(const fc_group_norm_desc *d, std::initializer_list<const void *> 
     for (const void *p : params)
         FC_REQUIRE((uintptr_t)p % dtype_size(d->param_type) == 0, FC_ERR_INVALID_ARG,
                    "a parameter's address is no multiple of its element size");
+    FC_REQUIRE((uintptr_t)mean % 4 == 0 && (uintptr_t)rstd % 4 == 0, FC_ERR_INVALID_ARG, "an address of mean or rstd is no multiple of 4");
     return FC_OK;
 }
 
@@ -1071,7 +1073,7 @@ int fc_group_norm_forward(fc_context *ctx, const fc_group_norm_desc *desc, const
     NormShape s;
     FC_PROPAGATE(norm_shape(desc, &s));
     if (s.batch == 0) return FC_OK;
-    FC_PROPAGATE(check_maps(desc, {d_x, d_y}, {d_gamma, d_beta}));
+    FC_PROPAGATE(check_maps(desc, {d_x, d_y}, {d_gamma, d_beta}, d_mean, d_rstd));
     FC_REQUIRE(d_y != d_x, FC_ERR_INVALID_ARG, "the output is the input");
     size_t need;
     FC_PROPAGATE(fc_group_norm_workspace(desc, &need, nullptr));
@@ -1118,7 +1120,8 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
     FC_REQUIRE(ctx != nullptr, FC_ERR_INVALID_ARG, "context is NULL");
     NormShape s;
     FC_PROPAGATE(norm_shape(desc, &s));
-    if (s.batch > 0) FC_PROPAGATE(check_maps(desc, {d_dy, d_x, d_dx ? d_dx : d_x}, {d_gamma, d_beta, d_dgamma, d_dbeta}));
+    if (s.batch > 0) FC_PROPAGATE(check_maps(desc, {d_dy, d_x, d_dx ? d_dx : d_x}, {}, nullptr, nullptr));
+    FC_PROPAGATE(check_maps(desc, {}, {d_gamma, d_beta, d_dgamma, d_dbeta}, d_mean, d_rstd));  // of no images they are written too
     FC_REQUIRE(d_dx == nullptr || (d_dx != d_x && d_dx != d_dy), FC_ERR_INVALID_ARG, "an output is an input");
     FC_REQUIRE(s.batch == 0 || (d_mean != nullptr && d_rstd != nullptr), FC_ERR_INVALID_ARG,
                "the gradient needs the forward pass's mean and rstd");

@@ -76,3 +76,23 @@ def test_sizes_past_32_bits_are_counted():
     lib = fc.load()
     assert lib.fc_gated_ff_workspace(C.byref(ffd(rows=1 << 21, hidden=1 << 13, type=1)), C.byref(f), C.byref(b)) == 0
     assert f.value >= (1 << 35) and b.value >= 3 << 35
+
+
+@pytest.mark.parametrize("batch", [0, 2])
+def test_addresses_that_are_no_multiple_of_the_element_are_refused(batch):
+    """Before the context is looked at (here bytes of zero): parameters' gradients of no images are written too."""
+    lib, ctx = fc.load(), C.create_string_buffer(1 << 16)
+    d, p, n = C.byref(gn(batch=batch)), 4096, 1 << 40
+    ops = [p, p, p, p, p, p, 2 * p, p, p, p, n]  # dy, x, gamma, beta, mean, rstd, dx, dgamma, dbeta, workspace, bytes
+    for i in (2, 3, 4, 5, 7, 8):
+        assert lib.fc_group_norm_backward(ctx, d, *[v + 2 if j == i else v for j, v in enumerate(ops)]) == INVALID, i
+        assert b"multiple" in lib.fc_last_error(), i
+    ops = [p, p, p, 2 * p, p, p, p, n]  # x, gamma, beta, y, mean, rstd, workspace, bytes
+    for i in (1, 2, 4, 5) if batch else ():
+        assert lib.fc_group_norm_forward(ctx, d, *[v + 2 if j == i else v for j, v in enumerate(ops)]) == INVALID, i
+        assert b"multiple" in lib.fc_last_error(), i
+    ops = [p, p, p, p, p, p, 2 * p, p, p, p, p, p, p, p, n]  # dy, x, three weights, saved, dx, six gradients, workspace, bytes
+    d = C.byref(ffd(rows=2 * batch))
+    for i in (5, 7, 8, 9, 10, 11, 12):
+        assert lib.fc_gated_ff_backward(ctx, d, *[v + 2 if j == i else v for j, v in enumerate(ops)]) == INVALID, i
+        assert b"multiple" in lib.fc_last_error(), i
