@@ -17,7 +17,7 @@
 // values the six largest are taken, hh, hm, mh, hl, lh, mm; the others are below 2^-25 of the result.  The tensor cores' fp32
 // additions round toward zero, which over a long reduction adds up to a bias of some 2e-8 an instruction: the five small
 // products, where that does not matter, have an accumulator of their own, and the sum of hh is taken over into registers,
-// rounded to nearest, every 256 steps.  Six times the work of a bf16 product; 98 TFLOP/s at 3137 rows 256->1024->256, where
+// rounded to nearest, every 256 steps.  Six times the work of a bf16 product; 107 TFLOP/s at 3137 rows 256->1024->256, where
 // products on the FP32 pipe gave 29.
 //
 // What bounds them, measured on one B200 in bf16: a plain product of 210 GFLOP takes 126 to 144 us by the clock that the power
@@ -294,18 +294,28 @@ __device__ __forceinline__ void put_planes(Outlet<PIECES> &out, const CUtensorMa
     if constexpr (PLANES == 1) {
         out.template put<OT>(map, v, x, y, 0, lane);
     } else {
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[j]));
+        const bool huge = most > 3.38e38f;  // where rounding to bf16 could give infinity, or it is there already
 #pragma unroll 1
         for (int z = 0; z < 3; ++z) {  // a loop, as the pieces are: a launch of one tile a CTA waits for the instructions themselves
             uint32_t w[1][16];
+            if (!huge) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float p = bf16_part(v[2 * j]), q = bf16_part(v[2 * j + 1]);  // of the third part: all that is left
-                const float two[2] = {p, q};
-                Vec<OT, 2> pair16;
-                pair16.pack(two);
-                w[0][j] = *reinterpret_cast<const uint32_t *>(&pair16);
-                v[2 * j] = fabsf(p) <= 3.4028234e38f ? v[2 * j] - p : 0.0f;
-                v[2 * j + 1] = fabsf(q) <= 3.4028234e38f ? v[2 * j + 1] - q : 0.0f;
+                for (int j = 0; j < 16; ++j) {  // of the third part: all that is left
+                    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[0][j]) : "f"(v[2 * j + 1]), "f"(v[2 * j]));
+                    v[2 * j] -= __uint_as_float(w[0][j] << 16);
+                    v[2 * j + 1] -= __uint_as_float(w[0][j] & 0xffff0000u);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float p = bf16_part(v[2 * j]), q = bf16_part(v[2 * j + 1]);
+                    w[0][j] = __float_as_uint(p) >> 16 | (__float_as_uint(q) & 0xffff0000u);
+                    v[2 * j] = fabsf(p) <= 3.4028234e38f ? v[2 * j] - p : 0.0f;
+                    v[2 * j + 1] = fabsf(q) <= 3.4028234e38f ? v[2 * j + 1] - q : 0.0f;
+                }
             }
             out.template put<1>(map, 0, w, x, y, z, 0, lane);
         }
