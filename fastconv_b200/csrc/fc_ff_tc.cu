@@ -102,7 +102,8 @@ __device__ __forceinline__ uint32_t first_cta(uint32_t addr) {  // the same plac
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
-// both CTAs are done with each other's barriers; nothing in memory is handed over
+// Nothing in memory is handed over, and no arrival at a barrier is ordered by it: each CTA has waited for those that the other
+// sends to its own barriers before it comes here (the producer for the ring's, the matrix warp for the accumulators').
 __device__ __forceinline__ void cluster_leave() {
     asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
 }
@@ -561,7 +562,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                 decode(item, mt, nt, share);
                 const int lo = share * P.kb_share, hi = min(P.kb_total, lo + P.kb_share);
                 const uint32_t small = tmem + (2 + (t & 1)) * P.bn;
-                if (PLANES == 3 && !mbar_wait(bar_small_empty(t & 1), ((t >> 1) & 1) ^ 1, abort_flag, P.status)) break;
+                if (PLANES == 3) ok = mbar_wait(bar_small_empty(t & 1), ((t >> 1) & 1) ^ 1, abort_flag, P.status);
                 for (int k_lo = lo; k_lo < hi && ok; k_lo += PLANES == 3 ? CHUNK : hi - lo, ++c) {
                     const int k_hi = PLANES == 3 ? min(hi, k_lo + CHUNK) : hi, acc = c & 1;
                     if (!mbar_wait(bar_acc_empty(acc), ((c >> 1) & 1) ^ 1, abort_flag, P.status)) {
@@ -602,6 +603,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FF_TC_THREADS, 1)
                         if (++s == S) s = 0, phase ^= 1;
                     }
                 }
+            }
+            // The last releases of both accumulators have arrived here, the other CTA's too, before this one may end: the waits
+            // that a further use of each would begin with.
+            for (int i = 0; i < 2 && ok; ++i, ++c, ++t) {
+                ok = mbar_wait(bar_acc_empty(c & 1), ((c >> 1) & 1) ^ 1, abort_flag, P.status);
+                if (PLANES == 3 && ok) ok = mbar_wait(bar_small_empty(t & 1), ((t >> 1) & 1) ^ 1, abort_flag, P.status);
             }
         }
     } else {
