@@ -490,6 +490,7 @@ __global__ void __launch_bounds__(256) igemm_tiny_unfused_kernel(const float *__
                                                                  float *__restrict__ out, IgemmParams P, Epilogue ep) {
     const int ohw = P.oh * P.ow;
     const int idx = blockIdx.x * blockDim.x + threadIdx.x;
+    pdl_wait();  // in every thread, before the first may leave: the input may be what the previous kernel writes
     if (idx >= P.n * P.oc * ohw) return;
     const int rem = idx % ohw, r = idx / ohw, k = r % P.oc, img = r / P.oc;
     const int oi = rem / P.ow, oj = rem - oi * P.ow;

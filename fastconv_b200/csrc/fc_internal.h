@@ -140,8 +140,11 @@ struct fc_context {
 // constant weights) comes before the wait.  pdl_wait() is a no-op for a plain launch.
 #ifdef __CUDACC__
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// None of the kernels signals early: pdl_trigger() marks where the signal used to be and does nothing, so a dependent
-// grid comes in when the blocks of its predecessor exit.  Measured on the VGG-16 stack
+// No kernel may leave the wait out, however little it does: kernels of the channels-last operators signal early
+// (last::pdl_next), what follows them then starts while they still write, and a grid that ends without having waited
+// ends before its predecessor does, which the next one's wait does not see.
+// None of the convolution layers' kernels signals early: pdl_trigger() marks where the signal used to be and does
+// nothing, so a dependent grid comes in when the blocks of its predecessor exit.  Measured on the VGG-16 stack
 // (CUDA graph, fp32): with griddepcontrol.launch_dependents at the top of every kernel 11.15 ms at 64 images, 1.684 at 8,
 // 0.400 at one; with the signal moved to where a block has only its stores left 10.96 / 1.638 / 0.392; without any signal
 // 10.92 / 1.631 / 0.382; without the attribute 10.92 / 1.632 / 0.384.  A dependent's blocks that come in early hold
