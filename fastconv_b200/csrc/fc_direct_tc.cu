@@ -458,14 +458,14 @@ int launch_direct_tc(fc_context *ctx, const float *d_in, float *d_nhwc, const fl
     if (folds_taps(full)) {
         const size_t smem = (size_t)full.ic * full.kh * (ow + full.kw - 1) * sizeof(float);
         FC_CHECK_CUDA(cudaFuncSetAttribute(fold_taps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        FC_CHECK_CUDA(launch_pdl(fold_taps_kernel, dim3((unsigned)(full.batch * oh)), dim3(256), smem, ctx->stream, d_in,
+        FC_CHECK_CUDA(launch_pdl(fold_taps_kernel, dim3((unsigned)(full.batch * oh)), dim3(256), smem, ctx, d_in,
                                  d_nhwc, full.ic, full.ih, full.iw, full.kh, full.kw, full.pad_top, full.pad_left, oh, ow));
         d = kernel_view(full, oh, ow);  // from here on: a 1x1, unpadded layer over the 32 folded channels
     }
     const int icp = round_up(d.ic, BK), hw = d.ih * d.iw;
     if (!folds_taps(full)) {
         dim3 grid((unsigned)ceil_div(hw, 32), (unsigned)(icp / 32), (unsigned)d.batch), block(256);
-        FC_CHECK_CUDA(launch_pdl(nchw_to_nhwc_kernel, grid, block, 0, ctx->stream, d_in, d_nhwc, d.ic, icp, hw));
+        FC_CHECK_CUDA(launch_pdl(nchw_to_nhwc_kernel, grid, block, 0, ctx, d_in, d_nhwc, d.ic, icp, hw));
     }
     const DirectPlan plan = make_plan(d, oh, ow, ctx->sm_count, cfg);
     const int bh = plan.bh, bw = plan.bw;
@@ -510,11 +510,11 @@ int launch_direct_tc(fc_context *ctx, const float *d_in, float *d_nhwc, const fl
     FC_PROPAGATE(make_map_nhwc(&tmX, d_nhwc, icp, d.iw, d.ih, d.batch, bw, bh, d.sw, d.sh));
     FC_PROPAGATE(make_map_3d(&tmW, d_wp, icp, d.oc, P.taps, P.bn));
     FC_CHECK_CUDA(cudaFuncSetAttribute(direct_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    FC_CHECK_CUDA(launch_pdl(direct_tc_kernel, dim3((unsigned)ctas), dim3(TC_THREADS), smem, ctx->stream, tmX, tmW, P));
+    FC_CHECK_CUDA(launch_pdl(direct_tc_kernel, dim3((unsigned)ctas), dim3(TC_THREADS), smem, ctx, tmX, tmW, P));
     if (late_epilogue) {
         const size_t total = (size_t)d.batch * d.oc * oh * ow;
         const unsigned nb = (unsigned)(ceil_div(total, 256) > (size_t)ctx->sm_count * 8 ? (size_t)ctx->sm_count * 8 : ceil_div(total, 256));
-        FC_CHECK_CUDA(launch_pdl(bias_relu_kernel, dim3(nb), dim3(256), 0, ctx->stream, d_out, ep, d.oc, oh * ow, total));
+        FC_CHECK_CUDA(launch_pdl(bias_relu_kernel, dim3(nb), dim3(256), 0, ctx, d_out, ep, d.oc, oh * ow, total));
     }
     return FC_OK;
 }

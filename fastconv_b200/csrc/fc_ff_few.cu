@@ -124,7 +124,7 @@ int launch_ff_few(fc_context *ctx, const FfProduct &p) {
     return with_type(p.type, [&](auto t) -> int {
         using T = decltype(t);
         auto go = [&](auto kernel) -> int {
-            FC_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)blocks), dim3(FEW_THREADS), 0, ctx->stream, p, log_shares));
+            FC_CHECK_CUDA(launch_early(kernel, dim3((unsigned)blocks), dim3(FEW_THREADS), 0, ctx, p, log_shares));
             return FC_OK;
         };
         if (p.kind == FF_GATE)

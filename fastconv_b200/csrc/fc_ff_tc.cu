@@ -264,7 +264,7 @@ __device__ __forceinline__ void saved_row(const FfTc &P, float *base, int y, int
             if (STORE) {
                 p[at] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             } else {
-                const float4 f = __ldg(p + at);
+                const float4 f = p[at];
                 v[4 * j] = f.x, v[4 * j + 1] = f.y, v[4 * j + 2] = f.z, v[4 * j + 3] = f.w;
             }
         };
@@ -284,7 +284,7 @@ __device__ __forceinline__ void saved_row(const FfTc &P, float *base, int y, int
             if (STORE)
                 *p = v[j];
             else
-                v[j] = __ldg(p);
+                v[j] = *p;
         }
     }
 }
@@ -811,7 +811,7 @@ __global__ void __launch_bounds__(256) ff_tc_join_kernel(const FfTc P, T *c0, T 
         if (q >= quads || row >= P.m || c == nullptr) continue;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int s = 0; s < P.splits; ++s) {
-            const float4 f = __ldg((const float4 *)P.part + (((size_t)s * P.m_tiles * 8 + block) * quads + q) * 32 + r);
+            const float4 f = ((const float4 *)P.part)[(((size_t)s * P.m_tiles * 8 + block) * quads + q) * 32 + r];
             v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
         }
         if (P.bias0)
@@ -981,7 +981,7 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
             const int room = R::kBytes / (P.kbs * ff_kb_bytes(PLANES, P.bn));
             P.stages = room < R::kMost ? room : R::kMost;
             FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-            FC_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)(2 * pairs)), dim3(FF_TC_THREADS), SMEM, ctx->stream, maps, P));
+            FC_CHECK_CUDA(launch_early(kernel, dim3((unsigned)(2 * pairs)), dim3(FF_TC_THREADS), SMEM, ctx, maps, P));
             return FC_OK;
         };
         if (p.kind == FF_GATE) return go(ff_tc_kernel<OT, T, PLANES, true, true, FF_GATE>, Ring<PLANES, FF_GATE>());
@@ -993,7 +993,7 @@ int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
         if (P.splits > 1) {
             long long blocks = ceil_div((size_t)P.m_tiles * 8 * 4 * ceil_div(p.n, 16), 8);
             if (blocks > 148 * 8) blocks = 148 * 8;
-            FC_CHECK_CUDA(launch_pdl(ff_tc_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, P, (T *)p.c0, (T *)p.c1,
+            FC_CHECK_CUDA(launch_early(ff_tc_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, ctx, P, (T *)p.c0, (T *)p.c1,
                                      (int)c_wide));
         }
         return FC_OK;

@@ -176,9 +176,9 @@ struct Sums {
         list.chunks = (int)ceil_div(rows, list.chunk_rows);
         return with_type(type, [&](auto t) -> int {
             using T = decltype(t);
-            FC_CHECK_CUDA(launch_pdl(ff_colsum_kernel<T>, dim3(list.blocks, list.chunks), dim3(SUM_COLS * SUM_ROWS), 0, ctx->stream, list));
+            FC_CHECK_CUDA(launch_early(ff_colsum_kernel<T>, dim3(list.blocks, list.chunks), dim3(SUM_COLS * SUM_ROWS), 0, ctx, list));
             if (list.chunks > 1)
-                FC_CHECK_CUDA(launch_pdl(ff_colsum_join_kernel<T>, dim3(list.blocks), dim3(SUM_COLS), 0, ctx->stream, list));
+                FC_CHECK_CUDA(launch_early(ff_colsum_join_kernel<T>, dim3(list.blocks), dim3(SUM_COLS), 0, ctx, list));
             return FC_OK;
         });
     }
@@ -314,7 +314,7 @@ struct Packer {
         return with_type(b.type, [&](auto t) -> int {
             long long blocks = ceil_div((size_t)total, 256);
             if (blocks > 148 * 16) blocks = 148 * 16;
-            FC_CHECK_CUDA(launch_pdl(ff_pack_kernel<decltype(t)>, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, list));
+            FC_CHECK_CUDA(launch_early(ff_pack_kernel<decltype(t)>, dim3((unsigned)blocks), dim3(256), 0, ctx, list));
             return FC_OK;
         });
     }

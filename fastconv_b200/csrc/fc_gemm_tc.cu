@@ -527,7 +527,7 @@ int launch_wino_gemm_tc(fc_context *ctx, const float *d_U, const float *d_V, flo
     dim3 grid((unsigned)ctas), block(split || u16 ? TC_SPLIT_THREADS : TC_THREADS);
     auto launch = [&](auto kernel) -> int {
         FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        FC_CHECK_CUDA(launch_pdl(kernel, grid, block, smem, ctx->stream, tmU, tmV, P));
+        FC_CHECK_CUDA(launch_pdl(kernel, grid, block, smem, ctx, tmU, tmV, P));
         return FC_OK;
     };
     if (u16) FC_PROPAGATE(launch(wino_gemm_tc_kernel<2, false>));

@@ -41,7 +41,7 @@ struct NormShape {
 template <typename T>
 __device__ __forceinline__ float param(const void *p, int c, int f32, float absent) {
     if (p == nullptr) return absent;
-    return f32 ? __ldg((const float *)p + c) : Elem<T>::load(((const T *)p)[c]);
+    return f32 ? ((const float *)p)[c] : Elem<T>::load(((const T *)p)[c]);
 }
 
 // the values of VEC channels from c on; c is a multiple of VEC
@@ -121,7 +121,7 @@ __device__ __forceinline__ float block_sum(float v, float *scratch) {
 
 // part[(img * chunks + chunk) * channels + c] = (mean, M2) of the channel over the chunk
 template <typename T, int VEC>
-__global__ void __launch_bounds__(NORM_THREADS) norm_part_kernel(const T *__restrict__ x, float2 *__restrict__ part,
+__global__ void __launch_bounds__(NORM_THREADS) norm_part_kernel(const T *x, float2 *__restrict__ part,
                                                                 const NormShape s) {
     __shared__ float2 stat[NORM_THREADS * VEC];
     pdl_wait();
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_part_kernel(const T *__rest
 }
 
 // mean and rstd of one group of one image from the chunks' sums
-__global__ void __launch_bounds__(NORM_THREADS) norm_join_kernel(const float2 *__restrict__ part, float *__restrict__ mean,
+__global__ void __launch_bounds__(NORM_THREADS) norm_join_kernel(const float2 *part, float *__restrict__ mean,
                                                                 float *__restrict__ rstd, const NormShape s) {
     __shared__ float scratch[NORM_THREADS / 32];
     pdl_wait();
@@ -197,9 +197,9 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_join_kernel(const float2 *_
 }
 
 template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(NORM_THREADS) norm_apply_kernel(const T *__restrict__ x, const void *__restrict__ gamma,
-                                                                 const void *__restrict__ beta, const float *__restrict__ mean,
-                                                                 const float *__restrict__ rstd, T *__restrict__ y,
+__global__ void __launch_bounds__(NORM_THREADS) norm_apply_kernel(const T *x, const void *gamma,
+                                                                 const void *beta, const float *mean,
+                                                                 const float *rstd, T *__restrict__ y,
                                                                  const NormShape s) {
     constexpr bool kExact = std::is_same<T, float>::value;
     pdl_wait();
@@ -263,11 +263,11 @@ struct BackChannels {
 
 // part[(img * chunks + chunk) * channels + c] = (sum dz, sum dz xhat) of the channel over the chunk
 template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(NORM_THREADS) norm_back_part_kernel(const T *__restrict__ dy, const T *__restrict__ x,
-                                                                     const void *__restrict__ gamma,
-                                                                     const void *__restrict__ beta,
-                                                                     const float *__restrict__ mean,
-                                                                     const float *__restrict__ rstd, float2 *__restrict__ part,
+__global__ void __launch_bounds__(NORM_THREADS) norm_back_part_kernel(const T *dy, const T *x,
+                                                                     const void *gamma,
+                                                                     const void *beta,
+                                                                     const float *mean,
+                                                                     const float *rstd, float2 *__restrict__ part,
                                                                      const NormShape s) {
     __shared__ float2 stat[NORM_THREADS * VEC];
     pdl_wait();
@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_part_kernel(const T *_
 
 // sums[img * channels + c] = the channel's (sum dz, sum dz xhat); ab[img * groups + g] = (A, B)
 template <typename T>
-__global__ void __launch_bounds__(NORM_THREADS) norm_back_join_kernel(const float2 *__restrict__ part,
-                                                                     const void *__restrict__ gamma, float2 *__restrict__ sums,
+__global__ void __launch_bounds__(NORM_THREADS) norm_back_join_kernel(const float2 *part,
+                                                                     const void *gamma, float2 *__restrict__ sums,
                                                                      float2 *__restrict__ ab, const NormShape s) {
     __shared__ float scratch[NORM_THREADS / 32];
     pdl_wait();
@@ -338,12 +338,12 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_join_kernel(const floa
 }
 
 template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(NORM_THREADS) norm_back_apply_kernel(const T *__restrict__ dy, const T *__restrict__ x,
-                                                                      const void *__restrict__ gamma,
-                                                                      const void *__restrict__ beta,
-                                                                      const float *__restrict__ mean,
-                                                                      const float *__restrict__ rstd,
-                                                                      const float2 *__restrict__ ab, T *__restrict__ dx,
+__global__ void __launch_bounds__(NORM_THREADS) norm_back_apply_kernel(const T *dy, const T *x,
+                                                                      const void *gamma,
+                                                                      const void *beta,
+                                                                      const float *mean,
+                                                                      const float *rstd,
+                                                                      const float2 *ab, T *__restrict__ dx,
                                                                       const NormShape s) {
     pdl_wait();
     pdl_next();
@@ -529,8 +529,8 @@ struct GroupSums {
 // deviations from the mean, they are taken once more around the mean, so the variance never loses more than some four of
 // its 24 bits, however far the map is from zero.  The blocks of a cluster are joined by the means' distances.
 template <typename T, int ACT, bool UNI>
-__global__ void __launch_bounds__(FUSED_THREADS, UNI ? 4 : 2) norm_fused_kernel(const T *__restrict__ x, const void *__restrict__ gamma,
-                                                                  const void *__restrict__ beta, T *__restrict__ y,
+__global__ void __launch_bounds__(FUSED_THREADS, UNI ? 4 : 2) norm_fused_kernel(const T *x, const void *gamma,
+                                                                  const void *beta, T *__restrict__ y,
                                                                   float *__restrict__ mean, float *__restrict__ rstd,
                                                                   const NormShape s, const Fused f) {
     constexpr int VEC = 16 / sizeof(T);
@@ -689,11 +689,11 @@ __global__ void __launch_bounds__(FUSED_THREADS, UNI ? 4 : 2) norm_fused_kernel(
 
 // sums[img * channels + c]: the image's (sum dz, sum dz xhat)
 template <typename T, int ACT, bool UNI>
-__global__ void __launch_bounds__(FUSED_THREADS, UNI ? 4 : 2) norm_back_fused_kernel(const T *__restrict__ dy, const T *__restrict__ x,
-                                                                       const void *__restrict__ gamma,
-                                                                       const void *__restrict__ beta,
-                                                                       const float *__restrict__ mean,
-                                                                       const float *__restrict__ rstd, T *__restrict__ dx,
+__global__ void __launch_bounds__(FUSED_THREADS, UNI ? 4 : 2) norm_back_fused_kernel(const T *dy, const T *x,
+                                                                       const void *gamma,
+                                                                       const void *beta,
+                                                                       const float *mean,
+                                                                       const float *rstd, T *__restrict__ dx,
                                                                        float2 *__restrict__ sums, const NormShape s, const Fused f) {
     constexpr int VEC = 16 / sizeof(T);
     using V = Vec<T, VEC>;
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(FUSED_THREADS, UNI ? 4 : 2) norm_back_fused_ke
 
 // dgamma[c], dbeta[c]: the images' sums.  32 channels x 8 shares of the images to a block; the shares are added in order.
 template <typename T>
-__global__ void __launch_bounds__(NORM_THREADS) norm_back_params_kernel(const float2 *__restrict__ sums, void *dgamma, void *dbeta,
+__global__ void __launch_bounds__(NORM_THREADS) norm_back_params_kernel(const float2 *sums, void *dgamma, void *dbeta,
                                                                        const NormShape s) {
     __shared__ float2 shares[8][32];
     pdl_wait();
@@ -1092,7 +1092,7 @@ int fc_group_norm_forward(fc_context *ctx, const fc_group_norm_desc *desc, const
                     auto kernel = f.width > 1 ? norm_fused_kernel<T, A, true> : norm_fused_kernel<T, A, false>;
                     FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
                     FC_CHECK_CUDA(launch_clusters(kernel, dim3(f.blocks * f.cluster, s.batch), FUSED_THREADS, f.cluster, f.smem,
-                                                  ctx->stream, (const T *)d_x, d_gamma, d_beta, (T *)d_y, d_mean, d_rstd, s, f));
+                                                  ctx, (const T *)d_x, d_gamma, d_beta, (T *)d_y, d_mean, d_rstd, s, f));
                     return FC_OK;
                 });
         }
@@ -1101,13 +1101,13 @@ int fc_group_norm_forward(fc_context *ctx, const fc_group_norm_desc *desc, const
         FC_REQUIRE(blocks < (1ll << 31), FC_ERR_UNSUPPORTED, "%lld blocks", blocks);
         const NormWork w = norm_carve(s, d_workspace, false);
         float *mean = d_mean ? d_mean : w.mean, *rstd = d_rstd ? d_rstd : w.rstd;
-        FC_CHECK_CUDA(launch_pdl(norm_part_kernel<T, VEC>, dim3((unsigned)blocks), dim3(NORM_THREADS), 0, ctx->stream, (const T *)d_x,
+        FC_CHECK_CUDA(launch_early(norm_part_kernel<T, VEC>, dim3((unsigned)blocks), dim3(NORM_THREADS), 0, ctx, (const T *)d_x,
                                  w.part, s));
-        FC_CHECK_CUDA(launch_pdl(norm_join_kernel, dim3(s.batch * s.groups), dim3(NORM_THREADS), 0, ctx->stream,
+        FC_CHECK_CUDA(launch_early(norm_join_kernel, dim3(s.batch * s.groups), dim3(NORM_THREADS), 0, ctx,
                                  (const float2 *)w.part, mean, rstd, s));
         return with_act(desc->act, [&](auto a) -> int {
-            FC_CHECK_CUDA(launch_pdl(norm_apply_kernel<T, VEC, decltype(a)::value>, dim3((unsigned)blocks), dim3(NORM_THREADS), 0,
-                                     ctx->stream, (const T *)d_x, d_gamma, d_beta, (const float *)mean, (const float *)rstd,
+            FC_CHECK_CUDA(launch_early(norm_apply_kernel<T, VEC, decltype(a)::value>, dim3((unsigned)blocks), dim3(NORM_THREADS), 0,
+                                     ctx, (const T *)d_x, d_gamma, d_beta, (const float *)mean, (const float *)rstd,
                                      (T *)d_y, s));
             return FC_OK;
         });
@@ -1148,30 +1148,30 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
                     auto kernel = f.width > 1 ? norm_back_fused_kernel<T, A, true> : norm_back_fused_kernel<T, A, false>;
                     FC_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
                     FC_CHECK_CUDA(launch_clusters(kernel, dim3(f.blocks * f.cluster, s.batch), FUSED_THREADS, f.cluster, f.smem,
-                                                  ctx->stream, (const T *)d_dy, (const T *)d_x, d_gamma, d_beta, d_mean, d_rstd,
+                                                  ctx, (const T *)d_dy, (const T *)d_x, d_gamma, d_beta, d_mean, d_rstd,
                                                   (T *)d_dx, w.sums, s, f));
                     return FC_OK;
                 }));
         } else if (s.batch > 0) {
             FC_PROPAGATE(with_act(desc->act, [&](auto a) -> int {
-                FC_CHECK_CUDA(launch_pdl(norm_back_part_kernel<T, VEC, decltype(a)::value>, dim3((unsigned)blocks),
-                                         dim3(NORM_THREADS), 0, ctx->stream, (const T *)d_dy, (const T *)d_x, d_gamma, d_beta,
+                FC_CHECK_CUDA(launch_early(norm_back_part_kernel<T, VEC, decltype(a)::value>, dim3((unsigned)blocks),
+                                         dim3(NORM_THREADS), 0, ctx, (const T *)d_dy, (const T *)d_x, d_gamma, d_beta,
                                          d_mean, d_rstd, w.part, s));
                 return FC_OK;
             }));
-            FC_CHECK_CUDA(launch_pdl(norm_back_join_kernel<T>, dim3(s.batch * s.groups), dim3(NORM_THREADS), 0, ctx->stream,
+            FC_CHECK_CUDA(launch_early(norm_back_join_kernel<T>, dim3(s.batch * s.groups), dim3(NORM_THREADS), 0, ctx,
                                      (const float2 *)w.part, d_gamma, w.sums, w.ab, s));
             if (d_dx != nullptr)
                 FC_PROPAGATE(with_act(desc->act, [&](auto a) -> int {
-                    FC_CHECK_CUDA(launch_pdl(norm_back_apply_kernel<T, VEC, decltype(a)::value>, dim3((unsigned)blocks),
-                                             dim3(NORM_THREADS), 0, ctx->stream, (const T *)d_dy, (const T *)d_x, d_gamma, d_beta,
+                    FC_CHECK_CUDA(launch_early(norm_back_apply_kernel<T, VEC, decltype(a)::value>, dim3((unsigned)blocks),
+                                             dim3(NORM_THREADS), 0, ctx, (const T *)d_dy, (const T *)d_x, d_gamma, d_beta,
                                              d_mean, d_rstd, (const float2 *)w.ab, (T *)d_dx, s));
                     return FC_OK;
                 }));
         }
         if (d_dgamma != nullptr || d_dbeta != nullptr)
-            FC_CHECK_CUDA(launch_pdl(norm_back_params_kernel<T>, dim3((s.channels + 31) / 32),
-                                     dim3(NORM_THREADS), 0, ctx->stream, (const float2 *)w.sums, d_dgamma, d_dbeta, s));
+            FC_CHECK_CUDA(launch_early(norm_back_params_kernel<T>, dim3((s.channels + 31) / 32),
+                                     dim3(NORM_THREADS), 0, ctx, (const float2 *)w.sums, d_dgamma, d_dbeta, s));
         return FC_OK;
     });
 }

@@ -580,7 +580,7 @@ int launch_igemm_ffma(fc_context *ctx, const float *d_in, const float *d_kernel,
     const int sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
     if (igemm_is_tiny(d, oh, ow)) {  // the one shape class whose reference arithmetic is not a fused multiply-add
         const int total = d.batch * d.oc * oh * ow;
-        FC_CHECK_CUDA(launch_pdl(igemm_tiny_unfused_kernel, dim3((unsigned)ceil_div(total, 256)), dim3(256), 0, ctx->stream,
+        FC_CHECK_CUDA(launch_pdl(igemm_tiny_unfused_kernel, dim3((unsigned)ceil_div(total, 256)), dim3(256), 0, ctx,
                                  d_in, d_kernel, d_out, P, ep));
         return FC_OK;
     }

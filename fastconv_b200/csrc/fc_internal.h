@@ -132,6 +132,7 @@ struct fc_context {
     int *d_status;  // device word kernels with bounded waits report into
     cudaStream_t copy_in, copy_out;  // created on first use by the pipelined host forward
     unsigned peer_wait_polls;        // iteration limit of the flag waits of channel-split layers
+    bool signals_early;  // a kernel that signals early has been launched (or captured) on this stream; see launch_pdl
 };
 
 // Programmatic dependent launch.  Every kernel of the forward path is launched with the
@@ -154,8 +155,8 @@ __device__ __forceinline__ void pdl_trigger() {}
 namespace fc {
 bool pdl_enabled();
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                              Args &&...args) {
+inline cudaError_t launch_programmatic(bool programmatic, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                                       cudaStream_t stream, Args &&...args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -165,8 +166,18 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    cfg.numAttrs = programmatic ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+// The layers' kernels read their maps through the read-only path, which asks for data that nobody writes while the kernel
+// runs.  Behind a kernel that signals early they would start while it still writes, so on a context that has had one they
+// are launched in plain stream order (as fast, see above).  Not only directly behind one: a captured launch may be replayed
+// behind anything.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, const fc_context *ctx,
+                              Args &&...args) {
+    return launch_programmatic(pdl_enabled() && !ctx->signals_early, kernel, grid, block, smem, ctx->stream,
+                               static_cast<Args &&>(args)...);
 }
 }  // namespace fc
 #endif

@@ -353,18 +353,28 @@ class DeviceScope {
 
 // Lets the next kernel of the stream begin its set-up (barriers, tensor memory, descriptors) on SMs that this one leaves
 // free or has left; it touches nothing of this one's before its own pdl_wait().  Every block says so after its own wait, which
-// keeps the chain: a kernel ends only after the one before it.
+// keeps the chain: a kernel ends only after the one before it.  What another kernel may have written is read by plain loads, not
+// through the read-only path (ld.global.nc, which __ldg and pointers to const that are __restrict__ turn into): it has to stand
+// still from a kernel's start on, not from its wait on.
 __device__ __forceinline__ void pdl_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// A launch of clusters of `cluster` blocks, in stream order like every other (programmatic dependent launch).
+// Launches of kernels that call pdl_next(), in stream order like every other (programmatic dependent launch); the context
+// remembers that it has had one.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_early(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, fc_context *ctx, Args &&...args) {
+    ctx->signals_early = true;
+    return launch_programmatic(pdl_enabled(), kernel, grid, block, smem, ctx->stream, static_cast<Args &&>(args)...);
+}
+// in clusters of `cluster` blocks
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, unsigned threads, unsigned cluster, size_t smem,
-                                   cudaStream_t stream, Args &&...args) {
+                                   fc_context *ctx, Args &&...args) {
+    ctx->signals_early = true;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
+    cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;

@@ -25,8 +25,7 @@ struct MoveShape {
 
 // kPairs: two neighbouring channels of the channels-last map move as one word (16-bit types, even stride, 4-byte aligned).
 template <typename T, bool kToLast, bool kPairs, int TC>
-__global__ void __launch_bounds__(MOVE_THREADS, 8) map_move_kernel(float *__restrict__ planes, T *__restrict__ last_map,
-                                                               const MoveShape s) {
+__global__ void __launch_bounds__(MOVE_THREADS, 8) map_move_kernel(float *planes, T *last_map, const MoveShape s) {
     constexpr int TP = TILE / TC, PAD = TC < 32 ? 32 / TC : 1;  // the pad keeps a warp's columns in different banks
     __shared__ float tile[TC][TP + PAD];                        // [channel][pixel]
     const uint32_t rest = blockIdx.x / (uint32_t)s.ctiles, ct = blockIdx.x - rest * s.ctiles;
@@ -58,7 +57,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 8) map_move_kernel(float *__rest
         constexpr bool W = decltype(whole)::value;
         if (kToLast) {
             float v[P_ITEMS];  // all loads before the first use
-            plane_side(whole, [&](int i, int c, int px, bool in) { v[i] = in ? __ldg(plane + (size_t)c * s.pixels + px) : 0.0f; });
+            plane_side(whole, [&](int i, int c, int px, bool in) { v[i] = in ? plane[(size_t)c * s.pixels + px] : 0.0f; });
             plane_side(whole, [&](int i, int c, int px, bool) { tile[c][px] = v[i]; });
             __syncthreads();
             last_side(whole, [&](int, int c, int p, bool in) {
@@ -123,8 +122,8 @@ int move(fc_context *ctx, float *planes, void *last_map, int batch, int channels
         auto go = [&](auto pairs, auto width) -> int {
             constexpr bool P = decltype(pairs)::value;
             constexpr int TC = decltype(width)::value;
-            FC_CHECK_CUDA(launch_pdl(to_last ? map_move_kernel<T, true, P, TC> : map_move_kernel<T, false, P, TC>, dim3((unsigned)blocks),
-                                     dim3(MOVE_THREADS), 0, ctx->stream, planes, (T *)last_map, s));
+            FC_CHECK_CUDA(launch_early(to_last ? map_move_kernel<T, true, P, TC> : map_move_kernel<T, false, P, TC>, dim3((unsigned)blocks),
+                                     dim3(MOVE_THREADS), 0, ctx, planes, (T *)last_map, s));
             return FC_OK;
         };
         auto by_width = [&](auto pairs) -> int {

@@ -734,7 +734,7 @@ int launch_blocked_tma(fc_context *ctx, const float *d_U, const float *d_V, floa
     auto kern = wino_gemm_ffma_tma_kernel<BM, BN, MAP, BKT, NST, FLEX>;
     FC_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     dim3 grid((unsigned)ceil_div(g.tp, BN), (unsigned)ceil_div(g.oc, BM), 64), block(THREADS);
-    FC_CHECK_CUDA((launch_pdl(kern, grid, block, smem, ctx->stream, tmU, tmV, d_M, ctx->d_status, g.oc, g.tp, g.icp)));
+    FC_CHECK_CUDA((launch_pdl(kern, grid, block, smem, ctx, tmU, tmV, d_M, ctx->d_status, g.oc, g.tp, g.icp)));
     return FC_OK;
 }
 
@@ -749,7 +749,7 @@ int launch_blocked_tma_mixed(fc_context *ctx, const float *d_U, const float *d_V
     FC_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const int n_main = g.tp / 128;
     dim3 grid((unsigned)n_main + 1, (unsigned)ceil_div(g.oc, 128), 64), block(THREADS);
-    FC_CHECK_CUDA((launch_pdl(kern, grid, block, smem, ctx->stream, tmU, tmV, tmVtail, d_M, ctx->d_status, g.oc, g.tp, g.icp,
+    FC_CHECK_CUDA((launch_pdl(kern, grid, block, smem, ctx, tmU, tmV, tmVtail, d_M, ctx->d_status, g.oc, g.tp, g.icp,
                               n_main)));
     return FC_OK;
 }
@@ -759,7 +759,7 @@ template <int TN>
 int launch_skinny(fc_context *ctx, const float *d_U, const float *d_V, float *d_M, const WinoGeom &g) {
     if (ctx->d_status == nullptr) {  // no context behind the call: the plain-load kernel
         dim3 grid((unsigned)ceil_div(g.oc, SK_THREADS), 64), block(SK_THREADS);
-        FC_CHECK_CUDA(launch_pdl(wino_gemm_ffma_skinny_kernel<TN>, grid, block, 0, ctx->stream, d_U, d_V, d_M, g.oc, g.ocp,
+        FC_CHECK_CUDA(launch_pdl(wino_gemm_ffma_skinny_kernel<TN>, grid, block, 0, ctx, d_U, d_V, d_M, g.oc, g.ocp,
                                  g.tp, g.icp));
         return FC_OK;
     }
@@ -774,7 +774,7 @@ int launch_skinny(fc_context *ctx, const float *d_U, const float *d_V, float *d_
     FC_CHECK_CUDA(cudaFuncSetAttribute(wino_gemm_ffma_skinny_tma_kernel<TT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)smem));
     dim3 grid((unsigned)ceil_div(g.oc, 128), 64), block(ST_THREADS);
-    FC_CHECK_CUDA((launch_pdl(wino_gemm_ffma_skinny_tma_kernel<TT>, grid, block, smem, ctx->stream, tmU, tmV, d_M,
+    FC_CHECK_CUDA((launch_pdl(wino_gemm_ffma_skinny_tma_kernel<TT>, grid, block, smem, ctx, tmU, tmV, d_M,
                               ctx->d_status, g.oc, g.tp, g.icp)));
     return FC_OK;
 }
@@ -795,7 +795,7 @@ int launch_flex(fc_context *ctx, const float *d_U, const float *d_V, float *d_M,
     const size_t smem = (size_t)STAGES * BK * (128 + BN) * sizeof(float);
     FC_CHECK_CUDA(cudaFuncSetAttribute(wino_gemm_ffma_flex_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     dim3 grid((unsigned)ceil_div(g.tp, BN), (unsigned)ceil_div(g.oc, 128), 64), block(THREADS);
-    FC_CHECK_CUDA((launch_pdl(wino_gemm_ffma_flex_kernel<TN>, grid, block, smem, ctx->stream, d_U, d_V, d_M, g.oc, g.ocp,
+    FC_CHECK_CUDA((launch_pdl(wino_gemm_ffma_flex_kernel<TN>, grid, block, smem, ctx, d_U, d_V, d_M, g.oc, g.ocp,
                               g.tp, g.icp)));
     return FC_OK;
 }
@@ -806,7 +806,7 @@ int launch_blocked(fc_context *ctx, const float *d_U, const float *d_V, float *d
     auto kern = wino_gemm_ffma_kernel<BM, BN, MAP>;
     FC_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     dim3 grid((unsigned)ceil_div(g.tp, BN), (unsigned)ceil_div(g.oc, BM), 64), block(THREADS);
-    FC_CHECK_CUDA((launch_pdl(kern, grid, block, smem, ctx->stream, d_U, d_V, d_M, g.oc, g.ocp, g.tp, g.icp)));
+    FC_CHECK_CUDA((launch_pdl(kern, grid, block, smem, ctx, d_U, d_V, d_M, g.oc, g.ocp, g.tp, g.icp)));
     return FC_OK;
 }
 

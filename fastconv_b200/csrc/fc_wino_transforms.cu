@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(256) input_transform_kernel(const float *__res
 
 int launch_input_transform(fc_context *ctx, const float *d_in, float *d_V, const WinoGeom &g) {
     dim3 block(256), grid((unsigned)g.tp, (unsigned)ceil_div(g.icp, IT_CH));
-    FC_CHECK_CUDA(launch_pdl(input_transform_kernel, grid, block, 0, ctx->stream, d_in, d_V, g.tiles, g.ic, g.icp, g.tp,
+    FC_CHECK_CUDA(launch_pdl(input_transform_kernel, grid, block, 0, ctx, d_in, d_V, g.tiles, g.ic, g.icp, g.tp,
                              g.ih, g.iw, g.pad, g.th, g.tw));
     return FC_OK;
 }
@@ -409,26 +409,26 @@ int launch_input_transform_rowmajor(fc_context *ctx, const float *d_in, float *d
         dim3 wblock(32 * ITW_WARPS);
         if (g.tiles >= 32 * ITW_WARPS) {
             dim3 grid((unsigned)ceil_div(g.tp, 32 * ITW_WARPS), (unsigned)g.icp);
-            FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_wide_kernel<true>, grid, wblock, 0, ctx->stream, d_in, d_V, g.tiles,
+            FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_wide_kernel<true>, grid, wblock, 0, ctx, d_in, d_V, g.tiles,
                                      g.ic, g.icp, g.tp, g.ih, g.iw, g.pad, g.th, g.tw, pairs_on));
         } else {
             dim3 grid((unsigned)ceil_div(g.tp, 32), (unsigned)ceil_div(g.icp, ITW_WARPS));
-            FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_wide_kernel<false>, grid, wblock, 0, ctx->stream, d_in, d_V, g.tiles,
+            FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_wide_kernel<false>, grid, wblock, 0, ctx, d_in, d_V, g.tiles,
                                      g.ic, g.icp, g.tp, g.ih, g.iw, g.pad, g.th, g.tw, pairs_on));
         }
         return FC_OK;
     }
     if (g.tiles > 16) {
         dim3 grid((unsigned)ceil_div(g.tp, 32), (unsigned)g.icp);
-        FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_kernel<32>, grid, block, 0, ctx->stream, d_in, d_V, g.tiles,
+        FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_kernel<32>, grid, block, 0, ctx, d_in, d_V, g.tiles,
                                  g.ic, g.icp, g.tp, g.ih, g.iw, g.pad, g.th, g.tw));
     } else if (g.tiles > 8) {
         dim3 grid((unsigned)ceil_div(g.tp, 16), (unsigned)ceil_div(g.icp, 2));
-        FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_kernel<16>, grid, block, 0, ctx->stream, d_in, d_V, g.tiles,
+        FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_kernel<16>, grid, block, 0, ctx, d_in, d_V, g.tiles,
                                  g.ic, g.icp, g.tp, g.ih, g.iw, g.pad, g.th, g.tw));
     } else {
         dim3 grid((unsigned)ceil_div(g.tp, 8), (unsigned)ceil_div(g.icp, 4));
-        FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_kernel<8>, grid, block, 0, ctx->stream, d_in, d_V, g.tiles,
+        FC_CHECK_CUDA(launch_pdl(input_transform_rowmajor_kernel<8>, grid, block, 0, ctx, d_in, d_V, g.tiles,
                                  g.ic, g.icp, g.tp, g.ih, g.iw, g.pad, g.th, g.tw));
     }
     return FC_OK;
@@ -861,25 +861,25 @@ int launch_output_transform(fc_context *ctx, const float *d_M, float *d_out, con
         if (g.tiles >= 32 * OTW_WARPS) {  // four warps along the tile axis: reads of 512 bytes per position (1 % faster)
             dim3 grid((unsigned)ceil_div(g.tiles, 32 * OTW_WARPS), (unsigned)g.oc);
             FC_CHECK_CUDA(launch_pdl(upfront ? output_transform_wide_kernel<true, true> : output_transform_wide_kernel<true, false>,
-                                     grid, wblock, 0, ctx->stream, d_M, d_out, g.tiles, g.oc, g.tp, g.oh, g.ow, g.th, g.tw, ep));
+                                     grid, wblock, 0, ctx, d_M, d_out, g.tiles, g.oc, g.tp, g.oh, g.ow, g.th, g.tw, ep));
         } else {
             dim3 grid((unsigned)ceil_div(g.tiles, 32), (unsigned)ceil_div(g.oc, OTW_WARPS));
-            FC_CHECK_CUDA(launch_pdl(output_transform_wide_kernel<false, false>, grid, wblock, 0, ctx->stream, d_M, d_out, g.tiles,
+            FC_CHECK_CUDA(launch_pdl(output_transform_wide_kernel<false, false>, grid, wblock, 0, ctx, d_M, d_out, g.tiles,
                                      g.oc, g.tp, g.oh, g.ow, g.th, g.tw, ep));
         }
         return FC_OK;
     }
     if (g.tiles > 16) {
         dim3 grid((unsigned)ceil_div(g.tiles, 32), (unsigned)g.oc);
-        FC_CHECK_CUDA(launch_pdl(output_transform_kernel<32>, grid, block, 0, ctx->stream, d_M, d_out, g.tiles, g.oc, g.tp,
+        FC_CHECK_CUDA(launch_pdl(output_transform_kernel<32>, grid, block, 0, ctx, d_M, d_out, g.tiles, g.oc, g.tp,
                                  g.oh, g.ow, g.th, g.tw, ep));
     } else if (g.tiles > 8) {
         dim3 grid(1, (unsigned)ceil_div(g.oc, 2));
-        FC_CHECK_CUDA(launch_pdl(output_transform_kernel<16>, grid, block, 0, ctx->stream, d_M, d_out, g.tiles, g.oc, g.tp,
+        FC_CHECK_CUDA(launch_pdl(output_transform_kernel<16>, grid, block, 0, ctx, d_M, d_out, g.tiles, g.oc, g.tp,
                                  g.oh, g.ow, g.th, g.tw, ep));
     } else {
         dim3 grid(1, (unsigned)ceil_div(g.oc, 4));
-        FC_CHECK_CUDA(launch_pdl(output_transform_kernel<8>, grid, block, 0, ctx->stream, d_M, d_out, g.tiles, g.oc, g.tp,
+        FC_CHECK_CUDA(launch_pdl(output_transform_kernel<8>, grid, block, 0, ctx, d_M, d_out, g.tiles, g.oc, g.tp,
                                  g.oh, g.ow, g.th, g.tw, ep));
     }
     FC_CHECK_CUDA(cudaGetLastError());
@@ -897,7 +897,7 @@ int launch_output_transform_fused_gemm(fc_context *ctx, const float *d_U, const 
     auto go = [&](auto kern) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
-        return launch_pdl(kern, grid, block, smem, ctx->stream, d_U, d_V, d_out, g.tiles, g.oc, g.ocp, g.icp, g.tp, g.oh,
+        return launch_pdl(kern, grid, block, smem, ctx, d_U, d_V, d_out, g.tiles, g.oc, g.ocp, g.icp, g.tp, g.oh,
                           g.ow, g.th, g.tw, ep);
     };
     const bool epi = ep.bias != nullptr || ep.relu;
@@ -915,15 +915,15 @@ int launch_output_transform_scatter(fc_context *ctx, const float *d_M, const Pee
     dim3 block(256);
     if (g.tiles > 16) {
         dim3 grid((unsigned)ceil_div(g.tiles, 32), (unsigned)g.oc);
-        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_kernel<32>, grid, block, 0, ctx->stream, d_M, dst, g.tiles, g.oc,
+        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_kernel<32>, grid, block, 0, ctx, d_M, dst, g.tiles, g.oc,
                                  g.tp, g.oh, g.ow, g.th, g.tw, ep));
     } else if (g.tiles > 8) {
         dim3 grid(1, (unsigned)ceil_div(g.oc, 2));
-        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_kernel<16>, grid, block, 0, ctx->stream, d_M, dst, g.tiles, g.oc,
+        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_kernel<16>, grid, block, 0, ctx, d_M, dst, g.tiles, g.oc,
                                  g.tp, g.oh, g.ow, g.th, g.tw, ep));
     } else {
         dim3 grid(1, (unsigned)ceil_div(g.oc, 4));
-        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_kernel<8>, grid, block, 0, ctx->stream, d_M, dst, g.tiles, g.oc,
+        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_kernel<8>, grid, block, 0, ctx, d_M, dst, g.tiles, g.oc,
                                  g.tp, g.oh, g.ow, g.th, g.tw, ep));
     }
     return FC_OK;
@@ -934,15 +934,15 @@ int launch_output_transform_scatter_publish(fc_context *ctx, const float *d_M, c
     dim3 block(256);
     if (g.tiles > 16) {
         dim3 grid((unsigned)ceil_div(g.tiles, 32), (unsigned)g.oc);
-        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_publish_kernel<32>, grid, block, 0, ctx->stream, d_M, dst, g.tiles,
+        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_publish_kernel<32>, grid, block, 0, ctx, d_M, dst, g.tiles,
                                  g.oc, g.tp, g.oh, g.ow, g.th, g.tw, ep));
     } else if (g.tiles > 8) {
         dim3 grid(1, (unsigned)ceil_div(g.oc, 2));
-        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_publish_kernel<16>, grid, block, 0, ctx->stream, d_M, dst, g.tiles,
+        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_publish_kernel<16>, grid, block, 0, ctx, d_M, dst, g.tiles,
                                  g.oc, g.tp, g.oh, g.ow, g.th, g.tw, ep));
     } else {
         dim3 grid(1, (unsigned)ceil_div(g.oc, 4));
-        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_publish_kernel<8>, grid, block, 0, ctx->stream, d_M, dst, g.tiles,
+        FC_CHECK_CUDA(launch_pdl(output_transform_scatter_publish_kernel<8>, grid, block, 0, ctx, d_M, dst, g.tiles,
                                  g.oc, g.tp, g.oh, g.ow, g.th, g.tw, ep));
     }
     return FC_OK;

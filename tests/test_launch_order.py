@@ -93,3 +93,22 @@ def test_a_kernel_of_a_programmatic_launch_waits(file, name, body, helpers):
         text = without_lambdas(text)
         before = text[:text.index("pdl_wait()")]
         assert not re.search(r"\breturn\s*;", before), f"{file}: threads of {name} may leave before the wait"
+
+
+def test_what_an_early_kernel_may_still_write_is_not_read_through_the_read_only_path():
+    """Kernels that signal early, and those that start behind them, read by plain loads; all others are launched by launch_pdl,
+    which leaves the attribute out once the context has had an early kernel."""
+    early = [f for f in CSRC.glob("*.cu") if "pdl_next()" in code(f)]
+    assert len(early) >= 5
+    for path in (*early, CSRC / "fc_last.cuh"):
+        text = code(path)
+        assert "__ldg" not in text and "ld.global.nc" not in text, path.name
+        assert not re.search(r"const\s+\w+\s*\*\s*__restrict__", text), path.name
+    assert not re.search(r"launch_pdl\s*\(", "".join(code(p) for p in early))
+    moves = code(CSRC / "fc_map_move.cu")
+    assert "__restrict__" not in moves  # one of the two is read, by direction
+    internal, last = code(CSRC / "fc_internal.h"), code(CSRC / "fc_last.cuh")
+    assert "pdl_enabled() && !ctx->signals_early" in internal and last.count("ctx->signals_early = true") == 2
+    for path in CSRC.glob("*.cu"):
+        if path not in early:
+            assert "launch_early" not in code(path) and "launch_clusters" not in code(path) and "cudaLaunchKernelEx" not in code(path)
