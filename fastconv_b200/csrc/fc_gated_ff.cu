@@ -365,7 +365,7 @@ int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const voi
     if (b.rows == 0) return FC_OK;
     FC_PROPAGATE(check_pointers(b, {d_x, d_w_gate, d_w_up, d_w_down, d_y}, {d_b_gate, d_b_up, d_b_down}));
     FC_REQUIRE((uintptr_t)d_saved % 4 == 0, FC_ERR_INVALID_ARG, "the saved values' address is no multiple of 4");
-    FC_REQUIRE(d_y != d_x, FC_ERR_INVALID_ARG, "the output is the input");
+    FC_PROPAGATE(check_outputs({d_y, d_saved, d_workspace}, {d_x, d_w_gate, d_w_up, d_w_down, d_b_gate, d_b_up, d_b_down}));
     const Work w = carve(b, d_workspace, false);
     FC_PROPAGATE(check_workspace(d_workspace, workspace_bytes, w.bytes));
     DeviceScope dev(ctx->device);
@@ -409,7 +409,8 @@ int fc_gated_ff_backward(fc_context *ctx, const fc_gated_ff_desc *desc, const vo
     if (b.rows > 0) FC_PROPAGATE(check_pointers(b, {d_dy, d_x, d_w_gate, d_w_up, d_w_down, d_saved}, {}));
     FC_REQUIRE((uintptr_t)d_saved % 4 == 0, FC_ERR_INVALID_ARG, "the saved values' address is no multiple of 4");
     FC_PROPAGATE(check_pointers(b, {}, {d_dx, d_dw_gate, d_dw_up, d_dw_down, d_db_gate, d_db_up, d_db_down}));
-    FC_REQUIRE(d_dx == nullptr || (d_dx != d_x && d_dx != d_dy), FC_ERR_INVALID_ARG, "an output is an input");
+    FC_PROPAGATE(check_outputs({d_dx, d_dw_gate, d_dw_up, d_dw_down, d_db_gate, d_db_up, d_db_down, d_workspace},
+                               {d_dy, d_x, d_w_gate, d_w_up, d_w_down, d_saved}));
     const Work w = carve(b, d_workspace, true);
     FC_PROPAGATE(check_workspace(d_workspace, workspace_bytes, w.bytes));
     DeviceScope dev(ctx->device);

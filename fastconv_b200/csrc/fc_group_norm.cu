@@ -1074,7 +1074,7 @@ int fc_group_norm_forward(fc_context *ctx, const fc_group_norm_desc *desc, const
     FC_PROPAGATE(norm_shape(desc, &s));
     if (s.batch == 0) return FC_OK;
     FC_PROPAGATE(check_maps(desc, {d_x, d_y}, {d_gamma, d_beta}, d_mean, d_rstd));
-    FC_REQUIRE(d_y != d_x, FC_ERR_INVALID_ARG, "the output is the input");
+    FC_PROPAGATE(check_outputs({d_y, d_mean, d_rstd, d_workspace}, {d_x, d_gamma, d_beta}));
     size_t need;
     FC_PROPAGATE(fc_group_norm_workspace(desc, &need, nullptr));
     FC_REQUIRE(d_workspace != nullptr && aligned16(d_workspace) && workspace_bytes >= need, FC_ERR_INVALID_ARG,
@@ -1122,7 +1122,7 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
     FC_PROPAGATE(norm_shape(desc, &s));
     if (s.batch > 0) FC_PROPAGATE(check_maps(desc, {d_dy, d_x, d_dx ? d_dx : d_x}, {}, nullptr, nullptr));
     FC_PROPAGATE(check_maps(desc, {}, {d_gamma, d_beta, d_dgamma, d_dbeta}, d_mean, d_rstd));  // of no images they are written too
-    FC_REQUIRE(d_dx == nullptr || (d_dx != d_x && d_dx != d_dy), FC_ERR_INVALID_ARG, "an output is an input");
+    FC_PROPAGATE(check_outputs({d_dx, d_dgamma, d_dbeta, d_workspace}, {d_dy, d_x, d_gamma, d_beta, d_mean, d_rstd}));
     FC_REQUIRE(s.batch == 0 || (d_mean != nullptr && d_rstd != nullptr), FC_ERR_INVALID_ARG,
                "the gradient needs the forward pass's mean and rstd");
     size_t need;

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 #include "fc_internal.h"
 
 namespace fc {
@@ -336,6 +338,18 @@ int with_type(int type, F &&f) {
         case FC_DTYPE_F16: return f(__half());
         default: return f(float());
     }
+}
+
+// Refuses an output that begins where an input or another output does (NULL: absent).  Maps may lie in one another's gaps, so
+// ranges are not compared.
+inline int check_outputs(std::initializer_list<const void *> outputs, std::initializer_list<const void *> inputs) {
+    for (const void *const *o = outputs.begin(); o != outputs.end(); ++o) {
+        if (*o == nullptr) continue;
+        for (const void *i : inputs) FC_REQUIRE(*o != i, FC_ERR_INVALID_ARG, "an output is an input");
+        for (const void *const *p = outputs.begin(); p != o; ++p)
+            FC_REQUIRE(*o != *p, FC_ERR_INVALID_ARG, "two outputs are one");
+    }
+    return FC_OK;
 }
 
 // Makes the context's device current for one call and puts the caller's back.

@@ -111,6 +111,7 @@ int move(fc_context *ctx, float *planes, void *last_map, int batch, int channels
     FC_REQUIRE(planes != nullptr && last_map != nullptr, FC_ERR_INVALID_ARG, "NULL map");
     FC_REQUIRE((uintptr_t)planes % 4 == 0 && (uintptr_t)last_map % dtype_size(type) == 0, FC_ERR_INVALID_ARG,
                "a map's address is no multiple of its element size");
+    FC_PROPAGATE(check_outputs({to_last ? last_map : planes}, {to_last ? planes : last_map}));
     const int tc = channels > 32 ? 64 : channels > 16 ? 32 : channels > 8 ? 16 : 8;
     MoveShape s = {channels, pixels, stride, (channels + tc - 1) / tc, (int)ceil_div(pixels, TILE / tc)};
     const long long blocks = (long long)batch * s.ctiles * s.ptiles;

@@ -398,9 +398,10 @@ int fc_sharded_conv_time_device(fc_sharded_conv *sc, int warmup, int iters, floa
  *
  * Every function works on device pointers, asynchronously on the context's stream; the caller's current device is left
  * as it was.  Addresses and strides need no alignment beyond their element's size (16-byte aligned rows are faster).
- * Outputs must not overlap inputs or one another.  Sums and statistics are fp32 whatever the type, an output is rounded
- * once, and no result depends on the order in which blocks run.  The workspace is the caller's (16-byte aligned, of the
- * bytes that the _workspace function gives for the same descriptor); it holds nothing between calls, but calls
+ * Outputs must not overlap inputs, one another or the workspace; one that begins where another operand does is refused.
+ * Sums and statistics are fp32 whatever the type, an output is rounded once, and no result depends on the order in which
+ * blocks run.  The workspace is the caller's (16-byte aligned, of the bytes that the _workspace function gives for the same
+ * descriptor); it holds nothing between calls, but calls
  * that can overlap on the GPU need one each.  That includes replays of captured graphs: a captured call keeps the
  * workspace that it was captured with.  Nothing is allocated or synchronised, so every call can be captured. */
 typedef enum fc_dtype { FC_DTYPE_F32 = 0, FC_DTYPE_BF16 = 1, FC_DTYPE_F16 = 2 } fc_dtype;
