@@ -19,6 +19,7 @@ MODE_LABELS = {0: "fp32", 1: "3xtf32", 2: "tf32", 4: "tf32-u16"}  # what fc_conv
 MODE_NAMES = {"fp32": MATH_FP32_MIRRORED, "ffma": MATH_FP32_MIRRORED, "3xtf32": MATH_3XTF32, "tf32": MATH_TF32,
               "tf32-unbounded": MATH_TF32_UNBOUNDED, "tf32-u16": MATH_TF32_U16}
 DTYPE_NAMES = {"fp32": 0, "bf16": 1, "fp16": 2}
+FF_PRODUCT_NAMES = {"gate": 0, "down": 1, "back_gate": 2, "dx": 3, "dw_in": 4, "dw_down": 5}
 ACT_NAMES = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5}
 ALGO_NAMES = {"auto": ALGO_AUTO, "direct": ALGO_DIRECT, "im2col": ALGO_IM2COL, "winograd": ALGO_WINOGRAD}
 
@@ -43,6 +44,12 @@ class GatedFfDesc(C.Structure):
 
     _fields_ = ([(n, C.c_int32) for n in ("rows", "in_channels", "hidden", "out_channels", "type", "act")]
                 + [("x_stride", C.c_int64), ("y_stride", C.c_int64)])
+
+
+class FfProductPlan(C.Structure):
+    """fc_ff_product_plan"""
+
+    _fields_ = [("tile_columns", C.c_int32), ("shares", C.c_int32), ("tiles", C.c_int64)]
 
 
 class FastConvError(RuntimeError):
@@ -150,6 +157,7 @@ SIGNATURES = {
     "fc_group_norm_forward": (C.c_int, [_vp, C.POINTER(GroupNormDesc)] + [_vp] * 7 + [C.c_size_t]),
     "fc_group_norm_backward": (C.c_int, [_vp, C.POINTER(GroupNormDesc)] + [_vp] * 10 + [C.c_size_t]),
     "fc_gated_ff_workspace": (C.c_int, [C.POINTER(GatedFfDesc), _szp, _szp]),
+    "fc_gated_ff_plan": (C.c_int, [C.POINTER(GatedFfDesc), C.c_int, C.POINTER(FfProductPlan)]),
     "fc_gated_ff_forward": (C.c_int, [_vp, C.POINTER(GatedFfDesc)] + [_vp] * 10 + [C.c_size_t]),
     "fc_gated_ff_backward": (C.c_int, [_vp, C.POINTER(GatedFfDesc)] + [_vp] * 14 + [C.c_size_t]),
     "fc_diff": (C.c_float, [_vp, _vp, C.c_int]),

@@ -15,7 +15,7 @@ import ctypes as C
 from typing import Optional
 
 from . import _lib
-from ._lib import GatedFfDesc, GroupNormDesc, check
+from ._lib import FfProductPlan, GatedFfDesc, GroupNormDesc, check
 from .layers import Context, default_context
 
 
@@ -110,6 +110,14 @@ class GatedFeedForward(_Plan):
         desc = GatedFfDesc(rows, in_channels, hidden, in_channels if out_channels is None else out_channels,
                            _named(_lib.DTYPE_NAMES, "dtype", dtype), _named(_lib.ACT_NAMES, "act", act), x_stride, y_stride)
         self._take(ctx, _lib.load().fc_gated_ff_workspace, desc, train)
+
+    def product_plan(self, product: str):
+        """What "gate", "down", "back_gate", "dx", "dw_in" or "dw_down" is cut into on the tensor cores: `tile_columns`, `shares` of
+        the reduction and `tiles`."""
+        plan = FfProductPlan()
+        check(self._ready().fc_gated_ff_plan(self._ref, _named(_lib.FF_PRODUCT_NAMES, "product", product), C.byref(plan)),
+              "fc_gated_ff_plan")
+        return plan
 
     def forward(self, x: int, y: int, *, w_gate: int, w_up: int, w_down: int, b_gate: int = 0, b_up: int = 0, b_down: int = 0,
                 saved: int = 0) -> None:

@@ -900,6 +900,14 @@ size_t ff_tc_part_floats(const FfProduct &p) {
     return plan.splits > 1 ? (size_t)plan.splits * dests * ceil_div(m, 256) * 256 * round_up(p.n, 4) : 0;
 }
 
+fc_ff_product_plan ff_tc_cut(const FfProduct &p) {
+    int dests, m, kb_first, kb_total;
+    tc_shape(p, &dests, &m, &kb_first, &kb_total);
+    const FfTcPlan plan = ff_tc_plan(p.planes, p.kind, dests, m, p.n, kb_total, p.b_by_k);
+    const int columns = p.kind == FF_GATE ? plan.bn / 2 : plan.bn;
+    return fc_ff_product_plan{plan.bn, plan.splits, (int64_t)dests * (int64_t)ceil_div(m, 256) * (int64_t)ceil_div(p.n, columns)};
+}
+
 int launch_ff_tc(fc_context *ctx, const FfProduct &p) {
     int dests, m, kb_first, kb_total;
     tc_shape(p, &dests, &m, &kb_first, &kb_total);

@@ -225,7 +225,15 @@ FfProduct product(const Block &b, int kind, int m, int n, int k, const Matrix &a
     return p;
 }
 
-// the block's FF_STORE products
+// the block's products, but for what only a call knows
+FfProduct gate_product(const Block &b, const Matrix &x, const Matrix &w_gate, const void *w_up) {
+    FfProduct p = product(b, FF_GATE, b.rows, b.hidden, b.in, x, true, w_gate, true);
+    p.b1 = w_up;
+    return p;
+}
+FfProduct back_gate_product(const Block &b, const Matrix &dy, const Matrix &w_down) {
+    return product(b, FF_GATE_BACK, b.rows, b.hidden, b.out, dy, true, w_down, false);
+}
 FfProduct down_product(const Block &b, const Matrix &h, const Matrix &w_down, const void *bias, void *y) {
     FfProduct p = product(b, FF_STORE, b.rows, b.out, b.hidden, h, true, w_down, true);
     p.bias0 = bias;
@@ -356,6 +364,23 @@ int fc_gated_ff_workspace(const fc_gated_ff_desc *desc, size_t *forward_bytes, s
     return FC_OK;
 }
 
+int fc_gated_ff_plan(const fc_gated_ff_desc *desc, int product, fc_ff_product_plan *plan) {
+    Block b;
+    FC_PROPAGATE(block_of(desc, &b));
+    FC_REQUIRE(plan != nullptr, FC_ERR_INVALID_ARG, "plan is NULL");
+    FC_REQUIRE(b.rows > 0, FC_ERR_INVALID_ARG, "a block of no rows has no products");
+    const Matrix none = {};
+    switch (product) {
+        case FC_FF_GATE: *plan = ff_tc_cut(gate_product(b, none, none, nullptr)); return FC_OK;
+        case FC_FF_DOWN: *plan = ff_tc_cut(down_product(b, none, none, nullptr, nullptr)); return FC_OK;
+        case FC_FF_BACK_GATE: *plan = ff_tc_cut(back_gate_product(b, none, none)); return FC_OK;
+        case FC_FF_DX: *plan = ff_tc_cut(dx_product(b, none, none, nullptr, nullptr)); return FC_OK;
+        case FC_FF_DW_IN: *plan = ff_tc_cut(dw_in_product(b, none, none, nullptr, nullptr)); return FC_OK;
+        case FC_FF_DW_DOWN: *plan = ff_tc_cut(dw_down_product(b, none, none, nullptr)); return FC_OK;
+    }
+    FC_REQUIRE(false, FC_ERR_INVALID_ARG, "unknown product %d", product);
+}
+
 int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const void *d_x, const void *d_w_gate, const void *d_w_up,
                         const void *d_w_down, const void *d_b_gate, const void *d_b_up, const void *d_b_down, void *d_y,
                         float *d_saved, void *d_workspace, size_t workspace_bytes) {
@@ -373,8 +398,7 @@ int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const voi
     float *up = d_saved ? d_saved + (size_t)b.rows * b.hidden : nullptr;
     const Matrix x0 = {d_x, b.xs, 0}, wg0 = {d_w_gate, b.in, 0}, wd0 = {d_w_down, b.hidden, 0};
     auto gate = [&](const Matrix &x, const Matrix &w_gate, const void *w_up) {
-        FfProduct p = product(b, FF_GATE, b.rows, b.hidden, b.in, x, true, w_gate, true);
-        p.b1 = w_up;
+        FfProduct p = gate_product(b, x, w_gate, w_up);
         p.bias0 = d_b_gate;
         p.bias1 = d_b_up;
         p.gate = d_saved;
@@ -435,7 +459,7 @@ int fc_gated_ff_backward(fc_context *ctx, const fc_gated_ff_desc *desc, const vo
     }
     FC_PROPAGATE(pack.run(ctx));
 
-    FfProduct p = product(b, FF_GATE_BACK, b.rows, b.hidden, b.out, dy, true, w_down, false);
+    FfProduct p = back_gate_product(b, dy, w_down);
     p.gate = const_cast<float *>(d_saved);
     p.up = p.gate + (size_t)b.rows * b.hidden;
     p.a_skip = w.dgu.ld / 2;

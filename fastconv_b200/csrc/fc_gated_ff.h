@@ -51,6 +51,7 @@ bool ff_few_fits(const FfProduct &p);  // at most 8 rows
 int launch_ff_few(fc_context *ctx, const FfProduct &p);
 
 size_t ff_tc_part_floats(const FfProduct &p);  // what p.part has to hold
+fc_ff_product_plan ff_tc_cut(const FfProduct &p);
 int launch_ff_tc(fc_context *ctx, const FfProduct &p);
 
 }  // namespace fc

@@ -456,6 +456,22 @@ typedef struct fc_gated_ff_desc {
     int64_t x_stride, y_stride; /* of x and dx; of y and dy: elements from one row to the next.  0 = their channels */
 } fc_gated_ff_desc;
 int fc_gated_ff_workspace(const fc_gated_ff_desc *desc, size_t *forward_bytes, size_t *backward_bytes);
+/* What one of the block's products on the tensor cores is cut into, from the shape alone: tiles of 256 rows (of the product) by
+ * `tile_columns` (of FC_FF_GATE half as many columns of each of its two matrices), and shares of the reduction; a pair of SMs
+ * takes tiles, or shares of tiles, in turn.  (Forward passes of at most 8 aligned rows do without tiles.) */
+typedef enum fc_ff_product {
+    FC_FF_GATE = 0,      /* x by w_gate and w_up */
+    FC_FF_DOWN = 1,
+    FC_FF_BACK_GATE = 2, /* dy by w_down, with what makes the gradients of gate and up of it */
+    FC_FF_DX = 3,
+    FC_FF_DW_IN = 4,     /* dw_gate and dw_up */
+    FC_FF_DW_DOWN = 5
+} fc_ff_product;
+typedef struct fc_ff_product_plan {
+    int32_t tile_columns, shares;
+    int64_t tiles;
+} fc_ff_product_plan;
+int fc_gated_ff_plan(const fc_gated_ff_desc *desc, int product, fc_ff_product_plan *plan);
 /* d_b_gate, d_b_up [hidden], d_b_down [out_channels]: NULL = none.  d_saved: 2 * rows * hidden floats whatever the type, what the
  * backward pass needs of the values before the activation (in an order of the library's own); NULL = not wanted. */
 int fc_gated_ff_forward(fc_context *ctx, const fc_gated_ff_desc *desc, const void *d_x, const void *d_w_gate,
