@@ -97,6 +97,20 @@ __device__ __forceinline__ Place place_of(const NormShape &s) {
     return b;
 }
 
+// use(p, load(p)) for the thread's pixels p, N loads before the first use: plain loads stay behind the stores before them
+template <int N, typename L, typename U>
+__device__ __forceinline__ void over_pixels(const Place &b, L &&load, U &&use) {
+    int p = b.p0 + b.row;
+    for (; p + (N - 1) * b.rows < b.p1; p += N * b.rows) {
+        decltype(load(0)) v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = load(p + i * b.rows);
+#pragma unroll
+        for (int i = 0; i < N; ++i) use(p + i * b.rows, v[i]);
+    }
+    for (; p < b.p1; p += b.rows) use(p, load(p));
+}
+
 // joins (nb, mb, qb) into (na, ma, qa): count, mean, sum of squared deviations
 __device__ __forceinline__ void join(float &na, float &ma, float &qa, float nb, float mb, float qb) {
     if (nb == 0.0f) return;
@@ -218,18 +232,17 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_apply_kernel(const T *x, co
     }
     const T *src = x + (size_t)b.img * s.pixels * s.xs + b.c0;
     T *dst = y + (size_t)b.img * s.pixels * s.ys + b.c0;
-#pragma unroll 4
-    for (int p = b.p0 + b.row; p < b.p1; p += b.rows) {
-        float f[VEC];
-        Vec<T, VEC>::load(src + (size_t)p * s.xs).unpack(f);
+    over_pixels<4>(
+        b, [&](int p) { return Vec<T, VEC>::load(src + (size_t)p * s.xs); },
+        [&](int p, const Vec<T, VEC> &v) {
+            float f[VEC];
+            v.unpack(f);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] = act_value<ACT, kExact>(fmaf(f[i] - m[i], a[i], o[i]));
-        {
+            for (int i = 0; i < VEC; ++i) f[i] = act_value<ACT, kExact>(fmaf(f[i] - m[i], a[i], o[i]));
             Vec<T, VEC> out;
             out.pack(f);
             out.store(dst + (size_t)p * s.ys);
-        }
-    }
+        });
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------
@@ -321,10 +334,13 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_join_kernel(const floa
     for (int i = threadIdx.x; i < s.cpg; i += NORM_THREADS) {
         const int c = g * s.cpg + i;
         float2 t = make_float2(0.0f, 0.0f);
-        for (int k = 0; k < s.chunks; ++k) {
-            const float2 v = part[((size_t)img * s.chunks + k) * s.channels + c];
-            t.x += v.x;
-            t.y += v.y;
+        const float2 *src = part + (size_t)img * s.chunks * s.channels + c;
+        for (int k = 0; k < s.chunks; k += 16) {  // in order, sixteen loads at a time
+            float2 v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = k + j < s.chunks ? src[(size_t)(k + j) * s.channels] : make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) t.x += v[j].x, t.y += v[j].y;
         }
         sums[(size_t)img * s.channels + c] = t;
         const float w = param<T>(gamma, c, s.params_f32, 1.0f);
@@ -355,23 +371,25 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_back_apply_kernel(const T *
     for (int i = 0; i < VEC; ++i) t[i] = ab[b.img * s.groups + (b.c0 + i) / s.cpg];
     const T *sx = x + (size_t)b.img * s.pixels * s.xs + b.c0, *sdy = dy + (size_t)b.img * s.pixels * s.ys + b.c0;
     T *dst = dx + (size_t)b.img * s.pixels * s.xs + b.c0;
-#pragma unroll 2
-    for (int p = b.p0 + b.row; p < b.p1; p += b.rows) {
-        float f[VEC], d[VEC];
-        Vec<T, VEC>::load(sx + (size_t)p * s.xs).unpack(f);
-        Vec<T, VEC>::load(sdy + (size_t)p * s.ys).unpack(d);
+    struct Two {
+        Vec<T, VEC> x, dy;
+    };
+    over_pixels<2>(
+        b, [&](int p) { return Two{Vec<T, VEC>::load(sx + (size_t)p * s.xs), Vec<T, VEC>::load(sdy + (size_t)p * s.ys)}; },
+        [&](int p, const Two &v) {
+            float f[VEC], d[VEC];
+            v.x.unpack(f);
+            v.dy.unpack(d);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            float dz, xhat;
-            ch.template at<ACT>(i, f[i], d[i], dz, xhat);
-            f[i] = ch.r[i] * (fmaf(dz, ch.g[i], -t[i].x) - xhat * t[i].y);
-        }
-        {
+            for (int i = 0; i < VEC; ++i) {
+                float dz, xhat;
+                ch.template at<ACT>(i, f[i], d[i], dz, xhat);
+                f[i] = ch.r[i] * (fmaf(dz, ch.g[i], -t[i].x) - xhat * t[i].y);
+            }
             Vec<T, VEC> out;
             out.pack(f);
             out.store(dst + (size_t)p * s.xs);
-        }
-    }
+        });
 }
 
 // ---- one kernel: the map stays in shared memory between its statistics and its result ---------------------------------
