@@ -57,7 +57,8 @@ class _Plan:
         self.ctx.adopt(self)
 
     def release(self) -> None:
-        """Gives the workspace back.  Work already enqueued is safe: later users of the arena follow it on the stream."""
+        """Gives the workspace back.  Work already enqueued is safe: later users of the arena follow it on the stream.  A graph
+        that has captured a call writes to that workspace whenever it is replayed, so the plan has to outlive it."""
         if getattr(self, "_workspace", 0):
             self.ctx.free(self._workspace)
         self._workspace = 0

@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(SUM_COLS) ff_colsum_join_kernel(const SumList 
     ((T *)p.out)[c] = Elem<T>::store(v);
 }
 
-// shares of the rows: none up to 2048 of them, else blocks for every SM, of at least 512 rows
+// shares of the rows: one up to 2048 of them, else enough that blocks reach every SM: of at most 512 rows, but no more than 64
 int colsum_chunks(int rows) {
     if (rows <= 2048) return 1;
     const long long c = ceil_div(rows, 512);

@@ -31,8 +31,7 @@ struct FfProduct {
     int row_split;             // FF_STORE: m where there is one destination.  A null destination is not computed
     const void *bias0, *bias1; // one value a column, or null
     float *gate, *up;          // what stands before the activation: written by FF_GATE (null: not wanted), read by FF_GATE_BACK
-    float *part;               // FF_STORE with splits > 1: [splits][m][n]
-    int splits;
+    float *part;               // room for the shares of a split reduction: ff_tc_part_floats
 };
 
 // Where the saved value of row m, column n lies in the gate's or the up projection's share of `saved`: [rows][n] in fp32, in

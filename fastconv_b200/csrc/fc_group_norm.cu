@@ -12,8 +12,10 @@
 // One kernel where a cluster's shared memory holds an image's block of channels (then a map is read once); otherwise
 // three each way: sums of a chunk of pixels per channel, their join per group, the map itself.  The bound is memory: 64 x
 // 28x28x512 fp32 takes 46 us (4.5 TB/s, 0.68 of the measured copy rate; two blocks of 100 KB to an SM leave memory waiting
-// between a block's loads and its stores), 64 x 56x56x256 bf16 57 us forward and 124 us backward (3.6 and 2.5 TB/s), where
-// instructions and the special-function unit are as busy as memory.
+// between a block's loads and its stores), 64 x 56x56x256 bf16 57 us forward and 124 us backward (3.6 and 2.5 TB/s): half of the
+// issue slots are taken and memory is far from full, so a block's way from barrier to barrier is what it waits for.  In three
+// kernels, whose joins have one block a group: one 224x224x128 bf16 image in 32 groups 34 us forward and 106 backward (floors
+// 4 and 6), one 112x112x256 in 1 group 104 and 60 (2 and 3); element by element 64 x 56x56x256 bf16 at stride 259 176 and 369.
 #include <cooperative_groups.h>
 
 #include <numeric>
@@ -1037,7 +1039,7 @@ bool wide_ok(const NormShape &s, std::initializer_list<const void *> maps) {
     return true;
 }
 
-// f(T(), integral_constant<int, elements of a vector>) for the widest vector that fits
+// f(T(), integral_constant<int, elements of a vector>): 16 bytes, or 1 element where channels, strides or addresses do not fit
 template <typename F>
 int with_vectors(const NormShape &s, int type, std::initializer_list<const void *> maps, F &&f) {
     return with_type(type, [&](auto t) -> int {

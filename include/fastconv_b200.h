@@ -413,6 +413,9 @@ typedef enum fc_activation {
     FC_ACT_GELU_TANH = 4, /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
     FC_ACT_SIGMOID = 5    /* 1 / (1 + exp(-z)) */
 } fc_activation;
+/* Results of 16 bits are computed with the hardware's exponential, within 2^-15 of the activation before they are rounded, down to
+ * where a sigmoid is 2^-60: one below that may count as 2^-60, and a z far below zero that it multiplies as -64, so what
+ * should vanish is at most 6e-17.  The block in fp32 takes the same bound at exp(-87). */
 
 /* Between a convolution layer's maps, fp32 [batch][channels][pixels], and channels-last ones of element type `type`
  * (rounded to nearest on the way in).  Each direction is the gradient of the other. */
@@ -446,8 +449,10 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
  *   y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd
  * with the weights of 1x1 convolutions, contiguous: w_gate, w_up [hidden][in_channels], w_down [out_channels][hidden];
  * one row is a single token or pixel.  Weights, biases, gradients and maps are of one type; between the kernels the
- * products act(.) * (.), and in the backward pass the gradients of gate and up, are rounded to that type (in fp32 they
- * keep 24 bits).  fp32 values are multiplied as sums of three bf16 parts: where an operand or an intermediate is infinite,
+ * products act(.) * (.), and in the backward pass the gradients of gate and up (of which those of their biases are the sums), are
+ * rounded to that type (in fp32 they keep 24 bits): outputs are some 1.4 times as far from the exact ones as with one rounding
+ * at the end, and in fp16 such a product beyond 65504 is infinite, and what depends on it is not finite, even where the
+ * output itself would be.  fp32 values are multiplied as sums of three bf16 parts: where an operand or an intermediate is infinite,
  * fp32 results that depend on it are NaN. */
 typedef struct fc_gated_ff_desc {
     int32_t rows, in_channels, hidden, out_channels; /* rows 0: nothing to do (the weights' gradients are then zero) */
