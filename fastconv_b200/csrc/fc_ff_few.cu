@@ -4,7 +4,8 @@
 // A warp has four weight rows and a share of the reduction: per step each lane loads 16 bytes of the four (all in flight at
 // once) and of every row of A, which the first-level cache holds after the first warp, and multiplies in fp32 pairs.  Shares
 // of a reduction meet in shared memory, lanes by shuffles, both in a fixed order.  For FF_GATE the four are two rows of the
-// gate's weights and the same two of the up projection's.  One row 1024->4096->1024 in bf16, 25 MB of weights: 6.9 us
+// gate's weights and the same two of the up projection's.  h stays in fp32 whatever the type: no tensor core asks for less, and
+// it is a few KB beside the weights.  One row 1024->4096->1024 in bf16, 25 MB of weights: 6.9 us
 // for both launches, 3.6 TB/s (6.3 us replayed from a graph), where tensor-core tiles of 256 rows took 23.7; 8 rows are where the multiplications
 // begin to show beside the loads.
 #include <type_traits>
@@ -40,26 +41,35 @@ __global__ void __launch_bounds__(FEW_THREADS) ff_few_kernel(const FfProduct p, 
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int j = 0; j < NW; ++j) acc[r][j] = 0;
-    const T *a = (const T *)p.a;
+    using A = std::conditional_t<KIND == FF_GATE, T, float>;  // x; h
+    const A *a = (const A *)p.a;
     const int vectors = p.k / VEC, hop = 32 << log_shares;
 #pragma unroll(R > 2 ? 1 : 2)
     for (int i = (share << 5) + lane; i < vectors; i += hop) {
-        Vec<T, VEC> bv[NW], av[R];
+        constexpr int AN = 16 / sizeof(A);  // a vector of T is one or two of A
+        Vec<T, VEC> bv[NW];
+        Vec<A, AN> av[R][VEC / AN];
 #pragma unroll
         for (int j = 0; j < NW; ++j) bv[j] = Vec<T, VEC>::load(w[j] + (size_t)i * VEC);
 #pragma unroll
-        for (int r = 0; r < R; ++r) av[r] = Vec<T, VEC>::load(a + (r < p.m ? r : 0) * p.lda + (size_t)i * VEC);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int h = 0; h < VEC / AN; ++h)
+                av[r][h] = Vec<A, AN>::load(a + (r < p.m ? r : 0) * p.lda + (size_t)i * VEC + h * AN);
         Pair b[NW][VEC / 2];
 #pragma unroll
         for (int j = 0; j < NW; ++j) unpack_pairs(bv[j], b[j]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            Pair c[VEC / 2];
-            unpack_pairs(av[r], c);
 #pragma unroll
-            for (int j = 0; j < NW; ++j)
+            for (int h = 0; h < VEC / AN; ++h) {
+                Pair c[AN / 2];
+                unpack_pairs(av[r][h], c);
 #pragma unroll
-                for (int e = 0; e < VEC / 2; ++e) acc[r][j] = fma2(c[e], b[j][e], acc[r][j]);
+                for (int j = 0; j < NW; ++j)
+#pragma unroll
+                    for (int e = 0; e < AN / 2; ++e) acc[r][j] = fma2(c[e], b[j][h * AN / 2 + e], acc[r][j]);
+            }
         }
     }
     float mine = 0.0f;  // lane r * NW + j (R * NW <= 32) ends up with that sum
@@ -89,7 +99,7 @@ __global__ void __launch_bounds__(FEW_THREADS) ff_few_kernel(const FfProduct p, 
         if (p.bias0) g += Elem<T>::load(((const T *)p.bias0)[n]);
         if (p.bias1) u += Elem<T>::load(((const T *)p.bias1)[n]);
         act_both_rt(p.act, g, act, slope);
-        ((T *)p.c0)[r * p.ldc + n] = Elem<T>::store(act * u);
+        ((float *)p.c0)[r * p.ldc + n] = act * u;
         if (p.gate) {
             const int64_t at = ff_saved_at(r, n, p.m, p.n);
             p.gate[at] = g;
@@ -108,7 +118,7 @@ __global__ void __launch_bounds__(FEW_THREADS) ff_few_kernel(const FfProduct p, 
 // rows of whole, aligned 16-byte vectors along the reduction
 bool ff_few_fits(const FfProduct &p) {
     const int vec = 16 / (int)dtype_size(p.type);
-    if (p.m < 1 || p.m > 8 || !p.a_by_k || !p.b_by_k || p.b_split < p.k || p.row_split < p.m) return false;
+    if (p.m < 1 || p.m > FF_FEW_ROWS || !p.a_by_k || !p.b_by_k || p.b_split < p.k || p.row_split < p.m) return false;
     if (p.k % vec || p.lda % vec || p.ldb % vec) return false;
     return aligned16(p.a) && aligned16(p.b0) && aligned16(p.b1);
 }

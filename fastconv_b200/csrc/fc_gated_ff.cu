@@ -281,6 +281,7 @@ Work carve(const Block &b, void *base, bool backward) {
     size_t part = 0;
     auto at_least = [&](size_t n) { if (n > part) part = n; };
     w.h = matrix(b.rows, hidden);
+    if (!backward && b.rows <= FF_FEW_ROWS) c.take<float>((size_t)b.rows * hidden);  // h is fp32 there, and begins where w.h does
     w.x = matrix(b.rows, in);
     w.w_gate = matrix(b.hidden, in);
     w.w_up = matrix(b.hidden, in);

@@ -46,7 +46,8 @@ inline int64_t ff_saved_at(int64_t m, int64_t n, int64_t rows, int64_t cols) {
     return block * cols + ((n >> 2) * in_block + (m - block)) * 4 + (n & 3);
 }
 
-bool ff_few_fits(const FfProduct &p);  // at most 8 rows
+constexpr int FF_FEW_ROWS = 8;
+bool ff_few_fits(const FfProduct &p);  // at most FF_FEW_ROWS; FF_GATE's c0 and FF_STORE's a are fp32
 int launch_ff_few(fc_context *ctx, const FfProduct &p);
 
 size_t ff_tc_part_floats(const FfProduct &p);  // what p.part has to hold

@@ -450,7 +450,8 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_desc *desc, cons
  * with the weights of 1x1 convolutions, contiguous: w_gate, w_up [hidden][in_channels], w_down [out_channels][hidden];
  * one row is a single token or pixel.  Weights, biases, gradients and maps are of one type; between the kernels the
  * products act(.) * (.), and in the backward pass the gradients of gate and up (of which those of their biases are the sums), are
- * rounded to that type (in fp32 they keep 24 bits): outputs are some 1.4 times as far from the exact ones as with one rounding
+ * rounded to that type (in fp32, and in forward passes of at most 8 rows whose rows and addresses are multiples of 16 bytes, they
+ * keep 24 bits): outputs are some 1.4 times as far from the exact ones as with one rounding
  * at the end, and in fp16 such a product beyond 65504 is infinite, and what depends on it is not finite, even where the
  * output itself would be.  fp32 values are multiplied as sums of three bf16 parts: where an operand or an intermediate is infinite,
  * fp32 results that depend on it are NaN. */

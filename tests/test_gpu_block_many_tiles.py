@@ -5,7 +5,7 @@ import torch
 
 import fastconv_b200 as fc
 from fastconv_b200 import _lib
-from _last_ref import DTYPES, check, ff
+from _last_ref import DTYPES, U, act, act_error, check, ff
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +95,27 @@ def test_saved_values_lie_where_they_should(lctx, rows, f, dtype):
     want = ff({**{n: v.double().cpu() for n, v in t.items()}, "b_gate": None, "b_up": None, "b_down": None}, "silu", dtype)
     for name, half in zip(("gate", "up"), saved):
         check(by_place(half, rows, f), *want[name], "fp32", name)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,k,f,o", [(1, 8, 16, 256), (2, 16, 64, 64), (4, 64, 64, 40), (8, 32, 40, 128)])
+def test_blocks_of_few_rows_round_once(lctx, rows, k, f, o, dtype):
+    """Nothing is rounded to 16 bits before the result: the bound is that of the two products' fp32 sums, short ones here so that it is
+    small, and one half step."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(29)
+    rnd = lambda *s, by=1.0: (torch.randn(*s, generator=g) * by).to(dt)  # noqa: E731
+    x, wg, wu, wd = rnd(rows, k), rnd(f, k, by=k ** -0.5), rnd(f, k, by=k ** -0.5), rnd(o, f, by=f ** -0.5)
+    on = {n: v.cuda() for n, v in (("x", x), ("w_gate", wg), ("w_up", wu), ("w_down", wd))}
+    y = torch.empty(rows, o, dtype=dt, device="cuda")
+    plan = fc.GatedFeedForward(rows, k, f, o, dtype=dtype, ctx=lctx)
+    torch.cuda.synchronize()
+    plan.forward(at(on["x"]), at(y), **{n: at(v) for n, v in on.items() if n != "x"})
+    lctx.synchronize()
+    x, wg, wu, wd = (v.double() for v in (x, wg, wu, wd))
+    gate, up = x @ wg.t(), x @ wu.t()
+    e_gate, e_up = ((k + 4) * U * (x.abs() @ w.t().abs()) for w in (wg, wu))
+    a, e_a = act(gate, "silu")[0], act_error(gate, e_gate, "silu")[0]
+    h = a * up
+    e_h = 1.05 * (e_a * up.abs() + a.abs() * e_up + e_a * e_up) + U * h.abs()
+    check(y, h @ wd.t(), e_h @ wd.t().abs() + (f + 4) * U * (h.abs() @ wd.t().abs()), dtype, "y")
