@@ -5,9 +5,9 @@
 // once) and of every row of A, which the first-level cache holds after the first warp, and multiplies in fp32 pairs.  Shares
 // of a reduction meet in shared memory, lanes by shuffles, both in a fixed order.  For FF_GATE the four are two rows of the
 // gate's weights and the same two of the up projection's.  h stays in fp32 whatever the type: no tensor core asks for less, and
-// it is a few KB beside the weights.  One row 1024->4096->1024 in bf16, 25 MB of weights: 6.9 us
-// for both launches, 3.6 TB/s (6.3 us replayed from a graph), where tensor-core tiles of 256 rows took 23.7; 8 rows are where the multiplications
-// begin to show beside the loads.
+// it is a few KB beside the weights.  One row 1024->4096->1024 in bf16, 25 MB of weights: 6.8 to 7.1 us
+// for both launches, 3.6 TB/s (6.3 us replayed from a graph), where tensor-core tiles of 256 rows took 23.7; 8 rows are where the
+// multiplications begin to show beside the loads.
 #include <type_traits>
 
 #include "fc_gated_ff.h"

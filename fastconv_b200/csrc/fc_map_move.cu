@@ -4,7 +4,7 @@
 // One read and one write per element, nothing to compute: the bound is HBM.  A block turns a tile of 4096 elements in shared
 // memory, 64 channels x 64 pixels or, for maps of few channels, 32 x 128, 16 x 256 or 8 x 512, so that both sides see runs of
 // at least 128 bytes (of all its channels, where a pixel has fewer bytes); all loads of a thread are in flight at once.
-// 64 x 56x56x256 to bf16, 308 MB: 53 us, 5.8 TB/s, 0.88 of the measured copy rate; element by element in a loop 62 us.
+// 64 x 56x56x256 to bf16, 308 MB: 53 to 56 us, 5.5 to 5.8 TB/s, 0.84 to 0.89 of the measured copy rate; element by element in a loop 62 us.
 #include <type_traits>
 
 #include "fc_last.cuh"
